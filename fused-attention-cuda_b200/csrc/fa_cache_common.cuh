@@ -1,0 +1,95 @@
+// fa_cache_common.cuh -- device helpers shared by the paged cache's kernels.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "fa_cache.h"
+
+namespace fa_sm100 {
+
+// One sequence's part of the batch.  Everything here comes from device memory, so it is checked:
+// a value out of range is reported through the status word and replaced by one that is safe.
+struct SeqInfo {
+  int t0;    // first packed row
+  int n;     // new tokens
+  int len;   // keys held, this call's included
+};
+
+__device__ __forceinline__ void report_cache_index(const CacheView& c) {
+  atomicOr(c.status, kStCacheIndex);
+}
+
+__device__ __forceinline__ SeqInfo seq_info(const CacheView& c, int s) {
+  SeqInfo q;
+  int len = c.seq_lens[s];
+  if (c.cu_seqlens != nullptr) {
+    q.t0 = c.cu_seqlens[s];
+    const int end = c.cu_seqlens[s + 1];
+    if (q.t0 < 0 || end < q.t0 || end > c.T) {
+      report_cache_index(c);
+      q.t0 = 0;
+      q.n = 0;
+    } else {
+      q.n = end - q.t0;
+    }
+  } else {
+    q.n = c.T / c.n_seqs;
+    q.t0 = s * q.n;
+  }
+  const long long room = static_cast<long long>(c.max_pages) << c.page_shift;
+  if (len < 0 || len > room) {
+    report_cache_index(c);
+    len = len < 0 ? 0 : static_cast<int>(room);
+  }
+  q.len = len;
+  return q;
+}
+
+// Packed rows that belong to a sequence; the rows from here to T are behind the last one.
+__device__ __forceinline__ int live_rows(const CacheView& c) {
+  if (c.cu_seqlens == nullptr) return c.T;
+  const int end = c.cu_seqlens[c.n_seqs];
+  return end < 0 ? 0 : (end > c.T ? c.T : end);
+}
+
+// The page of sequence s that holds its keys [i << page_shift, ...), or -1 (reported).
+__device__ __forceinline__ int page_of(const CacheView& c, int s, int i) {
+  if (i < 0 || i >= c.max_pages) {
+    report_cache_index(c);
+    return -1;
+  }
+  const int p = c.block_table[static_cast<long long>(s) * c.table_stride + i];
+  if (p < 0 || p >= c.num_pages) {
+    report_cache_index(c);
+    return -1;
+  }
+  return p;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 to_float2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 to_float2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<__half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 to_float2<__nv_bfloat16>(uint32_t u) {
+  return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t from_float2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t from_float2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t from_float2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+}  // namespace fa_sm100

@@ -75,6 +75,7 @@
 
 #include "fa_fwd_lookahead.cuh"
 #include "fa_kernel_common.cuh"
+#include "fa_cache.h"
 #include "fa_launch.h"
 #include "fa_sm100.h"
 #include "sm100_ptx.cuh"
@@ -1005,7 +1006,14 @@ cudaError_t read_and_clear_status(unsigned int* bits) {
   if (bits != nullptr) *bits = v;
   if (e != cudaSuccess) return e;
   if (v == 0) return cudaSuccess;
-  return (v & kStBounds) != 0 ? cudaErrorAssert : cudaErrorLaunchTimeout;
+  if ((v & kStBounds) != 0) return cudaErrorAssert;
+  return (v & ~kStCacheIndex) != 0 ? cudaErrorLaunchTimeout : cudaErrorInvalidValue;
+}
+
+unsigned* status_word(cudaError_t* err) {
+  void* p = nullptr;
+  *err = cudaGetSymbolAddress(&p, g_status);
+  return static_cast<unsigned*>(p);
 }
 
 }  // namespace fa_sm100

@@ -7,6 +7,8 @@ functions, same validation messages.  The ops (registered by ``fused_attn._C``):
     torch.ops.fused_attn.forward_stage(q, k, v, is_causal, scale, stage) -> (O, LSE)
     torch.ops.fused_attn.forward_strided(q, k, v, is_causal, scale) -> (O, LSE)   [B200 addition]
     torch.ops.fused_attn.combine(o_parts, lse_parts) -> (O, LSE)                 [B200 addition]
+    torch.ops.fused_attn.cache_append(q, k, v, k_cache, ...) -> q rotated        [B200 addition]
+    torch.ops.fused_attn.cache_attention(q, k_cache, ...) -> (O, LSE)            [B200 addition]
     torch.ops.fused_attn.set_debug_overrides(block_m, block_n) -> ()
     torch.ops.fused_attn.impl_supports(stage, dtype_name, D) -> bool
     torch.ops.fused_attn.impl_name(stage) -> str
@@ -28,6 +30,8 @@ from . import abi, ops, workloads
 __all__ = [
     "__version__",
     "abi",
+    "cache_append",
+    "cache_attention",
     "combine",
     "debug_set_skip_kv_tile",
     "forward",
@@ -116,6 +120,55 @@ def combine(o_parts, lse_parts) -> tuple[Tensor, Tensor]:
     """
     _require_ext()
     return torch.ops.fused_attn.combine(list(o_parts), list(lse_parts))
+
+
+def cache_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor,
+                 v_scale: Tensor, block_table: Tensor, seq_lens: Tensor,
+                 cu_seqlens: Tensor | None = None, q: Tensor | None = None,
+                 cos: Tensor | None = None, sin: Tensor | None = None,
+                 interleaved: bool = False) -> Tensor | None:
+    """Write new tokens into a paged 8-bit key/value cache, rotating k (and q) by position.
+
+    The cache: ``k_cache`` / ``v_cache`` float8_e4m3fn [pages, Hkv, page_size, D] views (D 64 or
+    128 and contiguous, page_size 16..128; a token-major pool is passed as ``pool.transpose(1, 2)``)
+    and one scale for each page and kv head, ``k_scale`` / ``v_scale`` float32 [pages, Hkv]:
+    value = e4m3 * scale.  ``block_table`` int32 [S, max_pages] lists each sequence's pages,
+    ``seq_lens`` int32 [S] the keys it holds AFTER this call.
+
+    ``k``, ``v`` [T, Hkv, D] (fp16 / bf16 views) hold the sequences' last tokens, packed;
+    ``cu_seqlens`` int32 [S + 1] are their offsets (None: T / S for each).  ``cos`` / ``sin``
+    float32 [positions, rot_dim / 2] rotate the first rot_dim elements of each head, in pairs
+    (j, j + rot_dim / 2) or, ``interleaved``, (2j, 2j + 1); None stores k as it is.  With ``q``
+    [T, H, D] the rotated q is returned (zeros in rows behind the last sequence), else None.
+
+    Scales are powers of two, the least that hold a page's largest magnitude (448 * scale).  A page
+    that held earlier tokens keeps them: its scale only grows, and where it does they are rounded
+    to the new step.  Values that are not finite are stored as NaN.  Two sequences must not append
+    to one page in one call.  Pages, lengths, offsets and positions live on the device and are
+    checked there: what is out of range is skipped and reported by ``last_device_error`` as (1, bits).
+    """
+    _require_ext()
+    out = torch.ops.fused_attn.cache_append(q, k, v, k_cache, v_cache, k_scale, v_scale,
+                                            block_table, seq_lens, cu_seqlens, cos, sin,
+                                            bool(interleaved))
+    return out if q is not None else None
+
+
+def cache_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor,
+                    block_table: Tensor, seq_lens: Tensor, cu_seqlens: Tensor | None = None,
+                    is_causal: bool = True, scale: float | None = None, return_lse: bool = False):
+    """Attention of packed new tokens ``q`` [T, H, D] over the cache that ``cache_append`` fills
+    (same cache, table, lengths and offsets).  A sequence's n tokens are its last ones: query i
+    sees the keys j <= seq_len - n + i, or all seq_len of them without ``is_causal``.  One token
+    for each sequence is a decoding step, a whole prompt or a chunk of one a prefill step; a batch
+    may mix them.  Returns ``o`` [T, H, D], or ``(o, lse)`` with lse float32 [T, H]; a query
+    without a key gets o = 0 and lse = +inf, rows behind the last sequence are zero.  As
+    [T, H, 1, D] and [T, H, 1], (o, lse) is a partial for ``combine``."""
+    _require_ext()
+    o, lse = torch.ops.fused_attn.cache_attention(q, k_cache, v_cache, k_scale, v_scale,
+                                                  block_table, seq_lens, cu_seqlens,
+                                                  bool(is_causal), _resolve_scale(q, scale))
+    return (o, lse) if return_lse else o
 
 
 def forward_stage(q: Tensor, k: Tensor, v: Tensor, stage: int, is_causal: bool = False,

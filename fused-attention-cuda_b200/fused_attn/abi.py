@@ -22,6 +22,9 @@ EXPORTS = (
     "fa_combine",
     "fa_forward_noalloc",
     "fa_noalloc_scratch_bytes",
+    "fa_cache_append",
+    "fa_cache_attention",
+    "fa_cache_attention_workspace_bytes",
     "fa_workspace_bytes",
     "fa_impl_supports",
     "fa_set_debug_overrides",
@@ -64,6 +67,30 @@ class FaStrides(ctypes.Structure):
                 ("v", ctypes.c_longlong * 3), ("o", ctypes.c_longlong * 3)]
 
 
+class FaCache(ctypes.Structure):
+    """``fa_cache_t``: pages, scales, block table, lengths and offsets of a paged 8-bit cache."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("num_pages", ctypes.c_longlong),
+                ("page_size", ctypes.c_int), ("Hkv", ctypes.c_int), ("D", ctypes.c_int),
+                ("k_strides", ctypes.c_longlong * 3), ("v_strides", ctypes.c_longlong * 3),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_longlong),
+                ("max_pages", ctypes.c_int), ("seq_lens", ctypes.c_void_p),
+                ("cu_seqlens", ctypes.c_void_p), ("n_seqs", ctypes.c_int)]
+
+
+class FaAppend(ctypes.Structure):
+    """``fa_append_t``: the new tokens of ``fa_cache_append`` and their rotation."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_strides", ctypes.c_longlong * 2), ("v_strides", ctypes.c_longlong * 2),
+                ("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+                ("q_strides", ctypes.c_longlong * 2), ("H", ctypes.c_int),
+                ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
+                ("table_rows", ctypes.c_longlong), ("rot_dim", ctypes.c_int),
+                ("interleaved", ctypes.c_int)]
+
+
 _lib: ctypes.CDLL | None = None
 
 
@@ -99,6 +126,14 @@ def configure(L: ctypes.CDLL) -> ctypes.CDLL:
     L.fa_forward_noalloc.restype = i
     L.fa_noalloc_scratch_bytes.argtypes = []
     L.fa_noalloc_scratch_bytes.restype = ctypes.c_size_t
+    L.fa_cache_append.argtypes = [i, ctypes.POINTER(FaCache), ctypes.POINTER(FaAppend), i, vp]
+    L.fa_cache_append.restype = i
+    L.fa_cache_attention.argtypes = [i, ctypes.POINTER(FaCache), vp,
+                                     ctypes.POINTER(ctypes.c_longlong), vp, vp, vp, i, i,
+                                     ctypes.c_float, i, vp]
+    L.fa_cache_attention.restype = i
+    L.fa_cache_attention_workspace_bytes.argtypes = [ctypes.POINTER(FaCache), i, i]
+    L.fa_cache_attention_workspace_bytes.restype = ctypes.c_size_t
     L.fa_workspace_bytes.argtypes = [i, i, ctypes.POINTER(FaParams)]
     L.fa_workspace_bytes.restype = ctypes.c_size_t
     L.fa_impl_supports.argtypes = [i, i, i, i]
@@ -167,6 +202,30 @@ def forward_noalloc(impl: int, dtype: int, q: int, k: int, v: int, o: int, lse: 
 
 def noalloc_scratch_bytes() -> int:
     return int(lib().fa_noalloc_scratch_bytes())
+
+
+def _ref(struct):
+    return ctypes.byref(struct) if struct is not None else None
+
+
+def cache_append(dtype: int, cache: FaCache | None, new: FaAppend | None, T: int,
+                 stream: int = 0) -> int:
+    """Raw ``fa_cache_append``; returns the cudaError_t value."""
+    return int(lib().fa_cache_append(dtype, _ref(cache), _ref(new), T, stream or None))
+
+
+def cache_attention(dtype: int, cache: FaCache | None, q: int, q_strides: tuple[int, int], o: int,
+                    lse: int, workspace: int, T: int, H: int, scale: float, causal: bool,
+                    stream: int = 0) -> int:
+    """Raw ``fa_cache_attention`` on device pointers; returns the cudaError_t value."""
+    st = (ctypes.c_longlong * 2)(*q_strides)
+    return int(lib().fa_cache_attention(dtype, _ref(cache), q or None, st, o or None, lse or None,
+                                        workspace or None, T, H, scale, 1 if causal else 0,
+                                        stream or None))
+
+
+def cache_attention_workspace_bytes(cache: FaCache | None, H: int, T: int) -> int:
+    return int(lib().fa_cache_attention_workspace_bytes(_ref(cache), H, T))
 
 
 COMBINE_MAX_SPLITS = 64

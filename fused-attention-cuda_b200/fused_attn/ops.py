@@ -56,6 +56,39 @@ def _fake_combine(o_parts, lse_parts):
         o0.new_empty((b, h, n), dtype=torch.float32)
 
 
+def _check_cache(k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor,
+                 block_table: Tensor, seq_lens: Tensor, cu_seqlens: Tensor | None) -> None:
+    torch._check(k_cache.dim() == 4 and v_cache.dim() == 4,
+                 lambda: "k_cache and v_cache must be [pages, Hkv, page_size, D]")
+    torch._check(k_cache.dtype == torch.float8_e4m3fn and v_cache.dtype == torch.float8_e4m3fn,
+                 lambda: "k_cache and v_cache must be float8_e4m3fn")
+    d = k_cache.shape[3]
+    torch._check(d == 64 or d == 128, lambda: f"D must be 64 or 128, got {d}")
+    torch._check(k_scale.dim() == 2 and v_scale.dim() == 2,
+                 lambda: "k_scale and v_scale must be [pages, Hkv]")
+    torch._check(block_table.dim() == 2 and seq_lens.dim() == 1,
+                 lambda: "block_table must be [sequences, max_pages], seq_lens [sequences]")
+    torch._check(cu_seqlens is None or cu_seqlens.dim() == 1, lambda: "cu_seqlens must be 1-D")
+
+
+def _fake_cache_append(q, k, v, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
+                       cu_seqlens, cos, sin, interleaved):
+    _check_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens)
+    torch._check(k.dim() == 3 and v.dim() == 3, lambda: "k and v must be [T, heads, D]")
+    torch._check((cos is None) == (sin is None), lambda: "cos and sin come together")
+    if q is None:
+        return k.new_empty((0,))
+    torch._check(cos is not None, lambda: "q is rotated and needs cos and sin")
+    return q.new_empty(q.shape)
+
+
+def _fake_cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
+                          cu_seqlens, is_causal, scale):
+    _check_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, cu_seqlens)
+    torch._check(q.dim() == 3, lambda: "q must be [T, heads, D]")
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 def _fake_forward_stage(q: Tensor, k: Tensor, v: Tensor, is_causal: bool, scale: float, stage: int):
     _check_inputs(q, k, v)
     torch._check(1 <= stage <= 5, lambda: f"stage must be in 1..5, got {stage}")
@@ -77,6 +110,8 @@ def register_fakes() -> None:
     torch.library.register_fake("fused_attn::forward_stage", _fake_forward_stage)
     torch.library.register_fake("fused_attn::forward_strided", _fake_forward_strided)
     torch.library.register_fake("fused_attn::combine", _fake_combine)
+    torch.library.register_fake("fused_attn::cache_append", _fake_cache_append)
+    torch.library.register_fake("fused_attn::cache_attention", _fake_cache_attention)
     _registered = True
 
 

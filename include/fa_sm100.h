@@ -115,6 +115,81 @@ int fa_forward_noalloc(int impl, int dtype, const void* q, const void* k, const 
 /* Size of that scratch array in bytes (FA_NOALLOC_SCRATCH_BYTES). */
 size_t fa_noalloc_scratch_bytes(void);
 
+/* No counterpart in the reference: a key/value cache in pages, held in 8 bits (e4m3).
+ *
+ * Keys and values live in num_pages pages of page_size tokens (16, 32, 64 or 128) each, for every
+ * kv head D e4m3 values a token; k_scale / v_scale [num_pages, Hkv] (fp32, contiguous) hold one
+ * scale for each page and kv head, value = e4m3 * scale.  fa_cache_append writes powers of two in
+ * [2^-64, 2^120]; fa_cache_attention takes any positive finite scale.  k_strides / v_strides are
+ * the byte strides of (page, kv head, token), positive multiples of 16; d is contiguous.
+ *
+ * block_table [n_seqs, max_pages] (rows table_stride apart) lists each sequence's pages in order,
+ * seq_lens [n_seqs] the keys that each holds, those of the current call included.  The current
+ * call's T packed tokens are split by cu_seqlens [n_seqs + 1] (NULL: T / n_seqs each) and are the
+ * last ones of their sequences: new token i of n sits at position len - n + i.  These arrays live
+ * in device memory and are checked there: a page, length, offset or position out of range is
+ * skipped and reported by fa_last_device_error (cudaErrorInvalidValue), never followed.  Entries
+ * of block_table behind a sequence's last page are not read.  Rows of the packed tensors behind
+ * cu_seqlens[n_seqs] belong to no sequence: nothing is stored for them, and outputs get zeros. */
+typedef struct fa_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  long long num_pages;
+  int page_size;
+  int Hkv;
+  int D; /* 64 or 128 */
+  long long k_strides[3];
+  long long v_strides[3];
+  const int* block_table;
+  long long table_stride;
+  int max_pages;
+  const int* seq_lens;
+  const int* cu_seqlens;
+  int n_seqs;
+} fa_cache_t;
+
+/* The tokens that fa_cache_append adds: k, v [T, Hkv, D] and, to be rotated likewise, q [T, H, D]
+ * (or NULL) with its contiguous output q_out; element strides of (token, head), multiples of 16
+ * bytes.  cos, sin [table_rows, rot_dim / 2] (fp32, contiguous, by position) rotate the first
+ * rot_dim (a multiple of 16) elements of each head, in pairs (j, j + rot_dim / 2), or (2j, 2j + 1)
+ * when interleaved; both NULL: no rotation, and q must be NULL. */
+typedef struct fa_append {
+  const void* k;
+  const void* v;
+  long long k_strides[2];
+  long long v_strides[2];
+  const void* q;
+  void* q_out;
+  long long q_strides[2];
+  int H;
+  const float* cos;
+  const float* sin;
+  long long table_rows;
+  int rot_dim;
+  int interleaved;
+} fa_append_t;
+
+/* Writes T new tokens (fp16 or bf16) into their pages.  A page whose first new token is not its
+ * first slot keeps its earlier rows: its scale only grows, and where it does they are rounded to
+ * the new step; rows behind the last token stay as they are.  Stored values are the rotated ones
+ * rounded once, to nearest even; values that are not finite are stored as NaN.  Two sequences must
+ * not append to one page in one call.  q_out must not overlap q. */
+int fa_cache_append(int dtype, const fa_cache_t* cache, const fa_append_t* p, int T,
+                    cudaStream_t stream);
+
+/* Attention of T new query rows q [T, H, D] (fp16 or bf16, H % Hkv == 0, element strides of
+ * (token, head)) over the cache; o [T, H, D] (contiguous, q's type) and lse [T, H] (fp32, natural
+ * log) are written.  causal: a query sees the keys up to its own position; else all of its
+ * sequence's.  A query without a key gets o = 0, lse = +inf.  `workspace` (16-byte aligned) holds
+ * fa_cache_attention_workspace_bytes(cache, H, T) bytes, belongs to this call until it has run, and
+ * needs no initial value. */
+size_t fa_cache_attention_workspace_bytes(const fa_cache_t* cache, int H, int T);
+int fa_cache_attention(int dtype, const fa_cache_t* cache, const void* q,
+                       const long long* q_strides, void* o, float* lse, void* workspace, int T,
+                       int H, float scale, int causal, cudaStream_t stream);
+
 /* fa::workspace_bytes (attention.cuh:51; src/dispatch.cu:163-168).  0 for fp16/bf16.  For fp32
  * (FA_IMPL_FUSED, tf32 tensor cores) 4*D*N*(B*H + 2*B*Hkv) bytes: q, k and v rounded to tf32
  * (round to nearest) before the kernel reads them, instead of the tensor core's truncation. */
