@@ -37,10 +37,11 @@ __device__ __forceinline__ float finite_or_nan(float x) {
   return fabsf(x) < INFINITY ? x : __int_as_float(0x7fffffff);
 }
 
-// The least e in [kMinExp, kMaxExp] with a <= 448 * 2^e, a >= 0 finite.  448 = 1.75 * 2^8.
-__device__ __forceinline__ int needed_exp(float a) {
+// The least e in [kMinExp, kMaxExp] with a * 2^up <= 448 * 2^e, a >= 0 finite.  448 = 1.75 * 2^8.
+__device__ __forceinline__ int needed_exp(float a, int up) {
   const unsigned bits = __float_as_uint(a);
-  const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  const int e =
+      static_cast<int>(bits >> 23) - 127 - 8 + up + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return max(kMinExp, min(kMaxExp, e));
 }
 
@@ -104,14 +105,17 @@ struct Angles {
   float c[8], s[8];
 };
 
-__device__ __forceinline__ void load_angles(Angles& a, const AppendArgs& p, int pos, int col) {
+__device__ __forceinline__ void load_angles(Angles& a, const AppendArgs& p, int pos, int col,
+                                            float mul) {
   const long long at = static_cast<long long>(pos) * (p.rot_dim / 2) + col;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at) + i);
     const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + at) + i);
-    a.c[4 * i] = c.x, a.c[4 * i + 1] = c.y, a.c[4 * i + 2] = c.z, a.c[4 * i + 3] = c.w;
-    a.s[4 * i] = s.x, a.s[4 * i + 1] = s.y, a.s[4 * i + 2] = s.z, a.s[4 * i + 3] = s.w;
+    a.c[4 * i] = c.x * mul, a.c[4 * i + 1] = c.y * mul;
+    a.c[4 * i + 2] = c.z * mul, a.c[4 * i + 3] = c.w * mul;
+    a.s[4 * i] = s.x * mul, a.s[4 * i + 1] = s.y * mul;
+    a.s[4 * i + 2] = s.z * mul, a.s[4 * i + 3] = s.w * mul;
   }
 }
 
@@ -232,7 +236,7 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
   active = active && page >= 0;
   if (!active) b = a;
   const int rot = !is_v && p.cos != nullptr ? p.rot_dim : 0;
-  if (rot > 0 && active && page_pos + b > p.table_rows) {
+  if (p.cos != nullptr && active && page_pos + b > p.table_rows) {
     report_cache_index(c);  // positions that the table does not have are not stored
     const long long rows = p.table_rows - page_pos;
     b = rows > a ? static_cast<int>(rows) : a;
@@ -245,14 +249,24 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
   const long long* st = is_v ? p.sv : p.sk;
   const T* base = src + (t0 + page_pos - begin) * st[0] + head * st[1];  // of slot 0
 
+  // Two bf16 values near the type's largest can rotate past the range of 32 bits: rotated rows are
+  // held at half their size.
+  const int up = rot > 0 ? 1 : 0;
+  const float half = rot > 0 ? 0.5f : 1.f;
   float x[kKeep][8], y[kKeep][8];
   float amax = 0.f;
   auto fetch = [&](int slot, float(&fx)[8], float(&fy)[8]) {
     load_unit<T>(fx, fy, base + slot * st[0], u);
     if (u.angle >= 0) {
       Angles an;
-      load_angles(an, p, static_cast<int>(page_pos) + slot, u.angle);
+      load_angles(an, p, static_cast<int>(page_pos) + slot, u.angle, half);
       rotate_unit(fx, fy, an, p.interleaved);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        fx[i] *= half;
+        fy[i] *= half;
+      }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -282,16 +296,16 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
     for (int i = 1; i < WARPS; ++i) amax = fmaxf(amax, red[i]);
   }
   if (!active) return;
-  int e = needed_exp(amax);
+  int e = needed_exp(amax, up);
   if (a > 0) e = max(e, stored_exp(old));
   const float now = pow2f(e);
-  const float mul = pow2f(-e);
+  const float mul = pow2f(up - e);
   unsigned char* dst = (is_v ? c.v : c.k) + page * (is_v ? c.vs[0] : c.ks[0]) +
                        head * (is_v ? c.vs[1] : c.ks[1]);
   const long long dt = is_v ? c.vs[2] : c.ks[2];
   if (tid == 0) *scale = now;
   if (a > 0 && old != now) {  // earlier rows follow the page's scale
-    const float ratio = old * mul;
+    const float ratio = old * pow2f(-e);
     const int col = (tid % kLanes) * 16;
     for (int slot = row; slot < a; slot += kRows) {
       uint4* at = reinterpret_cast<uint4*>(dst + slot * dt + col);
@@ -350,7 +364,7 @@ __device__ void rotate_q(const AppendArgs& p, const Grid& g, long long group, in
   }
   const Unit u = unit_of(lane % kLanes, p.rot_dim, p.interleaved);
   Angles an;
-  if (pos >= 0 && u.angle >= 0) load_angles(an, p, pos, u.angle);
+  if (pos >= 0 && u.angle >= 0) load_angles(an, p, pos, u.angle, 1.f);
   const T* src = static_cast<const T*>(p.q) + t * p.sq[0];
   T* dst = static_cast<T*>(p.q_out) + static_cast<long long>(t) * p.H * D;
   const int h1 = min(p.H, h0 + g.q_heads);
