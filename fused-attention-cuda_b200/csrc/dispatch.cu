@@ -190,6 +190,8 @@ const char* check_strides(const long long st[3], size_t eb, const char* name) {
 
 namespace fa_sm100 {
 
+unsigned long long wait_timeout_ns() { return g_timeout_ns; }
+
 // Every check fa_forward makes before it launches, in its order and with its error codes:
 // parameters, strides (when given), the implementation on the current device, the workspace.
 cudaError_t check_forward_args(int impl, int dtype, const void* q, const void* k, const void* v,

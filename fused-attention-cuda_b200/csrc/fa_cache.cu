@@ -90,7 +90,64 @@ cudaError_t check_device() {
   return major == 10 && minor == 0 ? cudaSuccess : cudaErrorNotSupported;
 }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      return nullptr;
+    }
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+cudaError_t page_map(CUtensorMap* m, int* pos, void* base, const long long st[3],
+                     const CacheView& c, int D, int rows) {
+  const EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return cudaErrorNotSupported;
+  const long long stride[3] = {st[2], st[1], st[0]};  // token, head, page
+  const long long size[3] = {1ll << c.page_shift, c.Hkv, c.num_pages};
+  int order[3] = {0, 1, 2};
+  for (int i = 1; i < 3; ++i) {
+    for (int j = i; j > 0 && stride[order[j]] < stride[order[j - 1]]; --j) {
+      const int t = order[j];
+      order[j] = order[j - 1];
+      order[j - 1] = t;
+    }
+  }
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), 0, 0, 0};
+  cuuint64_t strides[3];
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(D), 1u, 1u, 1u};
+  *pos = 0;
+  for (int i = 0; i < 3; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(size[order[i]]);
+    strides[i] = static_cast<cuuint64_t>(stride[order[i]]);
+    if (order[i] == 0) box[i + 1] = static_cast<cuuint32_t>(rows);
+    *pos |= i << (2 * order[i]);
+  }
+  const cuuint32_t estride[4] = {1u, 1u, 1u, 1u};
+  const CUresult r =
+      enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, estride,
+          CU_TENSOR_MAP_INTERLEAVE_NONE,
+          D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 }  // namespace
+
+cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows) {
+  const cudaError_t e = page_map(&m->k, &m->k_pos, c.k, c.ks, c, D, rows);
+  return e != cudaSuccess ? e : page_map(&m->v, &m->v_pos, c.v, c.vs, c, D, rows);
+}
 
 int multiprocessors() {
   int dev = 0, sms = 0;
@@ -195,6 +252,6 @@ extern "C" int fa_cache_attention(int dtype, const fa_cache_t* c, const void* q,
   a.scale = scale;
   a.causal = causal != 0;
   a.workspace = workspace;
-  a.timeout_ns = 0;
+  a.timeout_ns = wait_timeout_ns();
   return launch_cache_attention(a, stream);
 }

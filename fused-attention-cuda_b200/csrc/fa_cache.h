@@ -2,6 +2,7 @@
 // its kernels (fa_cache_append.cu, fa_cache_attn.cu).  Not part of the public ABI.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -63,6 +64,15 @@ struct CacheAttnArgs {
 cudaError_t launch_cache_append(const AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
 size_t cache_attention_workspace(int H, int Hkv, int D, int T, int n_seqs, int sms);
+
+// Tensor maps of the pages {d, token, kv head, page}, the last three ordered by stride; `pos` packs
+// (two bits each) which of the map's dimensions 1-3 holds token, head and page.
+struct PageMaps {
+  CUtensorMap k, v;
+  int k_pos, v_pos;
+};
+// Boxes of `rows` tokens, swizzled by the row's D bytes.
+cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows);
 
 // Multiprocessors of the current device (148 when the query fails).
 int multiprocessors();

@@ -27,7 +27,8 @@ constexpr int kRun = 16;    // keys that a warp takes at a time; never more than
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = kRun * kWarps;  // keys of one unit of work
-constexpr int kStages = 6;            // runs in flight for each warp
+constexpr int kStages = 4;            // runs in flight for each warp
+constexpr int kPerSm = 3;             // CTAs on a multiprocessor
 constexpr float kLazy = 8.0f;         // the running maximum follows once it is off by 2^8
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -40,7 +41,8 @@ struct Layout {
   static constexpr int kMerge = kWarps * kRows * D * 4;  // reuses the ring
   static constexpr int kMain = kRing > kMerge ? kRing : kMerge;
   static constexpr int kScale = kWarps * kStages * 16;
-  static constexpr int kBytes = kMain + kScale;
+  static constexpr int kBars = kWarps * kStages * 8;
+  static constexpr int kBytes = kMain + kScale + kBars + 1024;  // the ring starts on 1024 bytes
 };
 
 // A partial result: kRows x D sums, then (m, l) of each row.
@@ -133,15 +135,17 @@ struct Finder {
   }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(on ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Bounded wait for a phase of this warp's copies; false when the time limit ran out (reported).
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, const CacheAttnArgs& a) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (globaltimer_ns() - t0 > a.timeout_ns) {
+      atomicOr(a.c.status, kStKFull);
+      return false;
+    }
+  }
+  return true;
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -160,10 +164,15 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
 
 // Two e4m3 values (the low or high half of u) as fp16.
 __device__ __forceinline__ uint32_t e4m3_lo(uint32_t u) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<unsigned short>(u), __NV_E4M3);
-  return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(u));
+  return r;
 }
-__device__ __forceinline__ uint32_t e4m3_hi(uint32_t u) { return e4m3_lo(u >> 16); }
+__device__ __forceinline__ uint32_t e4m3_hi(uint32_t u) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(u));
+  return r;
+}
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
@@ -190,15 +199,34 @@ __device__ __forceinline__ void value_scale(float s, float* add, float* inv) {
   *inv = 1.0f / s;
 }
 
+// Copies 16 keys of a page and head to shared memory, 128- or 64-byte swizzled (a row's 16-byte piece
+// p lies at p ^ (row & 7), or p ^ ((row >> 1) & 3) for rows of 64 bytes).
+__device__ __forceinline__ void load_page(uint32_t dst, const void* map, int pos, int slot, int head,
+                                          int page, uint32_t bar) {
+  const int pt = pos & 3, ph = (pos >> 2) & 3;
+  const int c0 = pt == 0 ? slot : (ph == 0 ? head : page);
+  const int c1 = pt == 1 ? slot : (ph == 1 ? head : page);
+  const int c2 = pt == 2 ? slot : (ph == 2 ? head : page);
+  tma_load_4d(dst, map, 0, c0, c1, c2, bar);
+}
+
+// The 16-byte pieces of a K row that lane column cq multiplies: neighbours, so that the eight lanes
+// of a shared-memory phase (two rows) read all eight pieces.
+template <int D>
+__device__ __forceinline__ int k_piece(int cq, int p) {
+  return (D / 64) * cq + p;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
-    const __grid_constant__ CacheAttnArgs a, float* partials) {
+__global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
+    const __grid_constant__ CacheAttnArgs a, const __grid_constant__ PageMaps maps,
+    float* partials) {
   using L = Layout<D>;
   constexpr int kSteps = D / 16;       // products of 16 along D
   constexpr int kWords = D / 16;       // 4-byte words of a K row that a lane holds
   constexpr int kPieces = D / 16;      // 16-byte pieces of a row
-  constexpr int kCopies = kRun * kPieces / 32;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ Finder<kThreads> finder;
   __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
 
@@ -222,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
 
   const long long total = finder.total(c, group);
   const int ctas = ctas_of(total);
-  if (blockIdx.x >= ctas) return;
+  if (blockIdx.x >= static_cast<unsigned>(ctas)) return;
   const long long u_begin = bound_of(total, blockIdx.x, ctas);
   const long long u_end = bound_of(total, blockIdx.x + 1, ctas);
   finder.find(c, group, u_begin);
@@ -231,7 +259,16 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
 
   const uint32_t ring = smem_u32(smem) + warp * kStages * L::kStage;
   RunScale* scales = reinterpret_cast<RunScale*>(smem + L::kMain) + warp * kStages;
+  const uint32_t bars = smem_u32(smem) + L::kMain + L::kScale + warp * kStages * 8;
   const int page_mask = (1 << c.page_shift) - 1;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  unsigned sent = 0, taken = 0;  // runs that this warp has issued and used, over all parts
+  bool alive = true;             // false once a wait ran out: nothing more is issued or used
 
   for (long long u = u_begin; u < u_end;) {
     SeqWork w = seq_work(c, s, group);
@@ -263,7 +300,7 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
       uint32_t raw[kSteps][2];
 #pragma unroll
       for (int p = 0; p < kSteps / 4; ++p) {
-        const uint4* at = reinterpret_cast<const uint4*>(src + 16 * (cq + 4 * p));
+        const uint4* at = reinterpret_cast<const uint4*>(src + 16 * k_piece<D>(cq, p));
         const uint4 v0 = on ? __ldg(at) : make_uint4(0, 0, 0, 0);
         const uint4 v1 = on ? __ldg(at + 1) : make_uint4(0, 0, 0, 0);
         const uint32_t f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
@@ -337,33 +374,26 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
     int issued = 0;
     auto issue = [&]() {
       const int i = issued++;
-      if (i < n_runs) {
-        if (i > 0 && (i & 31) == 0) {
-          now = next;
-          next = look_up(i + 32 + lane);
-        }
-        const int stage = i % kStages;
-        const int page = __shfl_sync(0xffffffffu, now.page, i & 31);
-        if (lane == (i & 31)) scales[stage] = now.sc;
-        const int key = first_key + i * kTile;
-        const uint32_t dst = ring + stage * L::kStage;
-        const int slot = key & page_mask;
-        const long long pg = page < 0 ? 0 : page;
-        const unsigned char* k = c.k + pg * c.ks[0] + head * c.ks[1] + slot * c.ks[2];
-        const unsigned char* v = c.v + pg * c.vs[0] + head * c.vs[1] + slot * c.vs[2];
-#pragma unroll
-        for (int j = 0; j < kCopies; ++j) {
-          const int at = lane + 32 * j;
-          const int row = at / kPieces, piece = at % kPieces;
-          // Rows behind the last key are filled with zeros: a page's tail holds anything.
-          const bool on = page >= 0 && key + row < w.q.len;
-          const int ks = D == 128 ? piece ^ (4 * (row & 1)) : piece;
-          const int vs = D == 128 ? piece ^ (row & 6) : piece ^ ((row >> 1) & 3);
-          cp_async16(dst + row * D + ks * 16, k + row * c.ks[2] + piece * 16, on);
-          cp_async16(dst + L::kHalf + row * D + vs * 16, v + row * c.vs[2] + piece * 16, on);
+      if (i >= n_runs || !alive) return;
+      if (i > 0 && (i & 31) == 0) {
+        now = next;
+        next = look_up(i + 32 + lane);
+      }
+      const int stage = sent % kStages;
+      ++sent;
+      const int page = __shfl_sync(0xffffffffu, now.page, i & 31);
+      if (lane == (i & 31)) scales[stage] = now.sc;
+      if (lane == 0) {
+        const uint32_t bar = bars + 8 * stage, dst = ring + stage * L::kStage;
+        if (page >= 0) {
+          const int slot = (first_key + i * kTile) & page_mask;
+          mbar_arrive_expect_tx(bar, L::kStage);
+          load_page(dst, &maps.k, maps.k_pos, slot, head, page, bar);
+          load_page(dst + L::kHalf, &maps.v, maps.v_pos, slot, head, page, bar);
+        } else {
+          mbar_arrive(bar);
         }
       }
-      cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue();
@@ -377,29 +407,31 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     for (int i = 0; i < n_runs; ++i) {
-      cp_async_wait<kStages - 2>();
-      __syncwarp();
-      issue();
-      const int stage = i % kStages;
+      const int stage = taken % kStages;
+      if (alive) alive = wait_copy(bars + 8 * stage, (taken / kStages) & 1, a);
+      alive = __all_sync(0xffffffffu, alive);
+      if (!alive) break;
+      ++taken;
+      issue();  // into the stage that every lane left before the vote
       const uint32_t kb = ring + stage * L::kStage;
       const uint32_t vb = kb + L::kHalf;
       const RunScale sc = scales[stage];
 
-      float sacc[2][4];
+      float sacc[2][2][4] = {};  // [8 keys][even, odd steps]: shorter chains of products
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
-        sacc[nt][0] = sacc[nt][1] = sacc[nt][2] = sacc[nt][3] = 0.f;
         const int key = nt * 8 + r;
         uint32_t kw[kWords];
 #pragma unroll
         for (int p = 0; p < kPieces / 4; ++p) {
-          const int piece = cq + 4 * p;
-          const uint4 v =
-              lds128(kb + key * D + (D == 128 ? piece ^ (4 * (key & 1)) : piece) * 16);
+          const int piece = k_piece<D>(cq, p);
+          const uint4 v = lds128(kb + key * D + (D == 128 ? piece ^ r : piece ^ ((r >> 1) & 3)) * 16);
           kw[4 * p] = v.x, kw[4 * p + 1] = v.y, kw[4 * p + 2] = v.z, kw[4 * p + 3] = v.w;
         }
 #pragma unroll
-        for (int t = 0; t < kSteps; ++t) mma_f16(sacc[nt], qf[t], e4m3_lo(kw[t]), e4m3_hi(kw[t]));
+        for (int t = 0; t < kSteps; ++t) {
+          mma_f16(sacc[nt][t & 1], qf[t], e4m3_lo(kw[t]), e4m3_hi(kw[t]));
+        }
       }
 
       float mul[2] = {sc.mul * row_mul[0], sc.mul * row_mul[1]};
@@ -408,7 +440,7 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
       for (int nt = 0; nt < 2; ++nt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          t[e >> 1][nt * 2 + (e & 1)] = fmaf(sacc[nt][e], mul[e >> 1], sc.add);
+          t[e >> 1][nt * 2 + (e & 1)] = fmaf(sacc[nt][0][e] + sacc[nt][1][e], mul[e >> 1], sc.add);
         }
       }
       const int key0 = first_key + i * kTile;
@@ -464,11 +496,20 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
       for (int k = 0; k < 4; ++k) {
         const int key = 2 * cq + (k & 1) + 8 * (k >> 1);
         if constexpr (D == 128) {
-          const uint4 v = lds128(vb + key * D + (r ^ (key & 6)) * 16);
+          const uint4 v = lds128(vb + key * D + (r ^ (key & 7)) * 16);
           vw[k][0] = v.x, vw[k][1] = v.y, vw[k][2] = v.z, vw[k][3] = v.w;
         } else {
           const uint2 v = lds64(vb + key * D + ((r >> 1) ^ ((key >> 1) & 3)) * 16 + (r & 1) * 8);
           vw[k][0] = v.x, vw[k][1] = v.y;
+        }
+      }
+      if (key0 + kRun > w.q.len || !sc.present) {  // behind the last key a page holds anything
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (key0 + 2 * cq + (k & 1) + 8 * (k >> 1) >= w.q.len || !sc.present) {
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) vw[k][j] = 0;
+          }
         }
       }
 #pragma unroll
@@ -483,7 +524,11 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
         mma_f16(acc[4 * j + 3], pf, e4m3_hi(a1), e4m3_hi(b1));
       }
     }
-    cp_async_wait<0>();
+    // Copies in flight when a wait ran out still write to this block's memory.
+    while (taken != sent) {
+      wait_copy(bars + 8 * (taken % kStages), (taken / kStages) & 1, a);
+      ++taken;
+    }
 
     // Merge the warps' sums: each scales its own to the block's maximum, then the block adds.
 #pragma unroll
@@ -567,7 +612,8 @@ __global__ void __launch_bounds__(kThreads) fa_cache_decode_kernel(
         }
       }
     }
-    __syncthreads();  // before the next part fills the ring
+    fence_proxy_async_smem();  // the sums were read: the next part's copies may overwrite them
+    __syncthreads();
     u += tile1 - tile0;
   }
 }
@@ -657,7 +703,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
   if (lane == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
 }
 
-int decode_ctas(int sms) { return 2 * sms; }
+int decode_ctas(int sms) { return kPerSm * sms; }
 
 template <typename T, int D>
 cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
@@ -673,10 +719,13 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
   const unsigned ctas = static_cast<unsigned>(std::max(1ll, want));
   float* partials = static_cast<float*>(a.workspace);
   constexpr int kSmem = Layout<D>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(fa_cache_decode_kernel<T, D>,
+  PageMaps maps;
+  cudaError_t e = make_page_maps(&maps, c, D, kRun);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(fa_cache_decode_kernel<T, D>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  fa_cache_decode_kernel<T, D><<<ctas, kThreads, kSmem, stream>>>(a, partials);
+  fa_cache_decode_kernel<T, D><<<ctas, kThreads, kSmem, stream>>>(a, maps, partials);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (tiles == 1) return cudaSuccess;  // no tuple has two units
   cudaLaunchConfig_t cfg = {};

@@ -48,6 +48,9 @@ cudaError_t launch_forward(const LaunchArgs& a, cudaStream_t stream);
 // Synchronises the current device, reads and clears the device status word.
 cudaError_t read_and_clear_status(unsigned int* bits);
 
+// Time limit of each device-side wait (fa_set_wait_timeout_ns).
+unsigned long long wait_timeout_ns();
+
 // Device-side status bits (which wait ran out).
 enum StatusBits : unsigned int {
   kStQFull = 1u << 0,    // MMA warp waiting for the Q tile
