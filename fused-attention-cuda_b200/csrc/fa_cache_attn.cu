@@ -22,31 +22,31 @@
 namespace fa_sm100 {
 namespace {
 
-constexpr int kRows = 16;   // query rows (token, head of the group) of one tile
 constexpr int kRun = 16;    // keys that a warp takes at a time; never more than a page
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = kRun * kWarps;  // keys of one unit of work
-constexpr int kStages = 4;            // runs in flight for each warp
-constexpr int kPerSm = 3;             // CTAs on a multiprocessor
 constexpr float kLazy = 8.0f;         // the running maximum follows once it is off by 2^8
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <int D>
+// A CTA's tile has 8 NT query rows (token, head of the group).
+template <int D, int NT>
 struct Layout {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kStages = D == 128 && NT == 1 ? 3 : 4;  // runs in flight for each warp
+  static constexpr int kPerSm = D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 5 : 4);  // CTAs
   static constexpr int kHalf = kRun * D;  // K or V bytes of a run
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kMerge = kWarps * kRows * D * 4;  // reuses the ring
   static constexpr int kMain = kRing > kMerge ? kRing : kMerge;
-  static constexpr int kScale = kWarps * kStages * 16;
+  static constexpr int kScale = kWarps * 64 * 16;
   static constexpr int kBars = kWarps * kStages * 8;
   static constexpr int kBytes = kMain + kScale + kBars + 1024;  // the ring starts on 1024 bytes
+  // A partial result: kRows x D sums, then (m, l) of each row.
+  static constexpr int kPartial = kRows * D + 2 * kRows;
 };
-
-// A partial result: kRows x D sums, then (m, l) of each row.
-__host__ __device__ constexpr int partial_floats(int D) { return kRows * D + 2 * kRows; }
 
 // Work of a sequence: row tiles x kv heads tuples, each of `tiles` units (at least one, so that a
 // row without keys is written too).
@@ -59,77 +59,85 @@ struct SeqWork {
   }
 };
 
-__device__ __forceinline__ SeqWork seq_work(const CacheView& c, int s, int group) {
+template <int ROWS>
+__device__ __forceinline__ SeqWork work_of(const SeqInfo& q, int group) {
   SeqWork w;
-  w.q = seq_info(c, s);
-  w.row_tiles = (w.q.n * group + kRows - 1) / kRows;
+  w.q = q;
+  w.row_tiles = (w.q.n * group + ROWS - 1) / ROWS;
   w.tiles = max(1, (w.q.len + kTile - 1) / kTile);
   return w;
 }
 
-// Units are numbered sequence by sequence; CTA i takes [bound(i), bound(i + 1)), never none: no more
-// CTAs work than there are units.
-__device__ __forceinline__ int ctas_of(long long total) {
-  return static_cast<int>(min(total, static_cast<long long>(gridDim.x)));
+template <int ROWS>
+__device__ __forceinline__ SeqWork seq_work(const CacheView& c, int s, int group) {
+  return work_of<ROWS>(seq_info(c, s), group);
 }
-__device__ __forceinline__ long long bound_of(long long total, int i, int ctas) {
-  return total * i / ctas;
+
+// Units are numbered sequence by sequence; CTA i of ceil(total / per) takes [i per, (i + 1) per).
+// Whole multiples keep the longest range as short as an even split would, with fewer CTAs that share
+// a tuple, and make the inverse one division.
+__device__ __forceinline__ long long units_per_cta(long long total) {
+  return (total + gridDim.x - 1) / gridDim.x;
 }
 
 struct Place {
   int s;            // sequence of the unit
+  SeqInfo q;
   long long first;  // its first unit
 };
 
-template <int THREADS>
-__device__ long long block_sum(long long x, long long* tmp) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) tmp[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) x += tmp[i];
-  return x;
-}
-
-// The total of units, then the sequence that holds one of them.
-template <int THREADS>
+// Every CTA adds up the units of all sequences and finds the one that its own range begins in.  The
+// lengths live on the device, so that a captured call follows them; THREADS sequences at a time.
+template <int THREADS, int ROWS>
 struct Finder {
   long long warp[THREADS / 32];
+  long long first;  // unit that the range begins with
   Place at;
 
-  __device__ long long total(const CacheView& c, int group) {
-    if (threadIdx.x == 0) at = Place{0, 0};
-    long long sum = 0;
-    for (int s = threadIdx.x; s < c.n_seqs; s += THREADS) sum += seq_work(c, s, group).units(c.Hkv);
-    return block_sum<THREADS>(sum, warp);
+  // Sums x over the block up to and including this thread; *sum is the block's.
+  __device__ long long scan(long long x, long long* sum) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += up;
+    }
+    __syncthreads();
+    if (lane == 31) warp[wid] = x;
+    __syncthreads();
+    *sum = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < wid) x += warp[i];
+      *sum += warp[i];
+    }
+    return x;
   }
 
-  __device__ void find(const CacheView& c, int group, long long target) {
-    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    long long run = 0;
+  // The total of units.  With at most THREADS sequences `mine` and `incl` are this thread's for find.
+  __device__ long long total(const CacheView& c, int group, SeqWork* w, long long* incl) {
+    if (threadIdx.x == 0) at = Place{0, SeqInfo{0, 0, 0}, 0};
+    long long run = 0, sum;
     for (int base = 0; base < c.n_seqs; base += THREADS) {
       const int s = base + threadIdx.x;
-      const long long mine = s < c.n_seqs ? seq_work(c, s, group).units(c.Hkv) : 0;
-      long long incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
+      *w = s < c.n_seqs ? seq_work<ROWS>(c, s, group) : SeqWork{SeqInfo{0, 0, 0}, 0, 1};
+      *incl = scan(w->units(c.Hkv), &sum);
+      run += sum;
+    }
+    return run;
+  }
+
+  __device__ void find(const CacheView& c, int group, SeqWork w, long long incl, long long unit) {
+    long long run = 0, sum;
+    for (int base = 0; base < c.n_seqs; base += THREADS) {
+      const int s = base + threadIdx.x;
+      if (c.n_seqs > THREADS) {
+        w = s < c.n_seqs ? seq_work<ROWS>(c, s, group) : SeqWork{SeqInfo{0, 0, 0}, 0, 1};
+        incl = run + scan(w.units(c.Hkv), &sum);
+        run += sum;
       }
-      __syncthreads();
-      if (lane == 31) warp[wid] = incl;
-      __syncthreads();
-      long long before = run;
-#pragma unroll
-      for (int i = 0; i < THREADS / 32; ++i) {
-        if (i < wid) before += warp[i];
-        run += warp[i];
-      }
-      incl += before;
-      if (mine > 0 && target >= incl - mine && target < incl) at = Place{s, incl - mine};
+      const long long mine = w.units(c.Hkv);
+      if (unit < incl && unit >= incl - mine) at = Place{s, w.q, incl - mine};
     }
     __syncthreads();
   }
@@ -174,6 +182,13 @@ __device__ __forceinline__ uint32_t e4m3_hi(uint32_t u) {
   return r;
 }
 
+// An 8 x 8 block of 16-bit values, two of a row to a lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t u) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(u));
+  return r;
+}
+
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -186,7 +201,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
 // What a run's scores need: t = s * mul + add, l += sum * inv.
 struct RunScale {
   float mul, add, inv;
-  int present;
+  int page;  // -1: the run's keys count as absent
 };
 
 // A page's value scale as (log2, reciprocal); exact for powers of two.  Scales are positive; zero
@@ -217,22 +232,22 @@ __device__ __forceinline__ int k_piece(int cq, int p) {
   return (D / 64) * cq + p;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_decode_kernel(
     const __grid_constant__ CacheAttnArgs a, const __grid_constant__ PageMaps maps,
     float* partials) {
-  using L = Layout<D>;
-  constexpr int kSteps = D / 16;       // products of 16 along D
-  constexpr int kWords = D / 16;       // 4-byte words of a K row that a lane holds
-  constexpr int kPieces = D / 16;      // 16-byte pieces of a row
+  using L = Layout<D, NT>;
+  constexpr int kRows = L::kRows;
+  constexpr int kSteps = D / 16;   // products of 16 along D
+  constexpr int kPieces = D / 16;  // 16-byte pieces of a K or V row
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  __shared__ Finder<kThreads> finder;
+  __shared__ Finder<kThreads, kRows> finder;
   __shared__ float merge_m[kWarps][kRows], merge_l[kWarps][kRows];
 
   const CacheView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = lane >> 2, cq = lane & 3;  // row (and key) group, column group of the fragments
+  const int r = lane >> 2, cq = lane & 3;  // row and column group of the fragments
   const int group = a.H / c.Hkv;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -248,22 +263,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
     }
   }
 
-  const long long total = finder.total(c, group);
-  const int ctas = ctas_of(total);
-  if (blockIdx.x >= static_cast<unsigned>(ctas)) return;
-  const long long u_begin = bound_of(total, blockIdx.x, ctas);
-  const long long u_end = bound_of(total, blockIdx.x + 1, ctas);
-  finder.find(c, group, u_begin);
+  SeqWork w;
+  long long incl;
+  const long long total = finder.total(c, group, &w, &incl);
+  const long long per = units_per_cta(total);
+  const long long u_begin = blockIdx.x * per, u_end = min(total, u_begin + per);
+  if (u_begin >= u_end) return;
+  finder.find(c, group, w, incl, u_begin);
   int s = finder.at.s;
   long long seq_first = finder.at.first;
+  w = work_of<kRows>(finder.at.q, group);
 
-  const uint32_t ring = smem_u32(smem) + warp * kStages * L::kStage;
-  RunScale* scales = reinterpret_cast<RunScale*>(smem + L::kMain) + warp * kStages;
-  const uint32_t bars = smem_u32(smem) + L::kMain + L::kScale + warp * kStages * 8;
+  const uint32_t ring = smem_u32(smem) + warp * L::kStages * L::kStage;
+  RunScale* table = reinterpret_cast<RunScale*>(smem + L::kMain) + warp * 64;
+  const uint32_t bars = smem_u32(smem) + L::kMain + L::kScale + warp * L::kStages * 8;
   const int page_mask = (1 << c.page_shift) - 1;
   if (lane == 0) {
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+    for (int i = 0; i < L::kStages; ++i) mbar_init(bars + 8 * i, 1);
     fence_mbar_init();
   }
   __syncwarp();
@@ -271,11 +288,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
   bool alive = true;             // false once a wait ran out: nothing more is issued or used
 
   for (long long u = u_begin; u < u_end;) {
-    SeqWork w = seq_work(c, s, group);
     while (u >= seq_first + w.units(c.Hkv)) {  // on to the sequence of unit u
       if (s + 1 >= c.n_seqs) return;
       seq_first += w.units(c.Hkv);
-      w = seq_work(c, ++s, group);
+      w = seq_work<kRows>(c, ++s, group);
     }
     const long long tuple = (u - seq_first) / w.tiles;
     const int tile0 = static_cast<int>(u - seq_first - tuple * w.tiles);
@@ -284,20 +300,85 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
     const int row0 = static_cast<int>(tuple - static_cast<long long>(head) * w.row_tiles) * kRows;
     const int rows = min(kRows, w.q.n * group - row0);
 
-    // Rows r and r + 8 of this lane: token, head and number of visible keys.
-    int limit[2];
-    float row_mul[2];
-    uint32_t qf[kSteps][4];
+    // Keys that the tile's last row sees, and those that all of its rows see.
+    const int last_token = (row0 + rows - 1) / group, first_token = row0 / group;
+    const int seen = a.causal ? max(0, w.q.len - w.q.n + last_token + 1) : w.q.len;
+    const int all_see = a.causal ? max(0, w.q.len - w.q.n + first_token + 1) : w.q.len;
+
+    // Runs of this warp: keys [first_key + i * kTile, + kRun), i < n_runs.
+    const int first_key = tile0 * kTile + warp * kRun;
+    const int stop = min(seen, tile1 * kTile);
+    const int n_runs = first_key < stop ? (stop - first_key + kTile - 1) / kTile : 0;
+
+    // Pages and scales of 32 runs at a time, a lane each, a batch ahead of their use: the page at
+    // the batch's first run, its scales 8 runs later, both into the table 16 runs later.
+    auto page_at = [&](int i) {
+      return i < n_runs ? page_of(c, s, (first_key + i * kTile) >> c.page_shift) : -1;
+    };
+    int page = page_at(lane);
+    float sk = 0.f, sv = 1.f;
+    auto read_scales = [&]() {
+      if (page >= 0) {
+        const long long at = static_cast<long long>(page) * c.Hkv + head;
+        sk = __ldg(c.k_scale + at);
+        sv = __ldg(c.v_scale + at);
+      }
+    };
+    auto write_table = [&](int i) {
+      RunScale sc;
+      sc.mul = sk;
+      value_scale(sv, &sc.add, &sc.inv);
+      sc.page = page;
+      table[i & 63] = sc;
+      __syncwarp();
+    };
+    auto send = [&](int i, int pg) {  // by one lane: run i's copies into the next stage
+      const int stage = sent % L::kStages;
+      const uint32_t bar = bars + 8 * stage, dst = ring + stage * L::kStage;
+      if (pg >= 0) {
+        const int slot = (first_key + i * kTile) & page_mask;
+        mbar_arrive_expect_tx(bar, L::kStage);
+        load_page(dst, &maps.k, maps.k_pos, slot, head, pg, bar);
+        load_page(dst + L::kHalf, &maps.v, maps.v_pos, slot, head, pg, bar);
+      } else {
+        mbar_arrive(bar);
+      }
+    };
+    int issued = 0;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int row = row0 + r + 8 * x;
-      const bool on = r + 8 * x < rows;
+    for (int i = 0; i < L::kStages - 1; ++i, ++issued) {  // before the scales are known
+      const int pg = __shfl_sync(0xffffffffu, page, i);
+      if (i < n_runs && alive) {
+        if (lane == 0) send(i, pg);
+        ++sent;
+      }
+    }
+    read_scales();
+    auto issue = [&]() {
+      const int i = issued++;
+      if (i >= n_runs) return;
+      const int step = i & 31;
+      if (step == 0) page = page_at(i + 32 + lane);
+      if (step == 8) read_scales();
+      if (step == 16) write_table(i + 16 + lane);
+      if (lane == 0) send(i, table[i & 63].page);
+      ++sent;
+    };
+
+    // Query row r of each 8: the B fragments.  Columns of step t are 4 neighbours of a row, so that
+    // a K word is the two halves of an A fragment.
+    uint32_t qf[NT][kSteps][2];
+    int limit[NT][2];      // visible keys of the rows 2cq, 2cq + 1 of each 8 (C fragments)
+    float row_mul[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int row = row0 + 8 * x + r;
+      const bool on = 8 * x + r < rows;
       const int token = on ? row / group : 0;
       const int h = head * group + (on ? row - token * group : 0);
-      limit[x] = on ? (a.causal ? max(0, w.q.len - w.q.n + token + 1) : w.q.len) : 0;
+      int lim = on ? (a.causal ? max(0, w.q.len - w.q.n + token + 1) : w.q.len) : 0;
       const T* src = static_cast<const T*>(a.q) + (w.q.t0 + token) * a.sq[0] + h * a.sq[1];
-      // Columns of step t: 4 neighbours, so that a K word is the two halves of a B fragment.
-      uint32_t raw[kSteps][2];
+      uint32_t(&raw)[kSteps][2] = qf[x];
 #pragma unroll
       for (int p = 0; p < kSteps / 4; ++p) {
         const uint4* at = reinterpret_cast<const uint4*>(src + 16 * k_piece<D>(cq, p));
@@ -307,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
 #pragma unroll
         for (int i = 0; i < 8; ++i) raw[4 * p + i / 2][i & 1] = f[i];
       }
-      row_mul[x] = a.scale * kLog2e;
+      float mul = a.scale * kLog2e;
       if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         float big = 0.f;
 #pragma unroll
@@ -321,10 +402,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
         const int e = big > 0.f && big < INFINITY
-                          ? min(126, max(-118, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 8))
+                          ? min(119, max(-118, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 8))
                           : 0;
         const float div = __int_as_float((127 - e) << 23);
-        row_mul[x] *= __int_as_float((127 + e) << 23);
+        mul *= __int_as_float((127 + e) << 23);
 #pragma unroll
         for (int t = 0; t < kSteps; ++t) {
 #pragma unroll
@@ -335,162 +416,116 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
         }
       }
 #pragma unroll
-      for (int t = 0; t < kSteps; ++t) {
-        qf[t][x] = raw[t][0];
-        qf[t][2 + x] = raw[t][1];
+      for (int e = 0; e < 2; ++e) {
+        limit[x][e] = __shfl_sync(0xffffffffu, lim, (2 * cq + e) * 4);
+        row_mul[x][e] = __shfl_sync(0xffffffffu, mul, (2 * cq + e) * 4);
       }
     }
-    // Keys that the tile's last row sees, and those that all of its rows see.
-    const int last_token = (row0 + rows - 1) / group, first_token = row0 / group;
-    const int seen = a.causal ? max(0, w.q.len - w.q.n + last_token + 1) : w.q.len;
-    const int all_see = a.causal ? max(0, w.q.len - w.q.n + first_token + 1) : w.q.len;
+    write_table(lane);
 
-    // Runs of this warp: keys [first_key + i * kTile, + kRun), i < n_runs.
-    const int first_key = tile0 * kTile + warp * kRun;
-    const int stop = min(seen, tile1 * kTile);
-    const int n_runs = first_key < stop ? (stop - first_key + kTile - 1) / kTile : 0;
-
-    // Page numbers and scales of 32 runs at a time, one to a lane, looked up a batch ahead.
-    struct Batch {
-      int page;
-      RunScale sc;
-    };
-    auto look_up = [&](int i) {
-      Batch b;
-      b.page = -1;
-      b.sc = RunScale{0.f, 0.f, 0.f, 0};
-      if (i < n_runs) {
-        b.page = page_of(c, s, (first_key + i * kTile) >> c.page_shift);
-        if (b.page >= 0) {
-          const long long at = static_cast<long long>(b.page) * c.Hkv + head;
-          b.sc.mul = __ldg(c.k_scale + at);
-          value_scale(__ldg(c.v_scale + at), &b.sc.add, &b.sc.inv);
-          b.sc.present = 1;
-        }
-      }
-      return b;
-    };
-    Batch now = look_up(lane), next = look_up(32 + lane);
-    int issued = 0;
-    auto issue = [&]() {
-      const int i = issued++;
-      if (i >= n_runs || !alive) return;
-      if (i > 0 && (i & 31) == 0) {
-        now = next;
-        next = look_up(i + 32 + lane);
-      }
-      const int stage = sent % kStages;
-      ++sent;
-      const int page = __shfl_sync(0xffffffffu, now.page, i & 31);
-      if (lane == (i & 31)) scales[stage] = now.sc;
-      if (lane == 0) {
-        const uint32_t bar = bars + 8 * stage, dst = ring + stage * L::kStage;
-        if (page >= 0) {
-          const int slot = (first_key + i * kTile) & page_mask;
-          mbar_arrive_expect_tx(bar, L::kStage);
-          load_page(dst, &maps.k, maps.k_pos, slot, head, page, bar);
-          load_page(dst + L::kHalf, &maps.v, maps.v_pos, slot, head, page, bar);
-        } else {
-          mbar_arrive(bar);
-        }
-      }
-    };
+    // Sums transposed: columns (D / 8) r + 2 j + (e >> 1), row 2cq + (e & 1) of each 8.
+    float acc[NT][D / 16][4];
+    float m[NT][2], l[NT][2];
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue();
-
-    float acc[D / 8][4];
+    for (int x = 0; x < NT; ++x) {
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
+      for (int j = 0; j < D / 16; ++j) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+        for (int e = 0; e < 4; ++e) acc[x][j][e] = 0.f;
+      }
+      m[x][0] = m[x][1] = -INFINITY;
+      l[x][0] = l[x][1] = 0.f;
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     for (int i = 0; i < n_runs; ++i) {
-      const int stage = taken % kStages;
-      if (alive) alive = wait_copy(bars + 8 * stage, (taken / kStages) & 1, a);
+      const int stage = taken % L::kStages;
+      if (alive) alive = wait_copy(bars + 8 * stage, (taken / L::kStages) & 1, a);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       ++taken;
       issue();  // into the stage that every lane left before the vote
       const uint32_t kb = ring + stage * L::kStage;
       const uint32_t vb = kb + L::kHalf;
-      const RunScale sc = scales[stage];
+      const RunScale sc = table[i & 63];
 
-      float sacc[2][2][4] = {};  // [8 keys][even, odd steps]: shorter chains of products
+      // Scores, transposed: keys r, r + 8 by rows 2cq, 2cq + 1.  Even and odd steps apart, for
+      // shorter chains of products.
+      float sacc[NT][2][4] = {};
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const int key = nt * 8 + r;
-        uint32_t kw[kWords];
+      for (int p = 0; p < kPieces / 4; ++p) {
+        const int piece = k_piece<D>(cq, p);
+        const uint32_t at =
+            kb + r * D + (D == 128 ? piece ^ r : piece ^ ((r >> 1) & 3)) * 16;
+        const uint4 lo = lds128(at), hi = lds128(at + 8 * D);
+        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-        for (int p = 0; p < kPieces / 4; ++p) {
-          const int piece = k_piece<D>(cq, p);
-          const uint4 v = lds128(kb + key * D + (D == 128 ? piece ^ r : piece ^ ((r >> 1) & 3)) * 16);
-          kw[4 * p] = v.x, kw[4 * p + 1] = v.y, kw[4 * p + 2] = v.z, kw[4 * p + 3] = v.w;
-        }
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t kf[4] = {e4m3_lo(wl[t]), e4m3_lo(wh[t]), e4m3_hi(wl[t]), e4m3_hi(wh[t])};
 #pragma unroll
-        for (int t = 0; t < kSteps; ++t) {
-          mma_f16(sacc[nt][t & 1], qf[t], e4m3_lo(kw[t]), e4m3_hi(kw[t]));
+          for (int x = 0; x < NT; ++x) mma_f16(sacc[x][t & 1], kf, qf[x][4 * p + t][0], qf[x][4 * p + t][1]);
         }
       }
 
-      float mul[2] = {sc.mul * row_mul[0], sc.mul * row_mul[1]};
-      float t[2][4];  // [row][key]
+      float t[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
+      for (int x = 0; x < NT; ++x) {
+        const float mul[2] = {sc.mul * row_mul[x][0], sc.mul * row_mul[x][1]};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          t[e >> 1][nt * 2 + (e & 1)] = fmaf(sacc[nt][0][e] + sacc[nt][1][e], mul[e >> 1], sc.add);
-        }
+        for (int e = 0; e < 4; ++e) t[x][e] = fmaf(sacc[x][0][e] + sacc[x][1][e], mul[e & 1], sc.add);
       }
       const int key0 = first_key + i * kTile;
-      if (key0 + kRun > all_see || !sc.present) {
+      const bool ragged = key0 + kRun > w.q.len || sc.page < 0;
+      if (key0 + kRun > all_see || sc.page < 0) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int lim = sc.present ? limit[x] - key0 : 0;
+        for (int x = 0; x < NT; ++x) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            if ((e >> 1) * 8 + 2 * cq + (e & 1) >= lim) t[x][e] = -INFINITY;
+            if (sc.page < 0 || key0 + r + 8 * (e >> 1) >= limit[x][e & 1]) t[x][e] = -INFINITY;
           }
         }
       }
-      float big[2];
       bool moved = false;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        big[x] = fmaxf(fmaxf(t[x][0], t[x][1]), fmaxf(t[x][2], t[x][3]));
-        moved |= big[x] > m[x] + kLazy;
+      for (int x = 0; x < NT; ++x) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) moved |= fmaxf(t[x][e], t[x][e + 2]) > m[x][e] + kLazy;
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          big[x] = fmaxf(big[x], __shfl_xor_sync(0xffffffffu, big[x], 1));
-          big[x] = fmaxf(big[x], __shfl_xor_sync(0xffffffffu, big[x], 2));
-          const float to = fmaxf(m[x], big[x]);
-          const float f = to == m[x] ? 1.f : ex2_approx(m[x] - to);
-          m[x] = to;
-          l[x] *= f;
+        for (int x = 0; x < NT; ++x) {
 #pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            acc[j][2 * x] *= f;
-            acc[j][2 * x + 1] *= f;
+          for (int e = 0; e < 2; ++e) {
+            float big = fmaxf(t[x][e], t[x][e + 2]);
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 4));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 8));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 16));
+            const float to = fmaxf(m[x][e], big);
+            const float f = to == m[x][e] ? 1.f : ex2_approx(m[x][e] - to);
+            m[x][e] = to;
+            l[x][e] *= f;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+              acc[x][j][e] *= f;
+              acc[x][j][e + 2] *= f;
+            }
           }
         }
       }
-      uint32_t pf[4];
+      uint32_t pf[NT][2];  // P's B fragments: the 8 x 8 blocks of P transposed
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float ref = m[x] == -INFINITY ? 0.f : m[x];
+      for (int x = 0; x < NT; ++x) {
         float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = ex2_approx(t[x][e] - ref);
-        l[x] = fmaf((p[0] + p[1]) + (p[2] + p[3]), sc.inv, l[x]);
-        pf[x] = from_float2<__half>(p[0], p[1]);
-        pf[2 + x] = from_float2<__half>(p[2], p[3]);
+        for (int e = 0; e < 4; ++e) {
+          p[e] = ex2_approx(t[x][e] - (m[x][e & 1] == -INFINITY ? 0.f : m[x][e & 1]));
+        }
+        l[x][0] = fmaf(p[0] + p[2], sc.inv, l[x][0]);
+        l[x][1] = fmaf(p[1] + p[3], sc.inv, l[x][1]);
+        pf[x][0] = transpose8(from_float2<__half>(p[0], p[1]));
+        pf[x][1] = transpose8(from_float2<__half>(p[2], p[3]));
       }
 
-      // V: this lane's keys 2cq, 2cq + 1, 2cq + 8, 2cq + 9 and columns (D / 8) r .. + D / 8: column
-      // block j of the products holds the columns (D / 8) n + j, n = 0..7.
+      // V, transposed: this lane's keys 2cq, 2cq + 1, 2cq + 8, 2cq + 9 and columns (D / 8) r + ...
       uint32_t vw[4][D / 32];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -502,60 +537,63 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
           const uint2 v = lds64(vb + key * D + ((r >> 1) ^ ((key >> 1) & 3)) * 16 + (r & 1) * 8);
           vw[k][0] = v.x, vw[k][1] = v.y;
         }
-      }
-      if (key0 + kRun > w.q.len || !sc.present) {  // behind the last key a page holds anything
+        if (ragged && (sc.page < 0 || key0 + key >= w.q.len)) {  // a page's tail holds anything
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (key0 + 2 * cq + (k & 1) + 8 * (k >> 1) >= w.q.len || !sc.present) {
-#pragma unroll
-            for (int j = 0; j < D / 32; ++j) vw[k][j] = 0;
-          }
+          for (int j = 0; j < D / 32; ++j) vw[k][j] = 0;
         }
       }
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
+      for (int j = 0; j < D / 32; ++j) {  // columns 4j .. 4j + 3 of the lane's
         const uint32_t a0 = __byte_perm(vw[0][j], vw[1][j], 0x5140);
         const uint32_t a1 = __byte_perm(vw[0][j], vw[1][j], 0x7362);
         const uint32_t b0 = __byte_perm(vw[2][j], vw[3][j], 0x5140);
         const uint32_t b1 = __byte_perm(vw[2][j], vw[3][j], 0x7362);
-        mma_f16(acc[4 * j], pf, e4m3_lo(a0), e4m3_lo(b0));
-        mma_f16(acc[4 * j + 1], pf, e4m3_hi(a0), e4m3_hi(b0));
-        mma_f16(acc[4 * j + 2], pf, e4m3_lo(a1), e4m3_lo(b1));
-        mma_f16(acc[4 * j + 3], pf, e4m3_hi(a1), e4m3_hi(b1));
+        const uint32_t v0[4] = {e4m3_lo(a0), e4m3_hi(a0), e4m3_lo(b0), e4m3_hi(b0)};
+        const uint32_t v1[4] = {e4m3_lo(a1), e4m3_hi(a1), e4m3_lo(b1), e4m3_hi(b1)};
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          mma_f16(acc[x][2 * j], v0, pf[x][0], pf[x][1]);
+          mma_f16(acc[x][2 * j + 1], v1, pf[x][0], pf[x][1]);
+        }
       }
     }
     // Copies in flight when a wait ran out still write to this block's memory.
     while (taken != sent) {
-      wait_copy(bars + 8 * (taken % kStages), (taken / kStages) & 1, a);
+      wait_copy(bars + 8 * (taken % L::kStages), (taken / L::kStages) & 1, a);
       ++taken;
     }
 
     // Merge the warps' sums: each scales its own to the block's maximum, then the block adds.
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (cq == 0) {
-        merge_m[warp][r + 8 * x] = m[x];
-        merge_l[warp][r + 8 * x] = l[x];
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o *= 2) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], o);
+        if (r == 0) {
+          merge_m[warp][8 * x + 2 * cq + e] = m[x][e];
+          merge_l[warp][8 * x + 2 * cq + e] = l[x][e];
+        }
       }
     }
     __syncthreads();  // and no warp reads its ring any more
     float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float top = merge_m[0][r + 8 * x];
+    for (int x = 0; x < NT; ++x) {
 #pragma unroll
-      for (int i = 1; i < kWarps; ++i) top = fmaxf(top, merge_m[i][r + 8 * x]);
-      const float f = m[x] == -INFINITY ? (l[x] == l[x] ? 0.f : l[x]) : ex2_approx(m[x] - top);
-      float* at = sums + (warp * kRows + r + 8 * x) * D;
+      for (int e = 0; e < 2; ++e) {
+        const int row = 8 * x + 2 * cq + e;
+        float top = merge_m[0][row];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+        for (int i = 1; i < kWarps; ++i) top = fmaxf(top, merge_m[i][row]);
+        const float f = m[x][e] == -INFINITY ? (l[x][e] == l[x][e] ? 0.f : l[x][e])
+                                             : ex2_approx(m[x][e] - top);
+        float* at = sums + (warp * kRows + row) * D + r * (D / 8);
 #pragma unroll
-        for (int j = 0; j < D / 8; j += 4) {
-          *reinterpret_cast<float4*>(at + (2 * cq + n) * (D / 8) + j) =
-              make_float4(acc[j][2 * x + n] * f, acc[j + 1][2 * x + n] * f,
-                          acc[j + 2][2 * x + n] * f, acc[j + 3][2 * x + n] * f);
+        for (int j = 0; j < D / 16; j += 2) {
+          *reinterpret_cast<float4*>(at + 2 * j) =
+              make_float4(acc[x][j][e] * f, acc[x][j][e + 2] * f, acc[x][j + 1][e] * f,
+                          acc[x][j + 1][e + 2] * f);
         }
       }
     }
@@ -572,16 +610,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
         const float wm = merge_m[i][row], wl = merge_l[i][row];
         lsum += wm == -INFINITY ? (wl == wl ? 0.f : wl) : wl * ex2_approx(wm - top);
       }
-      float out[kPer];
+      float4 out[kPer / 4];
 #pragma unroll
-      for (int k = 0; k < kPer; k += 4) {
-        float4 v = *reinterpret_cast<const float4*>(sums + row * D + col + k);
+      for (int k = 0; k < kPer / 4; ++k) {
+        out[k] = *reinterpret_cast<const float4*>(sums + row * D + col + 4 * k);
 #pragma unroll
         for (int i = 1; i < kWarps; ++i) {
-          const float4 x = *reinterpret_cast<const float4*>(sums + (i * kRows + row) * D + col + k);
-          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+          const float4 x =
+              *reinterpret_cast<const float4*>(sums + (i * kRows + row) * D + col + 4 * k);
+          out[k].x += x.x, out[k].y += x.y, out[k].z += x.z, out[k].w += x.w;
         }
-        out[k] = v.x, out[k + 1] = v.y, out[k + 2] = v.z, out[k + 3] = v.w;
       }
       if (whole) {
         const int token = (row0 + row) / group;
@@ -590,21 +628,18 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
         const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
         T* o = static_cast<T*>(a.o) + at * D + col;
 #pragma unroll
-        for (int k = 0; k < kPer; k += 8) {
-          uint4 v;
-          v.x = from_float2<T>(out[k] * inv, out[k + 1] * inv);
-          v.y = from_float2<T>(out[k + 2] * inv, out[k + 3] * inv);
-          v.z = from_float2<T>(out[k + 4] * inv, out[k + 5] * inv);
-          v.w = from_float2<T>(out[k + 6] * inv, out[k + 7] * inv);
-          *reinterpret_cast<uint4*>(o + k) = v;
+        for (int k = 0; k < kPer / 4; ++k) {
+          uint2 v;
+          v.x = from_float2<T>(out[k].x * inv, out[k].y * inv);
+          v.y = from_float2<T>(out[k].z * inv, out[k].w * inv);
+          *reinterpret_cast<uint2*>(o + 4 * k) = v;
         }
         if (col == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
       } else {
-        float* part = partials + (2ll * blockIdx.x + (u == u_begin ? 0 : 1)) * partial_floats(D);
+        float* part = partials + (2ll * blockIdx.x + (u == u_begin ? 0 : 1)) * L::kPartial;
 #pragma unroll
-        for (int k = 0; k < kPer; k += 4) {
-          *reinterpret_cast<float4*>(part + row * D + col + k) =
-              make_float4(out[k], out[k + 1], out[k + 2], out[k + 3]);
+        for (int k = 0; k < kPer / 4; ++k) {
+          *reinterpret_cast<float4*>(part + row * D + col + 4 * k) = out[k];
         }
         if (col == 0) {
           part[kRows * D + row] = top;
@@ -622,28 +657,30 @@ __global__ void __launch_bounds__(kThreads, kPerSm) fa_cache_decode_kernel(
 // range begins inside of, if no earlier CTA's does too.  Each row's parts are split over warps.
 constexpr int kCombineWarps = 16;
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
     const __grid_constant__ CacheAttnArgs a, const float* partials) {
+  using L = Layout<D, NT>;
+  constexpr int kRows = L::kRows;
   constexpr int kPer = D / 32;
-  __shared__ Finder<32 * kCombineWarps> finder;
+  __shared__ Finder<32 * kCombineWarps, kRows> finder;
   __shared__ float sums[kCombineWarps][D];
   __shared__ float tops[kCombineWarps], lsums[kCombineWarps];
   const CacheView& c = a.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = a.H / c.Hkv;
   const int me = blockIdx.x;
-  const long long total = finder.total(c, group);
-  const int ctas = ctas_of(total);
-  if (me == 0 || me >= ctas) return;
-  const long long begin = bound_of(total, me, ctas);
-  finder.find(c, group, begin);
-  const int s = finder.at.s;
+  SeqWork w;
+  long long incl;
+  const long long total = finder.total(c, group, &w, &incl);
+  const long long per = units_per_cta(total), begin = me * per;
+  if (me == 0 || begin >= total) return;
+  finder.find(c, group, w, incl, begin);
   const long long seq_first = finder.at.first;
-  const SeqWork w = seq_work(c, s, group);
+  w = work_of<kRows>(finder.at.q, group);
   const long long tuple = (begin - seq_first) / w.tiles;
   const long long first = seq_first + tuple * w.tiles, end = first + w.tiles;
-  if (first == begin || bound_of(total, me - 1, ctas) > first) return;
+  if (first == begin || begin - per > first) return;
   const int head = static_cast<int>(tuple / w.row_tiles);
   const int row0 = static_cast<int>(tuple - static_cast<long long>(head) * w.row_tiles) * kRows;
   const int rows = min(kRows, w.q.n * group - row0);
@@ -652,25 +689,38 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
   int split = 1;  // rows side by side; the warps of a row share its parts
   while (split < rows) split *= 2;
   const int row = warp % split, share = warp / split, shares = kCombineWarps / split;
-  int last = me;  // one past the last CTA with a part
-  while (last < ctas && bound_of(total, last, ctas) < end) ++last;
+  const int last = static_cast<int>((end - 1) / per);  // the last CTA with a part
   float top = -INFINITY, lsum = 0.f, acc[kPer] = {};
   if (row < rows) {
-    for (int i = me - 1 + share; i < last; i += shares) {
-      const int slot = bound_of(total, i, ctas) >= first ? 0 : 1;
-      const float* part = partials + (2ll * i + slot) * partial_floats(D);
-      const float pm = part[kRows * D + row], pl = part[kRows * D + kRows + row];
-      if (pm == -INFINITY && pl == 0.f) continue;
-      float v[kPer];
+    constexpr int kBatch = 4;  // parts in flight
+    for (int i0 = me - 1 + share; i0 <= last; i0 += kBatch * shares) {
+      float pm[kBatch], pl[kBatch], v[kBatch][kPer];
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) v[k] = part[row * D + lane * kPer + k];
-      const float to = fmaxf(top, pm);
-      const float f0 = top == -INFINITY ? 0.f : ex2_approx(top - to);
-      const float f1 = pm == -INFINITY ? 1.f : ex2_approx(pm - to);
-      top = to;
-      lsum = lsum * f0 + pl * f1;
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = i0 + b * shares;
+        pm[b] = -INFINITY;
+        pl[b] = 0.f;
+        if (i <= last) {
+          // Its first part, unless it is the one that this tuple starts inside of.
+          const int slot = i * per >= first ? 0 : 1;
+          const float* part = partials + (2ll * i + slot) * L::kPartial;
+          pm[b] = part[kRows * D + row];
+          pl[b] = part[kRows * D + kRows + row];
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f0 + v[k] * f1;
+          for (int k = 0; k < kPer; ++k) v[b][k] = part[row * D + lane * kPer + k];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (pm[b] == -INFINITY && pl[b] == 0.f) continue;
+        const float to = fmaxf(top, pm[b]);
+        const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - to);
+        const float f1 = pm[b] == -INFINITY ? 1.f : ex2_approx(pm[b] - to);
+        top = to;
+        lsum = lsum * f0 + pl[b] * f1;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f0 + v[b][k] * f1;
+      }
     }
   }
 #pragma unroll
@@ -686,7 +736,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
     const float pm = tops[other], pl = lsums[other];
     if (pm == -INFINITY && pl == 0.f) continue;
     const float to = fmaxf(top, pm);
-    const float f0 = top == -INFINITY ? 0.f : ex2_approx(top - to);
+    const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - to);
     const float f1 = pm == -INFINITY ? 1.f : ex2_approx(pm - to);
     top = to;
     lsum = lsum * f0 + pl * f1;
@@ -703,29 +753,27 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
   if (lane == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
 }
 
-int decode_ctas(int sms) { return kPerSm * sms; }
-
-template <typename T, int D>
+template <typename T, int D, int NT>
 cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
+  using L = Layout<D, NT>;
   const CacheView& c = a.c;
   const int group = a.H / c.Hkv;
   // No more CTAs than units that the table could hold.
   const long long room = static_cast<long long>(c.max_pages) << c.page_shift;
   const long long tiles = std::max(1ll, (room + kTile - 1) / kTile);
   const long long tuples =
-      (static_cast<long long>(c.T) * group / kRows + c.n_seqs) * c.Hkv;
-  const long long want = std::min<long long>(decode_ctas(multiprocessors()),
+      (static_cast<long long>(c.T) * group / L::kRows + c.n_seqs) * c.Hkv;
+  const long long want = std::min<long long>(static_cast<long long>(L::kPerSm) * multiprocessors(),
                                              tuples > (1ll << 40) / tiles ? (1ll << 40) : tuples * tiles);
   const unsigned ctas = static_cast<unsigned>(std::max(1ll, want));
   float* partials = static_cast<float*>(a.workspace);
-  constexpr int kSmem = Layout<D>::kBytes;
   PageMaps maps;
   cudaError_t e = make_page_maps(&maps, c, D, kRun);
   if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(fa_cache_decode_kernel<T, D>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  e = cudaFuncSetAttribute(fa_cache_decode_kernel<T, D, NT>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return e;
-  fa_cache_decode_kernel<T, D><<<ctas, kThreads, kSmem, stream>>>(a, maps, partials);
+  fa_cache_decode_kernel<T, D, NT><<<ctas, kThreads, L::kBytes, stream>>>(a, maps, partials);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (tiles == 1) return cudaSuccess;  // no tuple has two units
   cudaLaunchConfig_t cfg = {};
@@ -737,22 +785,42 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fa_cache_combine_kernel<T, D>, a,
+  return cudaLaunchKernelEx(&cfg, fa_cache_combine_kernel<T, D, NT>, a,
                             static_cast<const float*>(partials));
+}
+
+// Tiles of 8 query rows where a sequence has no more on average, else of 16.
+bool narrow_tiles(int H, int Hkv, int T, int n_seqs) {
+  return static_cast<long long>(T) * (H / Hkv) <= 8ll * n_seqs;
+}
+
+template <typename T, int D>
+cudaError_t launch_d(const CacheAttnArgs& a, cudaStream_t stream) {
+  return narrow_tiles(a.H, a.c.Hkv, a.c.T, a.c.n_seqs) ? launch_t<T, D, 1>(a, stream)
+                                                       : launch_t<T, D, 2>(a, stream);
+}
+
+template <int D>
+size_t workspace_d(int H, int Hkv, int T, int n_seqs, int sms) {
+  const int floats = narrow_tiles(H, Hkv, T, n_seqs)
+                         ? Layout<D, 1>::kPerSm * Layout<D, 1>::kPartial
+                         : Layout<D, 2>::kPerSm * Layout<D, 2>::kPartial;
+  return 2ull * sms * floats * sizeof(float);
 }
 
 }  // namespace
 
-size_t cache_attention_workspace(int, int, int D, int, int, int sms) {
-  return 2ull * decode_ctas(sms) * partial_floats(D) * sizeof(float);
+size_t cache_attention_workspace(int H, int Hkv, int D, int T, int n_seqs, int sms) {
+  return D == 64 ? workspace_d<64>(H, Hkv, T, n_seqs, sms)
+                 : workspace_d<128>(H, Hkv, T, n_seqs, sms);
 }
 
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, cudaStream_t stream) {
   if (a.dtype == FA_DTYPE_F16) {
-    return a.D == 64 ? launch_t<__half, 64>(a, stream) : launch_t<__half, 128>(a, stream);
+    return a.D == 64 ? launch_d<__half, 64>(a, stream) : launch_d<__half, 128>(a, stream);
   }
-  return a.D == 64 ? launch_t<__nv_bfloat16, 64>(a, stream)
-                   : launch_t<__nv_bfloat16, 128>(a, stream);
+  return a.D == 64 ? launch_d<__nv_bfloat16, 64>(a, stream)
+                   : launch_d<__nv_bfloat16, 128>(a, stream);
 }
 
 }  // namespace fa_sm100
