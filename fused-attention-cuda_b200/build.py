@@ -41,7 +41,7 @@ NVCC_FLAGS = [*ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPI
               "-Xcompiler", "-Wall", f"-I{INCLUDE}", f"-I{CSRC}"]
 
 KERNEL_SOURCES = ["fa_fwd_sm100.cu", "dispatch.cu", "fa_combine.cu", "fa_noalloc.cu", "fa_cache.cu",
-                  "fa_cache_append.cu", "fa_cache_attn.cu"]
+                  "fa_cache_append.cu", "fa_cache_attn.cu", "fa_cache_tile.cu"]
 KERNEL_HEADERS = ["sm100_ptx.cuh", "fa_launch.h", "fa_kernel_common.cuh", "fa_fwd_lookahead.cuh",
                   "fa_cache.h", "fa_cache_common.cuh"]
 

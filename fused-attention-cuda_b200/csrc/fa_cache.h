@@ -63,6 +63,9 @@ struct CacheAttnArgs {
 
 cudaError_t launch_cache_append(const AppendArgs& a, cudaStream_t stream);
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, cudaStream_t stream);
+// Sequences with few query rows on average (fa_cache_attn.cu) or many (fa_cache_tile.cu).
+cudaError_t launch_cache_tile(const CacheAttnArgs& a, cudaStream_t stream);
+size_t cache_tile_workspace(int D, int sms);
 size_t cache_attention_workspace(int H, int Hkv, int D, int T, int n_seqs, int sms);
 
 // Tensor maps of the pages {d, token, kv head, page}, the last three ordered by stride; `pos` packs
@@ -71,8 +74,8 @@ struct PageMaps {
   CUtensorMap k, v;
   int k_pos, v_pos;
 };
-// Boxes of `rows` tokens, swizzled by the row's D bytes.
-cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows);
+// Boxes of `rows` tokens, swizzled by the row's D bytes or row after row.
+cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows, bool swizzled);
 
 // Multiprocessors of the current device (148 when the query fails).
 int multiprocessors();

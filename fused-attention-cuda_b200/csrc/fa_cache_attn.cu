@@ -310,8 +310,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
     const int stop = min(seen, tile1 * kTile);
     const int n_runs = first_key < stop ? (stop - first_key + kTile - 1) / kTile : 0;
 
-    // Pages and scales of 32 runs at a time, a lane each, a batch ahead of their use: the page at
-    // the batch's first run, its scales 8 runs later, both into the table 16 runs later.
+    // Pages and scales of 32 runs at a time, a lane each, a batch ahead of their use: the page when
+    // run 4 of the batch before is issued, its scales 8 runs later, both into the table 8 runs later.
+    static_assert(L::kStages <= 4, "the first runs are issued without this schedule");
     auto page_at = [&](int i) {
       return i < n_runs ? page_of(c, s, (first_key + i * kTile) >> c.page_shift) : -1;
     };
@@ -358,9 +359,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
       const int i = issued++;
       if (i >= n_runs) return;
       const int step = i & 31;
-      if (step == 0) page = page_at(i + 32 + lane);
-      if (step == 8) read_scales();
-      if (step == 16) write_table(i + 16 + lane);
+      if (step == 4) page = page_at(i + 28 + lane);
+      if (step == 12) read_scales();
+      if (step == 20) write_table(i + 12 + lane);
       if (lane == 0) send(i, table[i & 63].page);
       ++sent;
     };
@@ -768,7 +769,7 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
   const unsigned ctas = static_cast<unsigned>(std::max(1ll, want));
   float* partials = static_cast<float*>(a.workspace);
   PageMaps maps;
-  cudaError_t e = make_page_maps(&maps, c, D, kRun);
+  cudaError_t e = make_page_maps(&maps, c, D, kRun, true);
   if (e != cudaSuccess) return e;
   e = cudaFuncSetAttribute(fa_cache_decode_kernel<T, D, NT>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
@@ -794,6 +795,11 @@ bool narrow_tiles(int H, int Hkv, int T, int n_seqs) {
   return static_cast<long long>(T) * (H / Hkv) <= 8ll * n_seqs;
 }
 
+// More than 16 rows on average go to the kernel on tcgen05 (fa_cache_tile.cu).
+bool wide_tiles(int H, int Hkv, int T, int n_seqs) {
+  return static_cast<long long>(T) * (H / Hkv) > 16ll * n_seqs;
+}
+
 template <typename T, int D>
 cudaError_t launch_d(const CacheAttnArgs& a, cudaStream_t stream) {
   return narrow_tiles(a.H, a.c.Hkv, a.c.T, a.c.n_seqs) ? launch_t<T, D, 1>(a, stream)
@@ -811,11 +817,13 @@ size_t workspace_d(int H, int Hkv, int T, int n_seqs, int sms) {
 }  // namespace
 
 size_t cache_attention_workspace(int H, int Hkv, int D, int T, int n_seqs, int sms) {
+  if (wide_tiles(H, Hkv, T, n_seqs)) return cache_tile_workspace(D, sms);
   return D == 64 ? workspace_d<64>(H, Hkv, T, n_seqs, sms)
                  : workspace_d<128>(H, Hkv, T, n_seqs, sms);
 }
 
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, cudaStream_t stream) {
+  if (wide_tiles(a.H, a.c.Hkv, a.c.T, a.c.n_seqs)) return launch_cache_tile(a, stream);
   if (a.dtype == FA_DTYPE_F16) {
     return a.D == 64 ? launch_d<__half, 64>(a, stream) : launch_d<__half, 128>(a, stream);
   }

@@ -1,0 +1,1042 @@
+// fa_cache_tile.cu -- attention over the paged e4m3 cache for sequences with many query rows: prompt
+// chunks, drafts, mixed batches.  Same mathematics as fa_cache_attn.cu (see there); here the two
+// products run on tcgen05 with their accumulators in tensor memory.
+//
+// A tile is up to 256 query rows of one (sequence, kv head): rows are (token, head of the group)
+// packed, so the group's heads share every key that is loaded and converted.  Keys come 128 at a time
+// (one unit of work).  The units of all sequences are numbered and split evenly over one CTA for each
+// multiprocessor; a tile that several CTAs share leaves fp32 partials for fa_cache_tile_merge_kernel.
+//
+//   warp 12      looks pages and scales up, loads e4m3 pages by TMA (two tiles of K and V in flight)
+//   warps 8-11   convert a tile to fp16 into the swizzled layout of the products (exact; K in two
+//                buffers, V in one): tcgen05 has no product of fp16 by e4m3, and rounding q and P to
+//                8 bits would cost what the cache's own 8 bits cost again
+//   warp 13      issues S = Q K^T and O += P V
+//   warps 0-3, 4-7   two softmax groups, a row to a thread.  With more than 128 rows group g has rows
+//                128 g .. and every key tile; otherwise both have the same rows and the key tiles
+//                alternate, and their sums are merged at the end (both lie in one lane of tensor memory).  Either way step i belongs to group
+//                i & 1, and the tensor core works for one group while the other exponentiates.
+//
+// S_g takes 128 columns of tensor memory, P_g (fp16) overwrites the last 64, O_g takes D.
+#include <algorithm>
+#include <cmath>
+
+#include "fa_cache_common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fa_sm100 {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kRows = 256;   // query rows of a tile
+constexpr int kHalfRows = 128;
+constexpr int kKeys = 128;   // keys of a unit
+constexpr int kGroups = kKeys / 16;
+constexpr int kTables = 8;   // scale tables in flight: more than the tiles between load and softmax
+constexpr int kPairBarrier = 1;  // named barrier of the two softmax groups
+constexpr float kLazy = 8.0f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct Layout {
+  static constexpr int kChunks = D / 64;             // 128-byte column chunks of an fp16 tile
+  static constexpr int kChunkBytes = kKeys * 128;
+  static constexpr int kTile16 = kChunks * kChunkBytes;  // 128 rows of fp16 (Q half, K or V tile)
+  static constexpr int kTile8 = kKeys * D;
+  static constexpr int kQ = 0;
+  static constexpr int kK16 = kQ + 2 * kTile16;
+  static constexpr int kV16 = kK16 + 2 * kTile16;
+  static constexpr int kK8 = kV16 + kTile16;
+  static constexpr int kV8 = kK8 + 2 * kTile8;
+  static constexpr int kTable = kV8 + 2 * kTile8;
+  static constexpr int kBars = kTable + kTables * kGroups * 16;
+  // Barriers.
+  static constexpr int kK8Full = 0, kK8Empty = 2, kV8Full = 4, kV8Empty = 6, kK16Full = 8,
+                       kK16Empty = 10, kV16Full = 12, kV16Empty = 13, kSFull = 14, kPFull = 16,
+                       kOFull = 18, kQFull = 20, kTabFull = 22, kDrain = kTabFull + kTables,
+                       kCount = kDrain + 1;
+  static constexpr int kMisc = kBars + 8 * kCount;
+  static constexpr int kClean = kMisc + 16;  // per table: every key of the tile is there
+  static constexpr int kBytes = kClean + 4 * kTables + 1024;
+  static constexpr int kColS = 0, kColO = 256, kCols = 512;
+  static constexpr int kPartial = kRows * D + 2 * kRows;  // floats
+  static_assert(kBytes <= 232448, "shared memory overflow");
+};
+
+struct RunScale {
+  float mul, add, inv;
+  int page;
+};
+
+// ---- work ----
+
+// sum over i < n of floor((2 i + b) / m)
+__device__ __forceinline__ long long sum_floors(unsigned n, unsigned m, unsigned b) {
+  long long sum = 0;
+  unsigned a = 2;
+  for (;;) {
+    if (a >= m) {
+      sum += static_cast<long long>(n) * (n - 1ll) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += static_cast<long long>(n) * (b / m);
+      b %= m;
+    }
+    const unsigned y = a * n + b;
+    if (y < m) return sum;
+    n = y / m;
+    b = y % m;
+    const unsigned t = m;
+    m = a;
+    a = t;
+  }
+}
+
+// The tiles of one (sequence, kv head).  Tile j's last row is a query that sees
+//   past + floor((256 j + 255) / group) + 1
+// keys (causal), so it has floor((2 j + base) / group) units, base = floor((255 + group (past + 128))
+// / 128), and the units in front of tile j have a closed form.  The last tile ends with the last row.
+struct SeqTiles {
+  SeqInfo q;
+  int rows, tiles;
+  bool causal;
+  int full;        // not causal: units of each tile
+  int last;        // units of the last tile
+  long long base;  // causal, see above
+  long long units;  // of one kv head
+
+  __device__ long long before(int j, int group) const {
+    if (!causal) return static_cast<long long>(j) * full;
+    if (j <= 0) return 0;
+    const long long whole = base / group;
+    return whole * j + sum_floors(j, group, static_cast<unsigned>(base - whole * group));
+  }
+  __device__ int of(int j, int group) const {
+    if (j == tiles - 1) return last;
+    return causal ? static_cast<int>((2ll * j + base) / group) : full;
+  }
+};
+
+__device__ __forceinline__ SeqTiles tiles_of(const SeqInfo& q, int group, bool causal) {
+  SeqTiles t;
+  t.q = q;
+  t.causal = causal;
+  t.rows = q.n * group;
+  t.tiles = (t.rows + kRows - 1) / kRows;
+  t.full = max(1, (q.len + kKeys - 1) / kKeys);
+  t.last = t.full;
+  t.base = 0;
+  t.units = 0;
+  if (t.tiles == 0) return t;
+  if (causal) {
+    // Queries in front of the cache count as if they saw their own keys: a few units too many.
+    const long long past = max(0, q.len - q.n);
+    t.base = (255 + group * (past + kKeys)) / kKeys;
+    t.last = static_cast<int>((t.rows - 1 + group * (past + kKeys)) / (static_cast<long long>(kKeys) * group));
+  }
+  t.units = t.before(t.tiles - 1, group) + t.last;
+  return t;
+}
+
+__device__ __forceinline__ long long units_per_cta(long long total) {
+  return (total + gridDim.x - 1) / gridDim.x;
+}
+
+// A place in the list of units: unit `u` is unit `tile` of row tile `j` of kv head `head`.
+struct Place {
+  int s, head, j, tile;
+};
+
+// All CTAs add up the units of the sequences and find the place that their own range begins at.
+struct Finder {
+  long long warp[kThreads / 32];
+  SeqInfo q;
+  long long first;
+  Place at;
+
+  __device__ long long scan(long long x, long long* sum) {
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += up;
+    }
+    __syncthreads();
+    if (lane == 31) warp[wid] = x;
+    __syncthreads();
+    *sum = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) {
+      if (i < wid) x += warp[i];
+      *sum += warp[i];
+    }
+    return x;
+  }
+
+  // Returns the total of units; places the first unit of CTA `cta`'s range, if it has one.
+  __device__ long long find(const CacheView& c, int group, bool causal, int cta, long long* per) {
+    if (threadIdx.x == 0) {
+      at = Place{0, 0, 0, 0};
+      q = SeqInfo{0, 0, 0};
+      first = 0;
+    }
+    long long mine = 0, incl = 0, total = 0, sum;
+    for (int base = 0; base < c.n_seqs; base += kThreads) {
+      const int s = base + threadIdx.x;
+      mine = s < c.n_seqs ? tiles_of(seq_info(c, s), group, causal).units * c.Hkv : 0;
+      incl = total + scan(mine, &sum);
+      total += sum;
+    }
+    *per = units_per_cta(total);
+    const long long unit = cta * *per;
+    if (unit < total) {
+      long long run = 0;
+      for (int base = 0; base < c.n_seqs; base += kThreads) {
+        const int s = base + threadIdx.x;
+        if (c.n_seqs > kThreads) {
+          mine = s < c.n_seqs ? tiles_of(seq_info(c, s), group, causal).units * c.Hkv : 0;
+          incl = run + scan(mine, &sum);
+          run += sum;
+        }
+        if (mine > 0 && unit < incl && unit >= incl - mine) {
+          at.s = s;
+          q = seq_info(c, s);
+          first = incl - mine;
+        }
+      }
+      __syncthreads();
+      if (threadIdx.x < 32) {  // 32 probes at a time for the row tile
+        const SeqTiles t = tiles_of(q, group, causal);
+        long long rel = unit - first;
+        const int head = t.units > 0 ? static_cast<int>(rel / t.units) : 0;
+        rel -= head * t.units;
+        int lo = 0, n = t.tiles;
+        while (n > 1) {
+          const int step = (n + 31) / 32;
+          const int probe = static_cast<int>(threadIdx.x) * step;
+          const bool below = probe < n && t.before(lo + probe, group) <= rel;
+          const int hit = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+          lo += hit * step;
+          n = min(step, n - hit * step);
+        }
+        if (threadIdx.x == 0) {
+          at.head = head;
+          at.j = lo;
+          at.tile = static_cast<int>(rel - t.before(lo, group));
+        }
+      }
+    }
+    __syncthreads();
+    return total;
+  }
+};
+
+// The part of a tile that a CTA works on, walked by every role by itself.
+struct Part {
+  SeqTiles t;
+  Place p;
+  long long left;  // units of the CTA's range from here on
+  int row0, rows;
+  int tile0, tile1;  // its units
+  int n_tiles;       // those that hold keys that a row sees
+  int seen;          // keys that the last row sees
+  bool pair;         // at most 128 rows: the key tiles alternate between the groups
+  bool whole;
+
+  __device__ void start(const Finder& f, int group, bool causal, long long units) {
+    t = tiles_of(f.q, group, causal);
+    p = f.at;
+    left = units;
+    set(group);
+  }
+  __device__ void set(int group) {
+    const int units = t.of(p.j, group);
+    row0 = p.j * kRows;
+    rows = min(kRows, t.rows - row0);
+    tile0 = p.tile;
+    tile1 = static_cast<int>(min(static_cast<long long>(units), tile0 + left));
+    whole = tile0 == 0 && tile1 == units;
+    const int last_token = (row0 + rows - 1) / group;
+    seen = t.causal ? min(t.q.len, max(0, t.q.len - t.q.n + last_token + 1)) : t.q.len;
+    n_tiles = max(0, min(tile1, (seen + kKeys - 1) / kKeys) - tile0);
+    pair = rows <= kHalfRows;
+  }
+  // On to the next part; false at the end of the range.
+  __device__ bool next(const CacheView& c, int group) {
+    left -= tile1 - tile0;
+    if (left <= 0) return false;
+    p.tile = 0;
+    if (++p.j >= t.tiles) {
+      p.j = 0;
+      if (++p.head >= c.Hkv) {
+        p.head = 0;
+        do {
+          if (++p.s >= c.n_seqs) return false;
+          t = tiles_of(seq_info(c, p.s), group, t.causal);
+        } while (t.tiles == 0);
+      }
+    }
+    set(group);
+    return true;
+  }
+};
+
+// ---- waits ----
+
+struct Waits {
+  volatile int* abort_flag;
+  unsigned long long timeout_ns;
+  unsigned* status;
+};
+
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, const Waits& w,
+                                              unsigned cause) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*w.abort_flag) return false;
+    if (globaltimer_ns() - t0 > w.timeout_ns) {
+      *w.abort_flag = 1;
+      atomicOr(w.status, cause);
+      return false;
+    }
+  }
+}
+
+// For this CTA's own copies and products in flight, on the way out.
+__device__ __forceinline__ void wait_out(uint32_t bar, uint32_t parity, const Waits& w) {
+  if (mbar_try_wait(bar, parity)) return;
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (globaltimer_ns() - t0 > w.timeout_ns) {
+      atomicOr(w.status, kStDrain);
+      return;
+    }
+  }
+}
+
+// ---- pieces of the roles ----
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+
+// Four e4m3 values as two words of fp16.
+__device__ __forceinline__ uint2 widen(uint32_t u) {
+  uint2 r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(r.x), "=r"(r.y)
+      : "r"(u));
+  return r;
+}
+
+// 16 bytes of row `row`, piece `piece` (16 columns), into the two 16-byte chunks of the swizzled fp16
+// tile.  The lanes of the second half of a row store their second chunk first: the eight lanes of a
+// phase then reach all banks.
+__device__ __forceinline__ void store_wide(uint32_t tile, int row, int piece, uint4 v) {
+  const uint2 a = widen(v.x), b = widen(v.y), c = widen(v.z), d = widen(v.w);
+  const uint4 w0 = make_uint4(a.x, a.y, b.x, b.y), w1 = make_uint4(c.x, c.y, d.x, d.y);
+  const uint32_t base = tile + (piece >> 2) * (kKeys * 128) + row * 128;
+  const int chunk = (piece & 3) * 2, flip = (piece >> 2) & 1;
+  sts128(base + (((chunk + flip) ^ (row & 7)) * 16), flip ? w1 : w0);
+  sts128(base + (((chunk + 1 - flip) ^ (row & 7)) * 16), flip ? w0 : w1);
+}
+
+__device__ __forceinline__ void load_page(uint32_t dst, const void* map, int pos, int head, int page,
+                                          uint32_t bar) {
+  const int pt = pos & 3, ph = (pos >> 2) & 3;
+  const int c0 = pt == 0 ? 0 : (ph == 0 ? head : page);
+  const int c1 = pt == 1 ? 0 : (ph == 1 ? head : page);
+  const int c2 = pt == 2 ? 0 : (ph == 2 ? head : page);
+  tma_load_4d(dst, map, 0, c0, c1, c2, bar);
+}
+
+__device__ __forceinline__ void value_scale(float s, float* add, float* inv) {
+  s = s != s ? s : fminf(fmaxf(s, 0x1p-64f), 0x1p120f);
+  const int bits = __float_as_int(s);
+  const float mant = __int_as_float((bits & 0x7fffff) | 0x3f800000);
+  *add = static_cast<float>((bits >> 23) - 127) + log2f(mant);
+  *inv = 1.0f / s;
+}
+
+// The 256 threads of the two softmax groups.
+__device__ __forceinline__ void pair_barrier() {
+  asm volatile("bar.sync %0, 256;" ::"n"(kPairBarrier) : "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
+    const __grid_constant__ CacheAttnArgs a, const __grid_constant__ PageMaps maps,
+    float* partials) {
+  using L = Layout<D>;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t sbase = (raw + 1023u) & ~1023u;
+  unsigned char* smem = smem_raw + (sbase - raw);
+  __shared__ Finder finder;
+  RunScale* tables = reinterpret_cast<RunScale*>(smem + L::kTable);
+  volatile int* clean = reinterpret_cast<volatile int*>(smem + L::kClean);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  auto bar = [sbase](int i) -> uint32_t { return sbase + L::kBars + 8u * i; };
+  const CacheView& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int group = a.H / c.Hkv;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  {  // rows behind the last sequence
+    const int live = live_rows(c);
+    const long long n = static_cast<long long>(c.T - live) * a.H;
+    T* o = static_cast<T*>(a.o) + static_cast<long long>(live) * a.H * D;
+    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + tid; i < n * (D / 8);
+         i += static_cast<long long>(gridDim.x) * kThreads) {
+      reinterpret_cast<uint4*>(o)[i] = make_uint4(0, 0, 0, 0);
+      if (i % (D / 8) == 0) a.lse[static_cast<long long>(live) * a.H + i / (D / 8)] = 0.f;
+    }
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(L::kK8Full + i), 1);
+      mbar_init(bar(L::kV8Full + i), 1);
+      mbar_init(bar(L::kK8Empty + i), 4);
+      mbar_init(bar(L::kV8Empty + i), 4);
+      mbar_init(bar(L::kK16Full + i), 4);
+      mbar_init(bar(L::kK16Empty + i), 1);
+      mbar_init(bar(L::kSFull + i), 1);
+      mbar_init(bar(L::kPFull + i), kHalfRows);
+      mbar_init(bar(L::kOFull + i), 1);
+      mbar_init(bar(L::kQFull + i), kHalfRows);
+    }
+    mbar_init(bar(L::kV16Full), 4);
+    mbar_init(bar(L::kV16Empty), 1);
+    for (int i = 0; i < kTables; ++i) mbar_init(bar(L::kTabFull + i), 1);
+    mbar_init(bar(L::kDrain), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  long long per;
+  const long long total = finder.find(c, group, a.causal, blockIdx.x, &per);
+  const long long u_begin = blockIdx.x * per;
+  if (u_begin >= total) return;  // the whole block
+  const long long n_units = min(total - u_begin, per);
+  if (warp == 13) {
+    tmem_alloc(smem_u32(tmem_slot), L::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Waits w{abort_flag, a.timeout_ns, c.status};
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax groups
+    const int g = warp >> 2;
+    const int r = tid & 127;  // tensor-memory lane
+    const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_col = tl + L::kColS + g * 128, o_col = tl + L::kColO + g * 128;
+    unsigned steps_done = 0, tiles_done = 0, parts_done = 0;
+    bool ok = true;
+    Part part;
+    part.start(finder, group, a.causal, n_units);
+    bool first_part = true;
+    do {
+      const SeqInfo& q = part.t.q;
+      const int row = part.pair ? r : g * kHalfRows + r;
+      const bool on = row < part.rows;
+      const int token = on ? (part.row0 + row) / group : 0;
+      const int h = part.p.head * group + (on ? part.row0 + row - token * group : 0);
+      const int limit = on ? (a.causal ? max(0, q.len - q.n + token + 1) : q.len) : 0;
+      const int my_steps = part.pair ? (part.n_tiles - g + 1) / 2 : part.n_tiles;
+      float row_mul = a.scale * kLog2e;
+      float m = -INFINITY, l = 0.f;
+      if (part.n_tiles > 0 && ok) {
+        // This thread's row of Q as fp16, swizzled.
+        const T* src = static_cast<const T*>(a.q) + static_cast<long long>(q.t0 + token) * a.sq[0] +
+                       h * a.sq[1];
+        uint4 v[D / 8];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          v[i] = on ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+        }
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          float big = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = to_float2<T>(u[k]);
+              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+          const int e = big > 0.f && big < INFINITY
+                            ? min(119, max(-118, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 8))
+                            : 0;
+          const float div = __int_as_float((127 - e) << 23);
+          row_mul *= __int_as_float((127 + e) << 23);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            uint32_t* u = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = to_float2<T>(u[k]);
+              u[k] = from_float2<__half>(f.x * div, f.y * div);
+            }
+          }
+        }
+        if (!part.pair || g == 0) {
+          const uint32_t dst = sbase + L::kQ + g * L::kTile16 + r * 128;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            sts128(dst + (i >> 3) * L::kChunkBytes + (((i & 7) ^ (r & 7)) * 16), v[i]);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(bar(L::kQFull + g));
+        }
+      }
+      // The first key that some row of this half does not see.
+      const int first_row = part.pair ? 0 : min(g * kHalfRows, part.rows - 1);
+      const int all_see = a.causal ? q.len - q.n + (part.row0 + first_row) / group + 1 : q.len;
+      for (int k = 0; k < my_steps && ok; ++k) {
+        const int i = part.pair ? 2 * k + g : k;
+        const unsigned at = tiles_done + i;
+        const int slot = at % kTables;
+        ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull) &&
+             wait_or_abort(bar(L::kSFull + g), steps_done & 1, w, kStSFull);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++steps_done;
+        tc_fence_after();
+        const RunScale* table = tables + slot * kGroups;
+        const int key0 = (part.tile0 + i) * kKeys;
+        const bool masked = key0 + kKeys > all_see || !clean[slot];
+        // Half a row at a time: both halves' maximum, then the second half's weights (still in
+        // registers) over its own scores, then the first half's, read again, next to them.
+        uint32_t u[64];
+        auto load_half = [&](int half) {
+          tmem_ld64_wait(s_col + 64 * half, u);
+          if (masked) {
+            const int lim = limit - key0 - 64 * half;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int lx = table[4 * half + x].page < 0 ? 0 : lim;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                if (16 * x + j >= lx) u[16 * x + j] = 0xff800000u;  // -inf
+              }
+            }
+          }
+        };
+        float top = m;
+        auto max_half = [&](int half) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              b[j] = fmaxf(__uint_as_float(u[16 * x + 4 * j]), __uint_as_float(u[16 * x + 4 * j + 1]));
+              b[j] = fmax3(b[j], __uint_as_float(u[16 * x + 4 * j + 2]),
+                           __uint_as_float(u[16 * x + 4 * j + 3]));
+            }
+            const RunScale sc = table[4 * half + x];
+            const float mul = fmaxf(sc.mul * row_mul, 1.1754944e-38f);
+            top = fmaxf(top, fmaf(fmax3(b[0], b[1], fmaxf(b[2], b[3])), mul, sc.add));
+          }
+        };
+        float ref, part_l = 0.f;
+        auto exp_half = [&](int half) {
+#pragma unroll
+          for (int x = 0; x < 4; x += 2) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const RunScale sc = table[4 * half + x + y];
+              const float mul = fmaxf(sc.mul * row_mul, 1.1754944e-38f);
+              const uint64_t mul2 = f2_pack(mul, mul);
+              const uint64_t add2 = f2_pack(sc.add - ref, sc.add - ref);
+              uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int at2 = 16 * (x + y) + 2 * j;
+                const uint64_t z = f2_fma(
+                    f2_pack(__uint_as_float(u[at2]), __uint_as_float(u[at2 + 1])), mul2, add2);
+                const float p0 = ex2_approx(f2_lo(z)), p1 = ex2_approx(f2_hi(z));
+                pk[8 * y + j] = pack2<__half>(p0, p1);
+                sum[j & 1] = f2_add(sum[j & 1], f2_pack(p0, p1));
+              }
+              const uint64_t both = f2_add(sum[0], sum[1]);
+              part_l = fmaf(f2_lo(both) + f2_hi(both), sc.inv, part_l);
+            }
+            tmem_st16(s_col + 64 + 32 * half + 8 * x, pk);
+          }
+        };
+        load_half(0);
+        max_half(0);
+        load_half(1);
+        max_half(1);
+        const bool moved = top > m + kLazy || (m == -INFINITY && top != -INFINITY);
+        const float alpha = moved ? (m == -INFINITY ? 0.f : ex2_approx(m - top)) : 1.f;
+        if (moved) m = top;
+        ref = m == -INFINITY ? 0.f : m;
+        exp_half(1);
+        load_half(0);
+        exp_half(0);
+        l = fmaf(l, alpha, part_l);
+        tmem_st_wait();
+        // S_g of this step completing implies that the O of the step before is complete.
+        if (k > 0 && __any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int col = 0; col < D; col += 32) {
+            uint32_t o[32];
+            tmem_ld32_wait(o_col + col, o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st32(o_col + col, o);
+          }
+          tmem_st_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(bar(L::kPFull + g));
+      }
+      tiles_done += part.n_tiles;
+      if (my_steps > 0 && ok) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kOFull + g), parts_done & 1, w, kStODone));
+        ++parts_done;
+        tc_fence_after();
+      }
+      // Alternating tiles: group 0 merges.  Both groups' sums of a row are in one lane of tensor
+      // memory; (m, l) of group 1 go there too, over its scores.  Both groups come to each of these
+      // barriers, whatever went wrong.
+      const bool merge = part.pair && part.n_tiles > 1;
+      float m1 = -INFINITY, l1 = 0.f;
+      if (merge) {
+        if (g == 1) {
+          const uint32_t ml[8] = {__float_as_uint(m), __float_as_uint(l), 0, 0, 0, 0, 0, 0};
+          tmem_st8(s_col, ml);
+          tmem_st_wait();
+          tc_fence_before();
+        }
+        pair_barrier();
+        if (g == 0) {
+          tc_fence_after();
+          uint32_t ml[32];
+          tmem_ld32_wait(tl + L::kColS + 128, ml);
+          m1 = __uint_as_float(ml[0]);
+          l1 = __uint_as_float(ml[1]);
+        }
+      }
+      // Tensor-memory loads are by the warp: rows that are off take part and store nothing.
+      if (ok && (!part.pair || g == 0)) {
+        const float top = fmaxf(m, m1);
+        const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - top);
+        const float f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - top);
+        // A row whose scores are all NaN has no maximum but a sum that is NaN.
+        const float lsum = (m == -INFINITY ? l : l * f0) + (m1 == -INFINITY ? l1 : l1 * f1);
+        const float w0 = lsum != lsum ? lsum : f0, w1 = lsum != lsum ? lsum : f1;
+        const float inv = part.whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
+        const long long at = static_cast<long long>(q.t0 + token) * a.H + h;
+        float* slot = partials + (2ll * blockIdx.x + (first_part ? 0 : 1)) * L::kPartial;
+#pragma unroll
+        for (int col = 0; col < D; col += 32) {
+          uint32_t u[32];
+          __syncwarp();
+          if (my_steps > 0) {
+            tmem_ld32_wait(o_col + col, u);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) u[j] = 0;
+          }
+          float o[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(u[j]) * w0;
+          if (merge) {
+            tmem_ld32_wait(o_col + 128 + col, u);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(u[j]), w1, o[j]);
+          }
+          if (on && part.whole) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at * D + col);
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              uint4 x;
+              x.x = from_float2<T>(o[j] * inv, o[j + 1] * inv);
+              x.y = from_float2<T>(o[j + 2] * inv, o[j + 3] * inv);
+              x.z = from_float2<T>(o[j + 4] * inv, o[j + 5] * inv);
+              x.w = from_float2<T>(o[j + 6] * inv, o[j + 7] * inv);
+              dst[j / 8] = x;
+            }
+          } else if (on) {
+            float4* dst = reinterpret_cast<float4*>(slot + row * D + col);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) dst[j / 4] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          }
+        }
+        if (on && part.whole) {
+          a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
+        } else if (on) {
+          slot[kRows * D + row] = top;
+          slot[kRows * D + kRows + row] = lsum;
+        }
+      }
+      if (merge) pair_barrier();  // group 1's sums were read
+      first_part = false;
+    } while (part.next(c, group));
+  } else if (warp < 12) {
+    // ---------------------------------------------------------------- conversion
+    constexpr int kPieces = D / 16, kStep = 128 / kPieces;
+    const int t = tid & 127;
+    const int piece = t % kPieces, row0 = t / kPieces;
+    unsigned n = 0;  // tiles converted
+    bool ok = true;
+    Part part;
+    part.start(finder, group, a.causal, n_units);
+    do {
+      for (int i = 0; i < part.n_tiles && ok; ++i, ++n) {
+        const int st = n & 1;
+        const uint32_t ph = (n >> 1) & 1;
+        // K
+        ok = wait_or_abort(bar(L::kK8Full + st), ph, w, kStKFull) &&
+             (n < 2 || wait_or_abort(bar(L::kK16Empty + st), ph ^ 1, w, kStKVEmpty));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        {
+          const uint32_t src = sbase + L::kK8 + st * L::kTile8 + t * 16;
+          const uint32_t dst = sbase + L::kK16 + st * L::kTile16;
+#pragma unroll
+          for (int x = 0; x < kPieces; ++x) {
+            store_wide(dst, row0 + x * kStep, piece, lds128(src + x * 2048));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(L::kK16Full + st));
+          mbar_arrive(bar(L::kK8Empty + st));
+        }
+        // V
+        ok = wait_or_abort(bar(L::kV8Full + st), ph, w, kStVFull) &&
+             (n < 1 || wait_or_abort(bar(L::kV16Empty), (n - 1) & 1, w, kStKVEmpty));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        {
+          const int slot = n % kTables;
+          const bool all = clean[slot];
+          const int left = part.t.q.len - (part.tile0 + i) * kKeys;  // keys that are there
+          const uint32_t src = sbase + L::kV8 + st * L::kTile8 + t * 16;
+          const uint32_t dst = sbase + L::kV16;
+#pragma unroll
+          for (int x = 0; x < kPieces; ++x) {
+            const int row = row0 + x * kStep;
+            uint4 v = lds128(src + x * 2048);
+            // Behind the last key a page holds anything, and 0 times that must be 0.
+            if (!all && (row >= left || tables[slot * kGroups + (row >> 4)].page < 0)) {
+              v = make_uint4(0, 0, 0, 0);
+            }
+            store_wide(dst, row, piece, v);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(L::kV16Full));
+          mbar_arrive(bar(L::kV8Empty + st));
+        }
+      }
+    } while (ok && part.next(c, group));
+  } else {
+    if (warp == 12) {
+      // -------------------------------------------------------------- pages
+      // Lane 8 b + x looks after 16 keys (run x) of tile b of four; pages are looked up four tiles
+      // ahead, their scales a tile later.
+      const int rows_page = 1 << c.page_shift;
+      const int x = lane & 7;
+      const bool leads = ((16 * x) & (rows_page - 1)) == 0;  // the run starts a page
+      const unsigned bytes = static_cast<unsigned>(rows_page) * D;
+      unsigned n = 0;  // tiles
+      unsigned k_sent = 0, v_sent = 0;
+      bool ok = true;
+      Part part;
+      part.start(finder, group, a.causal, n_units);
+      do {
+        const int keys_end = min(part.t.q.len, (part.tile0 + part.n_tiles) * kKeys);
+        const int head = part.p.head;
+        auto page_at = [&](int i) {
+          const int key = (part.tile0 + i + (lane >> 3)) * kKeys + 16 * x;
+          return key < keys_end ? page_of(c, part.p.s, key >> c.page_shift) : -1;
+        };
+        float sk = 0.f, sv = 1.f;
+        auto read_scales = [&](int page) {
+          if (page >= 0) {
+            const long long at = static_cast<long long>(page) * c.Hkv + head;
+            sk = __ldg(c.k_scale + at);
+            sv = __ldg(c.v_scale + at);
+          }
+        };
+        int next_page = part.n_tiles > 0 ? page_at(0) : -1;
+        read_scales(next_page);
+        RunScale sc = {0.f, 0.f, 0.f, -1};
+        for (int i = 0; i < part.n_tiles && ok; ++i, ++n) {
+          if ((i & 3) == 0) {
+            sc.page = next_page;
+            sc.mul = sk;
+            value_scale(sv, &sc.add, &sc.inv);
+            next_page = page_at(i + 4);
+          }
+          if ((i & 3) == 1) read_scales(next_page);
+          const int st = n & 1;
+          const uint32_t ph = (n >> 1) & 1;
+          if (n >= 2) {
+            ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kK8Empty + st), ph ^ 1, w, kStKVEmpty));
+            if (!ok) break;
+          }
+          const int slot = n % kTables;
+          const bool mine = (lane >> 3) == (i & 3);
+          if (mine) tables[slot * kGroups + x] = sc;
+          const unsigned there = __ballot_sync(0xffffffffu, mine && sc.page >= 0);
+          const unsigned copies = __ballot_sync(0xffffffffu, mine && sc.page >= 0 && leads);
+          const bool all = __popc(there) == kGroups &&
+                           (part.tile0 + i + 1) * kKeys <= part.t.q.len;
+          if (lane == 0) {
+            clean[slot] = all;
+            const unsigned sum = __popc(copies) * bytes;
+            if (sum > 0) {
+              mbar_arrive_expect_tx(bar(L::kK8Full + st), sum);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar(L::kTabFull + slot));
+            if (copies == 0) mbar_arrive(bar(L::kK8Full + st));
+          }
+          if (mine && sc.page >= 0 && leads) {
+            load_page(sbase + L::kK8 + st * L::kTile8 + 16 * x * D, &maps.k, maps.k_pos, head, sc.page,
+                      bar(L::kK8Full + st));
+          }
+          ++k_sent;
+          __syncwarp();
+          if (n >= 2) {
+            ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kV8Empty + st), ph ^ 1, w, kStKVEmpty));
+            if (!ok) break;
+          }
+          if (lane == 0) {
+            const unsigned sum = __popc(copies) * bytes;
+            if (sum > 0) {
+              mbar_arrive_expect_tx(bar(L::kV8Full + st), sum);
+            } else {
+              mbar_arrive(bar(L::kV8Full + st));
+            }
+          }
+          __syncwarp();
+          if (mine && sc.page >= 0 && leads) {
+            load_page(sbase + L::kV8 + st * L::kTile8 + 16 * x * D, &maps.v, maps.v_pos, head, sc.page,
+                      bar(L::kV8Full + st));
+          }
+          ++v_sent;
+        }
+      } while (ok && part.next(c, group));
+      // Every copy that was started lands before the block ends.
+      for (unsigned i = k_sent > 2 ? k_sent - 2 : 0; i < k_sent; ++i) {
+        wait_out(bar(L::kK8Full + (i & 1)), (i >> 1) & 1, w);
+      }
+      for (unsigned i = v_sent > 2 ? v_sent - 2 : 0; i < v_sent; ++i) {
+        wait_out(bar(L::kV8Full + (i & 1)), (i >> 1) & 1, w);
+      }
+    } else if (warp == 13 && lane == 0) {
+      // -------------------------------------------------------------- products
+      constexpr uint32_t kIdescS = idesc_mma(0, 128, kKeys, false);
+      constexpr uint32_t kIdescPV = idesc_mma(0, 128, D, true);
+      const uint64_t q_desc = sdesc_sw128(sbase + L::kQ, 16, 1024);
+      const uint64_t k_desc = sdesc_sw128(sbase + L::kK16, 16, 1024);
+      const uint64_t v_desc = sdesc_sw128(sbase + L::kV16, L::kChunkBytes, 1024);
+      unsigned tiles_done = 0;
+      unsigned q_done[2] = {0, 0}, p_done[2] = {0, 0};
+      bool ok = true;
+      Part part;
+      part.start(finder, group, a.causal, n_units);
+      do {
+        const bool pair = part.pair;
+        const int n_steps = pair ? part.n_tiles : 2 * part.n_tiles;
+        if (n_steps == 0) continue;
+        auto issue_s = [&](int i) -> bool {
+          const int g = i & 1;
+          const unsigned tile = tiles_done + (pair ? i : i >> 1);
+          const int st = tile & 1;
+          if (pair || g == 0) {
+            if (!wait_or_abort(bar(L::kK16Full + st), (tile >> 1) & 1, w, kStKFull)) return false;
+          }
+          tc_fence_after();
+          const uint64_t qd = q_desc + ((pair ? 0 : g * L::kTile16) >> 4);
+          const uint64_t kd = k_desc + ((st * L::kTile16) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk / 4) * L::kChunkBytes + (kk % 4) * 32;
+            umma_ss(tmem + L::kColS + g * 128, qd + (off >> 4), kd + (off >> 4), kIdescS, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(bar(L::kSFull + g));
+          if (pair || g == 1) umma_commit(bar(L::kK16Empty + st));
+          return true;
+        };
+        ok = wait_or_abort(bar(L::kQFull), q_done[0]++ & 1, w, kStQFull);
+        if (ok && !pair) ok = wait_or_abort(bar(L::kQFull + 1), q_done[1]++ & 1, w, kStQFull);
+        for (int i = 0; ok && i < 2 && i < n_steps; ++i) ok = issue_s(i);
+        for (int i = 0; ok && i < n_steps; ++i) {
+          const int g = i & 1;
+          const unsigned tile = tiles_done + (pair ? i : i >> 1);
+          ok = wait_or_abort(bar(L::kPFull + g), p_done[g]++ & 1, w, kStPFull);
+          if (ok && (pair || g == 0)) ok = wait_or_abort(bar(L::kV16Full), tile & 1, w, kStVFull);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk) {
+            umma_ts(tmem + L::kColO + g * 128, tmem + L::kColS + g * 128 + 64 + 8 * kk,
+                    v_desc + ((kk * 2048) >> 4), kIdescPV, (i > 1 || kk > 0) ? 1u : 0u);
+          }
+          if (pair || g == 1) umma_commit(bar(L::kV16Empty));
+          if (i + 2 < n_steps) {
+            ok = issue_s(i + 2);
+          } else {
+            umma_commit(bar(L::kOFull + g));
+          }
+        }
+        tiles_done += part.n_tiles;
+      } while (ok && part.next(c, group));
+      umma_commit(bar(L::kDrain));
+      wait_out(bar(L::kDrain), 0, w);
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 13) tmem_dealloc(tmem, L::kCols);
+}
+
+// Merges the parts of a tile that several CTAs share.  Block i looks after the tile that CTA i's range
+// begins inside of, if no earlier CTA's does too; a warp for each row.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) fa_cache_tile_merge_kernel(
+    const __grid_constant__ CacheAttnArgs a, const float* partials) {
+  using L = Layout<D>;
+  constexpr int kPer = D / 32, kWarps = kThreads / 32, kBatch = 4;
+  __shared__ Finder finder;
+  const CacheView& c = a.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = a.H / c.Hkv;
+  const int me = blockIdx.x;
+  long long per;
+  const long long total = finder.find(c, group, a.causal, me, &per);
+  const long long begin = me * per;
+  if (me == 0 || begin >= total) return;
+  const Place p = finder.at;
+  if (p.tile == 0 || p.tile > per) return;
+  const SeqTiles t = tiles_of(finder.q, group, a.causal);
+  const long long first = begin - p.tile, end = first + t.of(p.j, group);
+  const int last = static_cast<int>((end - 1) / per);  // the last CTA with a part
+  const int row0 = p.j * kRows, rows = min(kRows, t.rows - row0);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int row = warp; row < rows; row += kWarps) {
+    float top = -INFINITY, lsum = 0.f, acc[kPer] = {};
+    for (int i0 = me - 1; i0 <= last; i0 += kBatch) {
+      float pm[kBatch], pl[kBatch], v[kBatch][kPer];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        pm[b] = -INFINITY;
+        pl[b] = 0.f;
+        if (i0 + b <= last) {
+          const int slot = (i0 + b) * per >= first ? 0 : 1;
+          const float* part = partials + (2ll * (i0 + b) + slot) * L::kPartial;
+          pm[b] = part[kRows * D + row];
+          pl[b] = part[kRows * D + kRows + row];
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) v[b][k] = part[row * D + lane * kPer + k];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (pm[b] == -INFINITY && pl[b] == 0.f) continue;
+        const float to = fmaxf(top, pm[b]);
+        const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - to);
+        const float f1 = pm[b] == -INFINITY ? 1.f : ex2_approx(pm[b] - to);
+        top = to;
+        lsum = lsum * f0 + pl[b] * f1;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f0 + v[b][k] * f1;
+      }
+    }
+    const int token = (row0 + row) / group;
+    const long long at = static_cast<long long>(t.q.t0 + token) * a.H + p.head * group +
+                         (row0 + row - token * group);
+    const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+    uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + at * D + lane * kPer);
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) o[k / 2] = from_float2<T>(acc[k] * inv, acc[k + 1] * inv);
+    if (lane == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
+  using L = Layout<D>;
+  const CacheView& c = a.c;
+  const int group = a.H / c.Hkv;
+  // No more CTAs than units that the table could hold.
+  const long long room = static_cast<long long>(c.max_pages) << c.page_shift;
+  const long long units = std::max(1ll, (room + kKeys - 1) / kKeys);
+  const long long tiles = (static_cast<long long>(c.T) * group / kRows + c.n_seqs) * c.Hkv;
+  const long long want = tiles > (1ll << 40) / units ? (1ll << 40) : tiles * units;
+  const unsigned ctas =
+      static_cast<unsigned>(std::max(1ll, std::min<long long>(multiprocessors(), want)));
+  float* partials = static_cast<float*>(a.workspace);
+  PageMaps maps;
+  cudaError_t e = make_page_maps(&maps, c, D, 1 << c.page_shift, false);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(fa_cache_tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           L::kBytes);
+  if (e != cudaSuccess) return e;
+  fa_cache_tile_kernel<T, D><<<ctas, kThreads, L::kBytes, stream>>>(a, maps, partials);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  if (units == 1) return cudaSuccess;  // no tile has two units
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fa_cache_tile_merge_kernel<T, D>, a,
+                            static_cast<const float*>(partials));
+}
+
+}  // namespace
+
+size_t cache_tile_workspace(int D, int sms) {
+  const size_t floats = D == 64 ? Layout<64>::kPartial : Layout<128>::kPartial;
+  return 2 * sizeof(float) * static_cast<size_t>(sms) * floats;
+}
+
+cudaError_t launch_cache_tile(const CacheAttnArgs& a, cudaStream_t stream) {
+  if (a.dtype == FA_DTYPE_F16) {
+    return a.D == 64 ? launch_t<__half, 64>(a, stream) : launch_t<__half, 128>(a, stream);
+  }
+  return a.D == 64 ? launch_t<__nv_bfloat16, 64>(a, stream)
+                   : launch_t<__nv_bfloat16, 128>(a, stream);
+}
+
+}  // namespace fa_sm100

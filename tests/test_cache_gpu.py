@@ -342,6 +342,43 @@ def test_attention_layouts_agree():
     assert torch.equal(o3, o) and torch.equal(lse3, lse)
 
 
+@pytest.mark.parametrize("new,H", [(1, 2), (1, 12), (9, 4)])
+def test_attention_long_sequences(new, H):
+    """Enough keys that each CTA walks many pages of one sequence, against fp64 on the GPU."""
+    Hkv, D, page, lens = 1, 64, 16, [1300000, 1234, 5, 600001]
+    counts = [-(-n // page) for n in lens]
+    P = sum(counts)
+    g = torch.Generator(device="cuda").manual_seed(31)
+    pools = [torch.randn(P, Hkv, page, D, generator=g, device="cuda").to(E4M3) for _ in range(2)]
+    scales = [torch.exp2(torch.randint(-2, 3, (P, Hkv), generator=g, device="cuda").float()) for _ in range(2)]
+    order = torch.randperm(P, generator=g, device="cuda").int()
+    table = torch.full((4, max(counts)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for s, n in enumerate(counts):
+        table[s, :n] = order[at:at + n]
+        at += n
+    q = torch.randn(4 * new, H, D, generator=g, device="cuda").half()
+    o, lse = fused_attn.cache_attention(q, *pools, *scales, table, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                                        return_lse=True)
+    for s, n in enumerate(lens):
+        ids = table[s, :counts[s]].long()
+        k, v = (x.view(torch.uint8)[ids].view(E4M3).double() * sc[ids].double()[..., None, None]
+                for x, sc in zip(pools, scales))
+        k, v = k.reshape(-1, D)[:n], v.reshape(-1, D)[:n]
+        for i in range(new):
+            seen = max(0, n - new + i + 1)
+            a = q[s * new + i].double() @ k[:seen].T / 8
+            if seen == 0:
+                assert bool((lse[s * new + i] == math.inf).all())
+                continue
+            want = torch.softmax(a, -1)
+            room = want @ v[:seen].abs() * 2.0**-10 + 1e-6
+            want_o = want @ v[:seen]
+            assert bool(((o[s * new + i].double() - want_o).abs() <= room + want_o.abs() * 2.0**-11).all())
+            assert bool(((lse[s * new + i].double() - torch.logsumexp(a, -1)).abs() < 1e-4).all())
+    assert fused_attn.last_device_error() == (0, 0)
+
+
 def test_attention_repeats_bit_for_bit():
     s = Setup([3000, 1, 700, 2500], [1, 1, 3, 40], seed=19, page=64)
     o, lse = s.attend()
