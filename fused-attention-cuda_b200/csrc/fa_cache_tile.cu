@@ -17,7 +17,7 @@
 //                alternate, and their sums are merged at the end (both lie in one lane of tensor memory).  Either way step i belongs to group
 //                i & 1, and the tensor core works for one group while the other exponentiates.
 //
-// S_g takes 128 columns of tensor memory, P_g (fp16) overwrites the last 64, O_g takes D.
+// S_g takes 128 columns of tensor memory, P_g (fp16) overwrites the first 64, O_g takes D.
 #include <algorithm>
 #include <cmath>
 
@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax groups
+    regs_alloc<184>();  // 2 x 128 x 184 + 128 x 80 + 128 x 64 = 512 x 128
     const int g = warp >> 2;
     const int r = tid & 127;  // tensor-memory lane
     const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -516,87 +517,74 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         const int i = part.pair ? 2 * k + g : k;
         const unsigned at = tiles_done + i;
         const int slot = at % kTables;
-        ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull) &&
-             wait_or_abort(bar(L::kSFull + g), steps_done & 1, w, kStSFull);
+        ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull);
+        const RunScale* table = tables + slot * kGroups;
+        float mul[kGroups], add[kGroups];
+        if (ok) {
+#pragma unroll
+          for (int x = 0; x < kGroups; ++x) {
+            mul[x] = fmaxf(table[x].mul * row_mul, 1.1754944e-38f);
+            add[x] = table[x].add;
+          }
+          ok = wait_or_abort(bar(L::kSFull + g), steps_done & 1, w, kStSFull);
+        }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++steps_done;
         tc_fence_after();
-        const RunScale* table = tables + slot * kGroups;
         const int key0 = (part.tile0 + i) * kKeys;
-        const bool masked = key0 + kKeys > all_see || !clean[slot];
-        // Half a row at a time: both halves' maximum, then the second half's weights (still in
-        // registers) over its own scores, then the first half's, read again, next to them.
-        uint32_t u[64];
-        auto load_half = [&](int half) {
-          tmem_ld64_wait(s_col + 64 * half, u);
-          if (masked) {
-            const int lim = limit - key0 - 64 * half;
+        uint32_t u[kKeys];
+        tmem_ld2x64_wait(s_col, u);
+        if (key0 + kKeys > all_see || !clean[slot]) {
+          const int lim = limit - key0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int lx = table[4 * half + x].page < 0 ? 0 : lim;
+          for (int x = 0; x < kGroups; ++x) {
+            const int lx = table[x].page < 0 ? 0 : lim;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                if (16 * x + j >= lx) u[16 * x + j] = 0xff800000u;  // -inf
-              }
+            for (int j = 0; j < 16; ++j) {
+              if (16 * x + j >= lx) u[16 * x + j] = 0xff800000u;  // -inf
             }
           }
-        };
+        }
         float top = m;
-        auto max_half = [&](int half) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            float b[4];
+        for (int x = 0; x < kGroups; ++x) {
+          float b[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              b[j] = fmaxf(__uint_as_float(u[16 * x + 4 * j]), __uint_as_float(u[16 * x + 4 * j + 1]));
-              b[j] = fmax3(b[j], __uint_as_float(u[16 * x + 4 * j + 2]),
-                           __uint_as_float(u[16 * x + 4 * j + 3]));
-            }
-            const RunScale sc = table[4 * half + x];
-            const float mul = fmaxf(sc.mul * row_mul, 1.1754944e-38f);
-            top = fmaxf(top, fmaf(fmax3(b[0], b[1], fmaxf(b[2], b[3])), mul, sc.add));
+          for (int j = 0; j < 4; ++j) {
+            b[j] = fmaxf(__uint_as_float(u[16 * x + 4 * j]), __uint_as_float(u[16 * x + 4 * j + 1]));
+            b[j] = fmax3(b[j], __uint_as_float(u[16 * x + 4 * j + 2]),
+                         __uint_as_float(u[16 * x + 4 * j + 3]));
           }
-        };
-        float ref, part_l = 0.f;
-        auto exp_half = [&](int half) {
-#pragma unroll
-          for (int x = 0; x < 4; x += 2) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const RunScale sc = table[4 * half + x + y];
-              const float mul = fmaxf(sc.mul * row_mul, 1.1754944e-38f);
-              const uint64_t mul2 = f2_pack(mul, mul);
-              const uint64_t add2 = f2_pack(sc.add - ref, sc.add - ref);
-              uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const int at2 = 16 * (x + y) + 2 * j;
-                const uint64_t z = f2_fma(
-                    f2_pack(__uint_as_float(u[at2]), __uint_as_float(u[at2 + 1])), mul2, add2);
-                const float p0 = ex2_approx(f2_lo(z)), p1 = ex2_approx(f2_hi(z));
-                pk[8 * y + j] = pack2<__half>(p0, p1);
-                sum[j & 1] = f2_add(sum[j & 1], f2_pack(p0, p1));
-              }
-              const uint64_t both = f2_add(sum[0], sum[1]);
-              part_l = fmaf(f2_lo(both) + f2_hi(both), sc.inv, part_l);
-            }
-            tmem_st16(s_col + 64 + 32 * half + 8 * x, pk);
-          }
-        };
-        load_half(0);
-        max_half(0);
-        load_half(1);
-        max_half(1);
+          top = fmaxf(top, fmaf(fmax3(b[0], b[1], fmaxf(b[2], b[3])), mul[x], add[x]));
+        }
         const bool moved = top > m + kLazy || (m == -INFINITY && top != -INFINITY);
         const float alpha = moved ? (m == -INFINITY ? 0.f : ex2_approx(m - top)) : 1.f;
         if (moved) m = top;
-        ref = m == -INFINITY ? 0.f : m;
-        exp_half(1);
-        load_half(0);
-        exp_half(0);
-        l = fmaf(l, alpha, part_l);
+        const float ref = m == -INFINITY ? 0.f : m;
+        l *= alpha;
+#pragma unroll
+        for (int x = 0; x < kGroups; x += 2) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint64_t mul2 = f2_pack(mul[x + y], mul[x + y]);
+            const uint64_t add2 = f2_pack(add[x + y] - ref, add[x + y] - ref);
+            uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int at2 = 16 * (x + y) + 2 * j;
+              const uint64_t z =
+                  f2_fma(f2_pack(__uint_as_float(u[at2]), __uint_as_float(u[at2 + 1])), mul2, add2);
+              const float p0 = ex2_approx(f2_lo(z)), p1 = ex2_approx(f2_hi(z));
+              pk[8 * y + j] = pack2<__half>(p0, p1);
+              sum[j & 1] = f2_add(sum[j & 1], f2_pack(p0, p1));
+            }
+            const uint64_t both = f2_add(sum[0], sum[1]);
+            l = fmaf(f2_lo(both) + f2_hi(both), table[x + y].inv, l);
+          }
+          tmem_st16(s_col + 8 * x, pk);
+        }
         tmem_st_wait();
         // S_g of this step completing implies that the O of the step before is complete.
         if (k > 0 && __any_sync(0xffffffffu, moved)) {
@@ -698,6 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
     } while (part.next(c, group));
   } else if (warp < 12) {
     // ---------------------------------------------------------------- conversion
+    regs_dealloc<80>();
     constexpr int kPieces = D / 16, kStep = 128 / kPieces;
     const int t = tid & 127;
     const int piece = t % kPieces, row0 = t / kPieces;
@@ -717,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         {
           const uint32_t src = sbase + L::kK8 + st * L::kTile8 + t * 16;
           const uint32_t dst = sbase + L::kK16 + st * L::kTile16;
-#pragma unroll
+#pragma unroll 2
           for (int x = 0; x < kPieces; ++x) {
             store_wide(dst, row0 + x * kStep, piece, lds128(src + x * 2048));
           }
@@ -739,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           const int left = part.t.q.len - (part.tile0 + i) * kKeys;  // keys that are there
           const uint32_t src = sbase + L::kV8 + st * L::kTile8 + t * 16;
           const uint32_t dst = sbase + L::kV16;
-#pragma unroll
+#pragma unroll 2
           for (int x = 0; x < kPieces; ++x) {
             const int row = row0 + x * kStep;
             uint4 v = lds128(src + x * 2048);
@@ -759,6 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       }
     } while (ok && part.next(c, group));
   } else {
+    regs_dealloc<64>();
     if (warp == 12) {
       // -------------------------------------------------------------- pages
       // Lane 8 b + x looks after 16 keys (run x) of tile b of four; pages are looked up four tiles
@@ -903,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < kKeys / 16; ++kk) {
-            umma_ts(tmem + L::kColO + g * 128, tmem + L::kColS + g * 128 + 64 + 8 * kk,
+            umma_ts(tmem + L::kColO + g * 128, tmem + L::kColS + g * 128 + 8 * kk,
                     v_desc + ((kk * 2048) >> 4), kIdescPV, (i > 1 || kk > 0) ? 1u : 0u);
           }
           if (pair || g == 1) umma_commit(bar(L::kV16Empty));
