@@ -110,7 +110,7 @@ EncodeTiledFn encode_fn() {
 }
 
 cudaError_t page_map(CUtensorMap* m, int* pos, void* base, const long long st[3],
-                     const CacheView& c, int D, int rows, bool swizzled) {
+                     const CacheView& c, int D, int rows) {
   const EncodeTiledFn enc = encode_fn();
   if (enc == nullptr) return cudaErrorNotSupported;
   const long long stride[3] = {st[2], st[1], st[0]};  // token, head, page
@@ -137,18 +137,16 @@ cudaError_t page_map(CUtensorMap* m, int* pos, void* base, const long long st[3]
   const CUresult r =
       enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, estride,
           CU_TENSOR_MAP_INTERLEAVE_NONE,
-          !swizzled  ? CU_TENSOR_MAP_SWIZZLE_NONE
-          : D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                     : CU_TENSOR_MAP_SWIZZLE_64B,
+          D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows, bool swizzled) {
-  const cudaError_t e = page_map(&m->k, &m->k_pos, c.k, c.ks, c, D, rows, swizzled);
-  return e != cudaSuccess ? e : page_map(&m->v, &m->v_pos, c.v, c.vs, c, D, rows, swizzled);
+cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows) {
+  const cudaError_t e = page_map(&m->k, &m->k_pos, c.k, c.ks, c, D, rows);
+  return e != cudaSuccess ? e : page_map(&m->v, &m->v_pos, c.v, c.vs, c, D, rows);
 }
 
 int multiprocessors() {

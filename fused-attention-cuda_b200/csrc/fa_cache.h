@@ -74,8 +74,8 @@ struct PageMaps {
   CUtensorMap k, v;
   int k_pos, v_pos;
 };
-// Boxes of `rows` tokens, swizzled by the row's D bytes or row after row.
-cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows, bool swizzled);
+// Boxes of `rows` tokens, swizzled by the row's D bytes.
+cudaError_t make_page_maps(PageMaps* m, const CacheView& c, int D, int rows);
 
 // Multiprocessors of the current device (148 when the query fails).
 int multiprocessors();

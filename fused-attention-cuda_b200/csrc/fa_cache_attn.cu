@@ -769,7 +769,7 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
   const unsigned ctas = static_cast<unsigned>(std::max(1ll, want));
   float* partials = static_cast<float*>(a.workspace);
   PageMaps maps;
-  cudaError_t e = make_page_maps(&maps, c, D, kRun, true);
+  cudaError_t e = make_page_maps(&maps, c, D, kRun);
   if (e != cudaSuccess) return e;
   e = cudaFuncSetAttribute(fa_cache_decode_kernel<T, D, NT>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);

@@ -7,17 +7,23 @@
 // (one unit of work).  The units of all sequences are numbered and split evenly over one CTA for each
 // multiprocessor; a tile that several CTAs share leaves fp32 partials for fa_cache_tile_merge_kernel.
 //
-//   warp 12      looks pages and scales up, loads e4m3 pages by TMA (two tiles of K and V in flight)
-//   warps 8-11   convert a tile to fp16 into the swizzled layout of the products (exact; K in two
-//                buffers, V in one): tcgen05 has no product of fp16 by e4m3, and rounding q and P to
-//                8 bits would cost what the cache's own 8 bits cost again
+//   warp 12      looks pages and scales up
+//   warps 8-11   load e4m3 pages into registers, a tile ahead, and store them as fp16 in the swizzled
+//                layout of the products (exact; two buffers of K and of V): tcgen05 has no product of
+//                fp16 by e4m3, and rounding q and P to 8 bits would cost what the cache's own 8 bits
+//                cost again.  Registers and not TMA: a tile in flight takes no shared memory, which
+//                the fp16 buffers fill (with e4m3 tiles in shared memory V had one buffer, and its
+//                conversion, 1100 cycles, stood between two products: 608 us at 2048 x 16384 keys)
 //   warp 13      issues S = Q K^T and O += P V
 //   warps 0-3, 4-7   two softmax groups, a row to a thread.  With more than 128 rows group g has rows
 //                128 g .. and every key tile; otherwise both have the same rows and the key tiles
 //                alternate, and their sums are merged at the end (both lie in one lane of tensor memory).  Either way step i belongs to group
 //                i & 1, and the tensor core works for one group while the other exponentiates.
 //
-// S_g takes 128 columns of tensor memory, P_g (fp16) overwrites the first 64, O_g takes D.
+// A key tile goes through in two halves of 64 keys: S_g has two buffers of 64 columns in tensor memory,
+// P_g (fp16) overwrites the first 32 of its own, O_g takes D.  While a group exponentiates one half
+// the products of the other are under way.  (With one S of 128 columns a group waited for its PV and its
+// next S, 1800 of 5900 cycles.)
 #include <algorithm>
 #include <cmath>
 
@@ -43,30 +49,30 @@ struct Layout {
   static constexpr int kChunks = D / 64;             // 128-byte column chunks of an fp16 tile
   static constexpr int kChunkBytes = kKeys * 128;
   static constexpr int kTile16 = kChunks * kChunkBytes;  // 128 rows of fp16 (Q half, K or V tile)
-  static constexpr int kTile8 = kKeys * D;
   static constexpr int kQ = 0;
   static constexpr int kK16 = kQ + 2 * kTile16;
   static constexpr int kV16 = kK16 + 2 * kTile16;
-  static constexpr int kK8 = kV16 + kTile16;
-  static constexpr int kV8 = kK8 + 2 * kTile8;
-  static constexpr int kTable = kV8 + 2 * kTile8;
-  static constexpr int kBars = kTable + kTables * kGroups * 16;
+  static constexpr int kTable = kV16 + 2 * kTile16;
+  static constexpr int kBars = kTable + kTables * kGroups * 32;
   // Barriers.
-  static constexpr int kK8Full = 0, kK8Empty = 2, kV8Full = 4, kV8Empty = 6, kK16Full = 8,
-                       kK16Empty = 10, kV16Full = 12, kV16Empty = 13, kSFull = 14, kPFull = 16,
-                       kOFull = 18, kQFull = 20, kTabFull = 22, kDrain = kTabFull + kTables,
+  // kSFull, kPFull: group g, half h at + 2 g + h.
+  static constexpr int kK16Full = 0, kK16Empty = 2, kV16Full = 4, kV16Empty = 6, kSFull = 8,
+                       kPFull = 12, kODone = 16, kOFull = 18, kQFull = 20, kTabFull = 22,
+                       kTabEmpty = kTabFull + kTables, kDrain = kTabEmpty + kTables,
                        kCount = kDrain + 1;
   static constexpr int kMisc = kBars + 8 * kCount;
   static constexpr int kClean = kMisc + 16;  // per table: every key of the tile is there
   static constexpr int kBytes = kClean + 4 * kTables + 1024;
   static constexpr int kColS = 0, kColO = 256, kCols = 512;
   static constexpr int kPartial = kRows * D + 2 * kRows;  // floats
-  static_assert(kBytes <= 232448, "shared memory overflow");
+  static_assert(kBytes <= 230000, "shared memory overflow");  // and some for the static part
 };
 
+// 16 keys: what their scores need, and where they lie.
 struct RunScale {
   float mul, add, inv;
   int page;
+  long long k_at, v_at;  // byte offsets of the first key
 };
 
 // ---- work ----
@@ -233,7 +239,8 @@ struct Finder {
   }
 };
 
-// The part of a tile that a CTA works on, walked by every role by itself.
+// The part of a tile that a CTA works on.  Every warp walks the parts by itself, in shared memory:
+// they change seldom, and registers are short.
 struct Part {
   SeqTiles t;
   Place p;
@@ -244,11 +251,13 @@ struct Part {
   int seen;          // keys that the last row sees
   bool pair;         // at most 128 rows: the key tiles alternate between the groups
   bool whole;
+  bool more;         // false behind the last part
 
   __device__ void start(const Finder& f, int group, bool causal, long long units) {
     t = tiles_of(f.q, group, causal);
     p = f.at;
     left = units;
+    more = true;
     set(group);
   }
   __device__ void set(int group) {
@@ -263,23 +272,24 @@ struct Part {
     n_tiles = max(0, min(tile1, (seen + kKeys - 1) / kKeys) - tile0);
     pair = rows <= kHalfRows;
   }
-  // On to the next part; false at the end of the range.
-  __device__ bool next(const CacheView& c, int group) {
+  // On to the next part; `more` is false at the end of the range.
+  __device__ void next(const CacheView& c, int group) {
     left -= tile1 - tile0;
-    if (left <= 0) return false;
+    more = false;
+    if (left <= 0) return;
     p.tile = 0;
     if (++p.j >= t.tiles) {
       p.j = 0;
       if (++p.head >= c.Hkv) {
         p.head = 0;
         do {
-          if (++p.s >= c.n_seqs) return false;
+          if (++p.s >= c.n_seqs) return;
           t = tiles_of(seq_info(c, p.s), group, t.causal);
         } while (t.tiles == 0);
       }
     }
+    more = true;
     set(group);
-    return true;
   }
 };
 
@@ -320,12 +330,12 @@ __device__ __forceinline__ void wait_out(uint32_t bar, uint32_t parity, const Wa
 
 // ---- pieces of the roles ----
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
+// 16 bytes that are read once by this block.
+__device__ __forceinline__ uint4 ldg128(const unsigned char* p) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a)
-               : "memory");
+               : "l"(p));
   return v;
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
@@ -344,25 +354,11 @@ __device__ __forceinline__ uint2 widen(uint32_t u) {
   return r;
 }
 
-// 16 bytes of row `row`, piece `piece` (16 columns), into the two 16-byte chunks of the swizzled fp16
-// tile.  The lanes of the second half of a row store their second chunk first: the eight lanes of a
-// phase then reach all banks.
-__device__ __forceinline__ void store_wide(uint32_t tile, int row, int piece, uint4 v) {
+// 16 e4m3 values as fp16, 16 bytes at `lo` and 16 at `hi`.
+__device__ __forceinline__ void store_wide(uint32_t lo, uint32_t hi, uint4 v) {
   const uint2 a = widen(v.x), b = widen(v.y), c = widen(v.z), d = widen(v.w);
-  const uint4 w0 = make_uint4(a.x, a.y, b.x, b.y), w1 = make_uint4(c.x, c.y, d.x, d.y);
-  const uint32_t base = tile + (piece >> 2) * (kKeys * 128) + row * 128;
-  const int chunk = (piece & 3) * 2, flip = (piece >> 2) & 1;
-  sts128(base + (((chunk + flip) ^ (row & 7)) * 16), flip ? w1 : w0);
-  sts128(base + (((chunk + 1 - flip) ^ (row & 7)) * 16), flip ? w0 : w1);
-}
-
-__device__ __forceinline__ void load_page(uint32_t dst, const void* map, int pos, int head, int page,
-                                          uint32_t bar) {
-  const int pt = pos & 3, ph = (pos >> 2) & 3;
-  const int c0 = pt == 0 ? 0 : (ph == 0 ? head : page);
-  const int c1 = pt == 1 ? 0 : (ph == 1 ? head : page);
-  const int c2 = pt == 2 ? 0 : (ph == 2 ? head : page);
-  tma_load_4d(dst, map, 0, c0, c1, c2, bar);
+  sts128(lo, make_uint4(a.x, a.y, b.x, b.y));
+  sts128(hi, make_uint4(c.x, c.y, d.x, d.y));
 }
 
 __device__ __forceinline__ void value_scale(float s, float* add, float* inv) {
@@ -380,14 +376,14 @@ __device__ __forceinline__ void pair_barrier() {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
-    const __grid_constant__ CacheAttnArgs a, const __grid_constant__ PageMaps maps,
-    float* partials) {
+    const __grid_constant__ CacheAttnArgs a, float* partials) {
   using L = Layout<D>;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sbase = (raw + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (sbase - raw);
   __shared__ Finder finder;
+  __shared__ Part parts[kThreads / 32];
   RunScale* tables = reinterpret_cast<RunScale*>(smem + L::kTable);
   volatile int* clean = reinterpret_cast<volatile int*>(smem + L::kClean);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
@@ -410,20 +406,22 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   }
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(L::kK8Full + i), 1);
-      mbar_init(bar(L::kV8Full + i), 1);
-      mbar_init(bar(L::kK8Empty + i), 4);
-      mbar_init(bar(L::kV8Empty + i), 4);
       mbar_init(bar(L::kK16Full + i), 4);
       mbar_init(bar(L::kK16Empty + i), 1);
-      mbar_init(bar(L::kSFull + i), 1);
-      mbar_init(bar(L::kPFull + i), kHalfRows);
+      mbar_init(bar(L::kV16Full + i), 4);
+      mbar_init(bar(L::kV16Empty + i), 1);
+      mbar_init(bar(L::kODone + i), 1);
       mbar_init(bar(L::kOFull + i), 1);
       mbar_init(bar(L::kQFull + i), kHalfRows);
     }
-    mbar_init(bar(L::kV16Full), 4);
-    mbar_init(bar(L::kV16Empty), 1);
-    for (int i = 0; i < kTables; ++i) mbar_init(bar(L::kTabFull + i), 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar(L::kSFull + i), 1);
+      mbar_init(bar(L::kPFull + i), kHalfRows);
+    }
+    for (int i = 0; i < kTables; ++i) {
+      mbar_init(bar(L::kTabFull + i), 1);
+      mbar_init(bar(L::kTabEmpty + i), 1);
+    }
     mbar_init(bar(L::kDrain), 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -442,27 +440,33 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const Waits w{abort_flag, a.timeout_ns, c.status};
+  Part& part = parts[warp];
+  if (lane == 0) part.start(finder, group, a.causal, n_units);
+  __syncwarp();
+  auto next_part = [&]() {  // by whole warps
+    __syncwarp();
+    if (lane == 0) part.next(c, group);
+    __syncwarp();
+    return part.more;
+  };
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax groups
-    regs_alloc<184>();  // 2 x 128 x 184 + 128 x 80 + 128 x 64 = 512 x 128
     const int g = warp >> 2;
     const int r = tid & 127;  // tensor-memory lane
     const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_col = tl + L::kColS + g * 128, o_col = tl + L::kColO + g * 128;
     unsigned steps_done = 0, tiles_done = 0, parts_done = 0;
     bool ok = true;
-    Part part;
-    part.start(finder, group, a.causal, n_units);
     bool first_part = true;
     do {
-      const SeqInfo& q = part.t.q;
+      const SeqInfo q = part.t.q;
       const int row = part.pair ? r : g * kHalfRows + r;
       const bool on = row < part.rows;
       const int token = on ? (part.row0 + row) / group : 0;
       const int h = part.p.head * group + (on ? part.row0 + row - token * group : 0);
       const int limit = on ? (a.causal ? max(0, q.len - q.n + token + 1) : q.len) : 0;
-      const int my_steps = part.pair ? (part.n_tiles - g + 1) / 2 : part.n_tiles;
+      const int my_steps = 2 * (part.pair ? (part.n_tiles - g + 1) / 2 : part.n_tiles);  // halves
       float row_mul = a.scale * kLog2e;
       float m = -INFINITY, l = 0.f;
       if (part.n_tiles > 0 && ok) {
@@ -514,31 +518,31 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       const int first_row = part.pair ? 0 : min(g * kHalfRows, part.rows - 1);
       const int all_see = a.causal ? q.len - q.n + (part.row0 + first_row) / group + 1 : q.len;
       for (int k = 0; k < my_steps && ok; ++k) {
-        const int i = part.pair ? 2 * k + g : k;
+        const int half = k & 1, i = part.pair ? 2 * (k >> 1) + g : k >> 1;
         const unsigned at = tiles_done + i;
         const int slot = at % kTables;
+        const RunScale* table = tables + slot * kGroups + half * (kGroups / 2);
         ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull);
-        const RunScale* table = tables + slot * kGroups;
-        float mul[kGroups], add[kGroups];
+        float mul[kGroups / 2], add[kGroups / 2];
         if (ok) {
 #pragma unroll
-          for (int x = 0; x < kGroups; ++x) {
+          for (int x = 0; x < kGroups / 2; ++x) {
             mul[x] = fmaxf(table[x].mul * row_mul, 1.1754944e-38f);
             add[x] = table[x].add;
           }
-          ok = wait_or_abort(bar(L::kSFull + g), steps_done & 1, w, kStSFull);
+          ok = wait_or_abort(bar(L::kSFull + 2 * g + half), (steps_done >> 1) & 1, w, kStSFull);
         }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        ++steps_done;
         tc_fence_after();
-        const int key0 = (part.tile0 + i) * kKeys;
-        uint32_t u[kKeys];
-        tmem_ld2x64_wait(s_col, u);
-        if (key0 + kKeys > all_see || !clean[slot]) {
+        const uint32_t col0 = s_col + 64 * half;
+        const int key0 = (part.tile0 + i) * kKeys + 64 * half;
+        uint32_t u[64];
+        tmem_ld64_wait(col0, u);
+        if (key0 + 64 > all_see || !clean[slot]) {
           const int lim = limit - key0;
 #pragma unroll
-          for (int x = 0; x < kGroups; ++x) {
+          for (int x = 0; x < kGroups / 2; ++x) {
             const int lx = table[x].page < 0 ? 0 : lim;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -548,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         }
         float top = m;
 #pragma unroll
-        for (int x = 0; x < kGroups; ++x) {
+        for (int x = 0; x < kGroups / 2; ++x) {
           float b[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -564,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         const float ref = m == -INFINITY ? 0.f : m;
         l *= alpha;
 #pragma unroll
-        for (int x = 0; x < kGroups; x += 2) {
+        for (int x = 0; x < kGroups / 2; x += 2) {
           uint32_t pk[16];
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
@@ -583,11 +587,16 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
             const uint64_t both = f2_add(sum[0], sum[1]);
             l = fmaf(f2_lo(both) + f2_hi(both), table[x + y].inv, l);
           }
-          tmem_st16(s_col + 8 * x, pk);
+          tmem_st16(col0 + 8 * x, pk);
         }
         tmem_st_wait();
-        // S_g of this step completing implies that the O of the step before is complete.
         if (k > 0 && __any_sync(0xffffffffu, moved)) {
+          // O follows the maximum once the step before has been added to it.  The barrier counts this
+          // group's steps: it cannot pass this one, whose P is still to come, and has passed the last
+          // but one, which this step's S comes after.
+          ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kODone + g), (steps_done - 1) & 1, w, kStODone));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int col = 0; col < D; col += 32) {
             uint32_t o[32];
@@ -598,13 +607,16 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           }
           tmem_st_wait();
         }
+        ++steps_done;
         tc_fence_before();
-        mbar_arrive(bar(L::kPFull + g));
+        mbar_arrive(bar(L::kPFull + 2 * g + half));
       }
       tiles_done += part.n_tiles;
       if (my_steps > 0 && ok) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kOFull + g), parts_done & 1, w, kStODone));
+        // A barrier of its own: of the last two steps' phases of kODone either may be the current one.
+        ok = wait_or_abort(bar(L::kOFull + g), parts_done & 1, w, kStODone);
         ++parts_done;
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
       // Alternating tiles: group 0 merges.  Both groups' sums of a row are in one lane of tensor
@@ -683,90 +695,112 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       }
       if (merge) pair_barrier();  // group 1's sums were read
       first_part = false;
-    } while (part.next(c, group));
+    } while (next_part());
   } else if (warp < 12) {
     // ---------------------------------------------------------------- conversion
-    regs_dealloc<80>();
-    constexpr int kPieces = D / 16, kStep = 128 / kPieces;
+    constexpr int kPieces = D / 16, kStep = 128 / kPieces;  // kStep rows at a time
+    // Eight lanes that store together have two neighbouring rows and four pieces of one 128-byte
+    // chunk: their swizzled places are in different banks.
     const int t = tid & 127;
-    const int piece = t % kPieces, row0 = t / kPieces;
-    unsigned n = 0;  // tiles converted
+    const int piece = (t & 3) + (D == 128 ? ((t >> 3) & 1) * 4 : 0);
+    const int row0 = D == 128 ? ((t >> 2) & 1) + (t >> 4) * 2 : t >> 2;
+    const uint32_t spot = (piece >> 2) * L::kChunkBytes + row0 * 128;
+    const uint32_t lo = sbase + L::kK16 + spot + (((piece & 3) * 2) ^ (row0 & 7)) * 16;
+    const uint32_t hi = sbase + L::kK16 + spot + (((piece & 3) * 2 + 1) ^ (row0 & 7)) * 16;
+    const unsigned char* const k0 = c.k + (row0 & 15) * c.ks[2] + piece * 16;
+    const unsigned char* const v0 = c.v + (row0 & 15) * c.vs[2] + piece * 16;
+    unsigned n = 0;  // tiles stored
     bool ok = true;
-    Part part;
-    part.start(finder, group, a.causal, n_units);
-    do {
-      for (int i = 0; i < part.n_tiles && ok; ++i, ++n) {
-        const int st = n & 1;
-        const uint32_t ph = (n >> 1) & 1;
-        // K
-        ok = wait_or_abort(bar(L::kK8Full + st), ph, w, kStKFull) &&
-             (n < 2 || wait_or_abort(bar(L::kK16Empty + st), ph ^ 1, w, kStKVEmpty));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        {
-          const uint32_t src = sbase + L::kK8 + st * L::kTile8 + t * 16;
-          const uint32_t dst = sbase + L::kK16 + st * L::kTile16;
-#pragma unroll 2
-          for (int x = 0; x < kPieces; ++x) {
-            store_wide(dst, row0 + x * kStep, piece, lds128(src + x * 2048));
+    int i = 0, n_tiles = part.n_tiles;
+    uint4 kv[2][kPieces];
+    // This thread's pieces of K (which = 0) or V of tile i of the part, zeros where no key is.
+    auto fetch = [&](int which, unsigned at) {
+      const int slot = at % kTables;
+      const RunScale* table = tables + slot * kGroups + (row0 >> 4);
+      const unsigned char* base = which ? v0 : k0;
+      if (clean[slot]) {
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) {
+          const RunScale& run = table[x * kStep / 16];
+          kv[which][x] = ldg128(base + (which ? run.v_at : run.k_at));
+        }
+      } else {  // behind the last key a page holds anything, and 0 times that must be 0
+        const int left = part.t.q.len - (part.tile0 + i) * kKeys;  // keys that are there
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) {
+          const RunScale& run = table[x * kStep / 16];
+          kv[which][x] = make_uint4(0, 0, 0, 0);
+          if (row0 + x * kStep < left && run.page >= 0) {
+            kv[which][x] = ldg128(base + (which ? run.v_at : run.k_at));
           }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar(L::kK16Full + st));
-          mbar_arrive(bar(L::kK8Empty + st));
-        }
-        // V
-        ok = wait_or_abort(bar(L::kV8Full + st), ph, w, kStVFull) &&
-             (n < 1 || wait_or_abort(bar(L::kV16Empty), (n - 1) & 1, w, kStKVEmpty));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        {
-          const int slot = n % kTables;
-          const bool all = clean[slot];
-          const int left = part.t.q.len - (part.tile0 + i) * kKeys;  // keys that are there
-          const uint32_t src = sbase + L::kV8 + st * L::kTile8 + t * 16;
-          const uint32_t dst = sbase + L::kV16;
-#pragma unroll 2
-          for (int x = 0; x < kPieces; ++x) {
-            const int row = row0 + x * kStep;
-            uint4 v = lds128(src + x * 2048);
-            // Behind the last key a page holds anything, and 0 times that must be 0.
-            if (!all && (row >= left || tables[slot * kGroups + (row >> 4)].page < 0)) {
-              v = make_uint4(0, 0, 0, 0);
-            }
-            store_wide(dst, row, piece, v);
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(bar(L::kV16Full));
-          mbar_arrive(bar(L::kV8Empty + st));
         }
       }
-    } while (ok && part.next(c, group));
+    };
+    auto store = [&](int which, int st) {
+      const uint32_t to = (2 * which + st) * L::kTile16;
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) {
+        store_wide(lo + to + x * kStep * 128, hi + to + x * kStep * 128, kv[which][x]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar((which ? L::kV16Full : L::kK16Full) + st));
+    };
+    auto table_ready = [&](unsigned at) {
+      return wait_or_abort(bar(L::kTabFull + at % kTables), (at / kTables) & 1, w, kStKFull);
+    };
+    bool more = true;
+    while (more && n_tiles == 0) {
+      more = next_part();
+      n_tiles = part.n_tiles;
+    }
+    if (more) {
+      ok = __all_sync(0xffffffffu, table_ready(0));
+      if (ok) {
+        fetch(0, 0);
+        fetch(1, 0);
+      }
+    }
+    while (more && ok) {
+      const int st = n & 1;
+      const uint32_t ph = (n >> 1) & 1;
+      ok = n < 2 || wait_or_abort(bar(L::kK16Empty + st), ph ^ 1, w, kStKVEmpty);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      store(0, st);
+      // The tile after this one, in this part or a later one.
+      if (++i == n_tiles) {
+        i = 0;
+        do {
+          more = next_part();
+          n_tiles = part.n_tiles;
+        } while (more && n_tiles == 0);
+      }
+      if (more) {
+        ok = __all_sync(0xffffffffu, table_ready(n + 1));
+        if (ok) fetch(0, n + 1);
+      }
+      ok = ok && (n < 2 || wait_or_abort(bar(L::kV16Empty + st), ph ^ 1, w, kStKVEmpty));
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      store(1, st);
+      if (more) fetch(1, n + 1);
+      ++n;
+    }
   } else {
-    regs_dealloc<64>();
     if (warp == 12) {
       // -------------------------------------------------------------- pages
       // Lane 8 b + x looks after 16 keys (run x) of tile b of four; pages are looked up four tiles
       // ahead, their scales a tile later.
-      const int rows_page = 1 << c.page_shift;
       const int x = lane & 7;
-      const bool leads = ((16 * x) & (rows_page - 1)) == 0;  // the run starts a page
-      const unsigned bytes = static_cast<unsigned>(rows_page) * D;
       unsigned n = 0;  // tiles
-      unsigned k_sent = 0, v_sent = 0;
       bool ok = true;
-      Part part;
-      part.start(finder, group, a.causal, n_units);
       do {
         const int keys_end = min(part.t.q.len, (part.tile0 + part.n_tiles) * kKeys);
         const int head = part.p.head;
+        auto key_at = [&](int i) { return (part.tile0 + i + (lane >> 3)) * kKeys + 16 * x; };
         auto page_at = [&](int i) {
-          const int key = (part.tile0 + i + (lane >> 3)) * kKeys + 16 * x;
+          const int key = key_at(i);
           return key < keys_end ? page_of(c, part.p.s, key >> c.page_shift) : -1;
         };
         float sk = 0.f, sv = 1.f;
@@ -779,132 +813,123 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         };
         int next_page = part.n_tiles > 0 ? page_at(0) : -1;
         read_scales(next_page);
-        RunScale sc = {0.f, 0.f, 0.f, -1};
+        RunScale sc = {0.f, 0.f, 0.f, -1, 0, 0};
         for (int i = 0; i < part.n_tiles && ok; ++i, ++n) {
           if ((i & 3) == 0) {
+            const int slot = key_at(i) & ((1 << c.page_shift) - 1);
             sc.page = next_page;
             sc.mul = sk;
             value_scale(sv, &sc.add, &sc.inv);
+            sc.k_at = next_page * c.ks[0] + head * c.ks[1] + slot * c.ks[2];
+            sc.v_at = next_page * c.vs[0] + head * c.vs[1] + slot * c.vs[2];
             next_page = page_at(i + 4);
           }
           if ((i & 3) == 1) read_scales(next_page);
-          const int st = n & 1;
-          const uint32_t ph = (n >> 1) & 1;
-          if (n >= 2) {
-            ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kK8Empty + st), ph ^ 1, w, kStKVEmpty));
+          const int slot = n % kTables;
+          if (n >= kTables) {
+            ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kTabEmpty + slot),
+                                                       ((n / kTables) & 1) ^ 1, w, kStKVEmpty));
             if (!ok) break;
           }
-          const int slot = n % kTables;
           const bool mine = (lane >> 3) == (i & 3);
           if (mine) tables[slot * kGroups + x] = sc;
           const unsigned there = __ballot_sync(0xffffffffu, mine && sc.page >= 0);
-          const unsigned copies = __ballot_sync(0xffffffffu, mine && sc.page >= 0 && leads);
-          const bool all = __popc(there) == kGroups &&
-                           (part.tile0 + i + 1) * kKeys <= part.t.q.len;
           if (lane == 0) {
-            clean[slot] = all;
-            const unsigned sum = __popc(copies) * bytes;
-            if (sum > 0) {
-              mbar_arrive_expect_tx(bar(L::kK8Full + st), sum);
-            }
+            clean[slot] = __popc(there) == kGroups &&
+                          (part.tile0 + i + 1) * kKeys <= part.t.q.len;
           }
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(bar(L::kTabFull + slot));
-            if (copies == 0) mbar_arrive(bar(L::kK8Full + st));
-          }
-          if (mine && sc.page >= 0 && leads) {
-            load_page(sbase + L::kK8 + st * L::kTile8 + 16 * x * D, &maps.k, maps.k_pos, head, sc.page,
-                      bar(L::kK8Full + st));
-          }
-          ++k_sent;
-          __syncwarp();
-          if (n >= 2) {
-            ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kV8Empty + st), ph ^ 1, w, kStKVEmpty));
-            if (!ok) break;
-          }
-          if (lane == 0) {
-            const unsigned sum = __popc(copies) * bytes;
-            if (sum > 0) {
-              mbar_arrive_expect_tx(bar(L::kV8Full + st), sum);
-            } else {
-              mbar_arrive(bar(L::kV8Full + st));
-            }
-          }
-          __syncwarp();
-          if (mine && sc.page >= 0 && leads) {
-            load_page(sbase + L::kV8 + st * L::kTile8 + 16 * x * D, &maps.v, maps.v_pos, head, sc.page,
-                      bar(L::kV8Full + st));
-          }
-          ++v_sent;
+          if (lane == 0) mbar_arrive(bar(L::kTabFull + slot));
         }
-      } while (ok && part.next(c, group));
-      // Every copy that was started lands before the block ends.
-      for (unsigned i = k_sent > 2 ? k_sent - 2 : 0; i < k_sent; ++i) {
-        wait_out(bar(L::kK8Full + (i & 1)), (i >> 1) & 1, w);
-      }
-      for (unsigned i = v_sent > 2 ? v_sent - 2 : 0; i < v_sent; ++i) {
-        wait_out(bar(L::kV8Full + (i & 1)), (i >> 1) & 1, w);
-      }
+      } while (ok && next_part());
     } else if (warp == 13 && lane == 0) {
       // -------------------------------------------------------------- products
-      constexpr uint32_t kIdescS = idesc_mma(0, 128, kKeys, false);
+      constexpr uint32_t kIdescS = idesc_mma(0, 128, kKeys / 2, false);
       constexpr uint32_t kIdescPV = idesc_mma(0, 128, D, true);
+      constexpr uint32_t kHalfBytes = (kKeys / 2) * 128;  // 64 keys of a 128-byte chunk
       const uint64_t q_desc = sdesc_sw128(sbase + L::kQ, 16, 1024);
       const uint64_t k_desc = sdesc_sw128(sbase + L::kK16, 16, 1024);
       const uint64_t v_desc = sdesc_sw128(sbase + L::kV16, L::kChunkBytes, 1024);
       unsigned tiles_done = 0;
-      unsigned q_done[2] = {0, 0}, p_done[2] = {0, 0};
+      unsigned q_done[2] = {0, 0}, p_done[2] = {0, 0};  // p_done: tiles of group g
       bool ok = true;
-      Part part;
-      part.start(finder, group, a.causal, n_units);
       do {
+        // Round j: each group's next tile, half by half.  With more than 128 rows both groups have
+        // the same tile, otherwise tiles 2 j and 2 j + 1.
         const bool pair = part.pair;
-        const int n_steps = pair ? part.n_tiles : 2 * part.n_tiles;
-        if (n_steps == 0) continue;
-        auto issue_s = [&](int i) -> bool {
-          const int g = i & 1;
-          const unsigned tile = tiles_done + (pair ? i : i >> 1);
+        const int n_tiles = part.n_tiles;
+        const int rounds = pair ? (n_tiles + 1) / 2 : n_tiles;
+        auto tile_of = [&](int j, int g) { return pair ? 2 * j + g : j; };
+        auto issue_s = [&](int j, int g, int h) -> bool {
+          const int i = tile_of(j, g);
+          if (j >= rounds || i >= n_tiles) return true;
+          const unsigned tile = tiles_done + i;
           const int st = tile & 1;
-          if (pair || g == 0) {
+          if (h == 0 && (pair || g == 0)) {
             if (!wait_or_abort(bar(L::kK16Full + st), (tile >> 1) & 1, w, kStKFull)) return false;
+            tc_fence_after();
           }
-          tc_fence_after();
           const uint64_t qd = q_desc + ((pair ? 0 : g * L::kTile16) >> 4);
-          const uint64_t kd = k_desc + ((st * L::kTile16) >> 4);
+          const uint64_t kd = k_desc + ((st * L::kTile16 + h * kHalfBytes) >> 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t off = (kk / 4) * L::kChunkBytes + (kk % 4) * 32;
-            umma_ss(tmem + L::kColS + g * 128, qd + (off >> 4), kd + (off >> 4), kIdescS, kk > 0 ? 1u : 0u);
+            umma_ss(tmem + L::kColS + g * 128 + h * 64, qd + (off >> 4), kd + (off >> 4), kIdescS,
+                    kk > 0 ? 1u : 0u);
           }
-          umma_commit(bar(L::kSFull + g));
-          if (pair || g == 1) umma_commit(bar(L::kK16Empty + st));
+          umma_commit(bar(L::kSFull + 2 * g + h));
+          if (h == 1 && (pair || g == 1)) umma_commit(bar(L::kK16Empty + st));
           return true;
         };
-        ok = wait_or_abort(bar(L::kQFull), q_done[0]++ & 1, w, kStQFull);
-        if (ok && !pair) ok = wait_or_abort(bar(L::kQFull + 1), q_done[1]++ & 1, w, kStQFull);
-        for (int i = 0; ok && i < 2 && i < n_steps; ++i) ok = issue_s(i);
-        for (int i = 0; ok && i < n_steps; ++i) {
-          const int g = i & 1;
-          const unsigned tile = tiles_done + (pair ? i : i >> 1);
-          ok = wait_or_abort(bar(L::kPFull + g), p_done[g]++ & 1, w, kStPFull);
-          if (ok && (pair || g == 0)) ok = wait_or_abort(bar(L::kV16Full), tile & 1, w, kStVFull);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk) {
-            umma_ts(tmem + L::kColO + g * 128, tmem + L::kColS + g * 128 + 8 * kk,
-                    v_desc + ((kk * 2048) >> 4), kIdescPV, (i > 1 || kk > 0) ? 1u : 0u);
+        auto issue_pv = [&](int j, int g, int h) -> bool {
+          const int i = tile_of(j, g);
+          if (i >= n_tiles) return true;
+          const unsigned tile = tiles_done + i;
+          const int st = tile & 1;
+          if (!wait_or_abort(bar(L::kPFull + 2 * g + h), p_done[g] & 1, w, kStPFull)) return false;
+          if (h == 0 && (pair || g == 0)) {
+            if (!wait_or_abort(bar(L::kV16Full + st), (tile >> 1) & 1, w, kStVFull)) return false;
           }
-          if (pair || g == 1) umma_commit(bar(L::kV16Empty));
-          if (i + 2 < n_steps) {
-            ok = issue_s(i + 2);
-          } else {
-            umma_commit(bar(L::kOFull + g));
+          tc_fence_after();
+          const uint64_t vd = v_desc + ((st * L::kTile16 + h * kHalfBytes) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 32; ++kk) {
+            umma_ts(tmem + L::kColO + g * 128, tmem + L::kColS + g * 128 + h * 64 + 8 * kk,
+                    vd + ((kk * 2048) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(bar(L::kODone + g));
+          if (h == 1) {
+            if (j + 1 == rounds || tile_of(j + 1, g) >= n_tiles) umma_commit(bar(L::kOFull + g));
+            ++p_done[g];
+            if (pair || g == 1) {
+              umma_commit(bar(L::kV16Empty + st));
+              // Both the weights and V's buffer of this tile are done with its table.
+              mbar_arrive(bar(L::kTabEmpty + tile % kTables));
+            }
+          }
+          return true;
+        };
+        if (n_tiles > 0) {
+          ok = wait_or_abort(bar(L::kQFull), q_done[0]++ & 1, w, kStQFull);
+          if (ok && !pair) ok = wait_or_abort(bar(L::kQFull + 1), q_done[1]++ & 1, w, kStQFull);
+          tc_fence_after();
+        }
+        for (int h = 0; h < 2; ++h) {
+          for (int g = 0; g < 2; ++g) ok = ok && issue_s(0, g, h);
+        }
+        // S of the next tile follows the PV that read P from its columns: products that one thread
+        // issues execute in order.  Two groups on one tile take turns half by half.  With a tile each
+        // the first one's is finished first: the second one's next K is converted after the V that
+        // takes its place.
+        for (int j = 0; j < rounds && ok; ++j) {
+          for (int x = 0; x < 4; ++x) {
+            const int g = pair ? x >> 1 : x & 1, h = pair ? x & 1 : x >> 1;
+            ok = ok && issue_pv(j, g, h) && issue_s(j + 1, g, h);
           }
         }
-        tiles_done += part.n_tiles;
-      } while (ok && part.next(c, group));
+        tiles_done += n_tiles;
+        part.next(c, group);
+      } while (ok && part.more);
       umma_commit(bar(L::kDrain));
       wait_out(bar(L::kDrain), 0, w);
     }
@@ -992,13 +1017,11 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
   const unsigned ctas =
       static_cast<unsigned>(std::max(1ll, std::min<long long>(multiprocessors(), want)));
   float* partials = static_cast<float*>(a.workspace);
-  PageMaps maps;
-  cudaError_t e = make_page_maps(&maps, c, D, 1 << c.page_shift, false);
-  if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(fa_cache_tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaError_t e =
+      cudaFuncSetAttribute(fa_cache_tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            L::kBytes);
   if (e != cudaSuccess) return e;
-  fa_cache_tile_kernel<T, D><<<ctas, kThreads, L::kBytes, stream>>>(a, maps, partials);
+  fa_cache_tile_kernel<T, D><<<ctas, kThreads, L::kBytes, stream>>>(a, partials);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (units == 1) return cudaSuccess;  // no tile has two units
   cudaLaunchConfig_t cfg = {};
