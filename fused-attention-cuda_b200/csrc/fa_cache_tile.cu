@@ -369,6 +369,15 @@ __device__ __forceinline__ void value_scale(float s, float* add, float* inv) {
   *inv = 1.0f / s;
 }
 
+// True in one lane of the (converged) warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // The 256 threads of the two softmax groups.
 __device__ __forceinline__ void pair_barrier() {
   asm volatile("bar.sync %0, 256;" ::"n"(kPairBarrier) : "memory");
@@ -842,95 +851,110 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           if (lane == 0) mbar_arrive(bar(L::kTabFull + slot));
         }
       } while (ok && next_part());
-    } else if (warp == 13 && lane == 0) {
+    } else if (warp == 13) {
       // -------------------------------------------------------------- products
+      // The whole warp walks the schedule and one lane issues: with every operand the same in all
+      // lanes the compiler keeps them in uniform registers, where the instructions want them.
       constexpr uint32_t kIdescS = idesc_mma(0, 128, kKeys / 2, false);
       constexpr uint32_t kIdescPV = idesc_mma(0, 128, D, true);
       constexpr uint32_t kHalfBytes = (kKeys / 2) * 128;  // 64 keys of a 128-byte chunk
-      const uint64_t q_desc = sdesc_sw128(sbase + L::kQ, 16, 1024);
-      const uint64_t k_desc = sdesc_sw128(sbase + L::kK16, 16, 1024);
-      const uint64_t v_desc = sdesc_sw128(sbase + L::kV16, L::kChunkBytes, 1024);
+      const uint32_t base = __shfl_sync(0xffffffffu, sbase, 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t q_desc = sdesc_sw128(base + L::kQ, 16, 1024);
+      const uint64_t k_desc = sdesc_sw128(base + L::kK16, 16, 1024);
+      const uint64_t v_desc = sdesc_sw128(base + L::kV16, L::kChunkBytes, 1024);
       unsigned tiles_done = 0;
       unsigned q_done[2] = {0, 0}, p_done[2] = {0, 0};  // p_done: tiles of group g
       bool ok = true;
       do {
         // Round j: each group's next tile, half by half.  With more than 128 rows both groups have
         // the same tile, otherwise tiles 2 j and 2 j + 1.
-        const bool pair = part.pair;
-        const int n_tiles = part.n_tiles;
+        const bool pair = __shfl_sync(0xffffffffu, static_cast<int>(part.pair), 0);
+        const int n_tiles = __shfl_sync(0xffffffffu, part.n_tiles, 0);
         const int rounds = pair ? (n_tiles + 1) / 2 : n_tiles;
-        auto tile_of = [&](int j, int g) { return pair ? 2 * j + g : j; };
+        auto all = [](bool x) { return __all_sync(0xffffffffu, x); };
         auto issue_s = [&](int j, int g, int h) -> bool {
-          const int i = tile_of(j, g);
+          const int i = pair ? 2 * j + g : j;
           if (j >= rounds || i >= n_tiles) return true;
           const unsigned tile = tiles_done + i;
           const int st = tile & 1;
           if (h == 0 && (pair || g == 0)) {
-            if (!wait_or_abort(bar(L::kK16Full + st), (tile >> 1) & 1, w, kStKFull)) return false;
+            if (!all(wait_or_abort(bar(L::kK16Full + st), (tile >> 1) & 1, w, kStKFull))) return false;
             tc_fence_after();
           }
-          const uint64_t qd = q_desc + ((pair ? 0 : g * L::kTile16) >> 4);
+          const uint64_t qd = q_desc + (pair ? 0 : (g * L::kTile16) >> 4);
           const uint64_t kd = k_desc + ((st * L::kTile16 + h * kHalfBytes) >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * L::kChunkBytes + (kk % 4) * 32;
-            umma_ss(tmem + L::kColS + g * 128 + h * 64, qd + (off >> 4), kd + (off >> 4), kIdescS,
-                    kk > 0 ? 1u : 0u);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk / 4) * L::kChunkBytes + (kk % 4) * 32;
+              umma_ss(tm + L::kColS + g * 128 + h * 64, qd + (off >> 4), kd + (off >> 4), kIdescS,
+                      kk > 0 ? 1u : 0u);
+            }
+            umma_commit(bar(L::kSFull + 2 * g + h));
+            if (h == 1 && (pair || g == 1)) umma_commit(bar(L::kK16Empty + st));
           }
-          umma_commit(bar(L::kSFull + 2 * g + h));
-          if (h == 1 && (pair || g == 1)) umma_commit(bar(L::kK16Empty + st));
+          __syncwarp();
           return true;
         };
         auto issue_pv = [&](int j, int g, int h) -> bool {
-          const int i = tile_of(j, g);
+          const int i = pair ? 2 * j + g : j;
           if (i >= n_tiles) return true;
           const unsigned tile = tiles_done + i;
           const int st = tile & 1;
-          if (!wait_or_abort(bar(L::kPFull + 2 * g + h), p_done[g] & 1, w, kStPFull)) return false;
+          if (!all(wait_or_abort(bar(L::kPFull + 2 * g + h), p_done[g] & 1, w, kStPFull))) return false;
           if (h == 0 && (pair || g == 0)) {
-            if (!wait_or_abort(bar(L::kV16Full + st), (tile >> 1) & 1, w, kStVFull)) return false;
+            if (!all(wait_or_abort(bar(L::kV16Full + st), (tile >> 1) & 1, w, kStVFull))) return false;
           }
           tc_fence_after();
           const uint64_t vd = v_desc + ((st * L::kTile16 + h * kHalfBytes) >> 4);
+          const bool last = j + 1 == rounds || (pair && i + 2 >= n_tiles);
+          if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 32; ++kk) {
-            umma_ts(tmem + L::kColO + g * 128, tmem + L::kColS + g * 128 + h * 64 + 8 * kk,
-                    vd + ((kk * 2048) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
-          }
-          umma_commit(bar(L::kODone + g));
-          if (h == 1) {
-            if (j + 1 == rounds || tile_of(j + 1, g) >= n_tiles) umma_commit(bar(L::kOFull + g));
-            ++p_done[g];
-            if (pair || g == 1) {
-              umma_commit(bar(L::kV16Empty + st));
-              // Both the weights and V's buffer of this tile are done with its table.
-              mbar_arrive(bar(L::kTabEmpty + tile % kTables));
+            for (int kk = 0; kk < kKeys / 32; ++kk) {
+              umma_ts(tm + L::kColO + g * 128, tm + L::kColS + g * 128 + h * 64 + 8 * kk,
+                      vd + ((kk * 2048) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+            }
+            umma_commit(bar(L::kODone + g));
+            if (h == 1) {
+              if (last) umma_commit(bar(L::kOFull + g));
+              if (pair || g == 1) {
+                umma_commit(bar(L::kV16Empty + st));
+                // Both the weights and V's buffer of this tile are done with its table.
+                mbar_arrive(bar(L::kTabEmpty + tile % kTables));
+              }
             }
           }
+          __syncwarp();
+          if (h == 1) ++p_done[g];
           return true;
         };
         if (n_tiles > 0) {
-          ok = wait_or_abort(bar(L::kQFull), q_done[0]++ & 1, w, kStQFull);
-          if (ok && !pair) ok = wait_or_abort(bar(L::kQFull + 1), q_done[1]++ & 1, w, kStQFull);
+          ok = all(wait_or_abort(bar(L::kQFull), q_done[0]++ & 1, w, kStQFull));
+          if (ok && !pair) ok = all(wait_or_abort(bar(L::kQFull + 1), q_done[1]++ & 1, w, kStQFull));
           tc_fence_after();
         }
-        for (int h = 0; h < 2; ++h) {
-          for (int g = 0; g < 2; ++g) ok = ok && issue_s(0, g, h);
-        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) ok = ok && issue_s(0, x & 1, x >> 1);
         // S of the next tile follows the PV that read P from its columns: products that one thread
         // issues execute in order.  Two groups on one tile take turns half by half.  With a tile each
         // the first one's is finished first: the second one's next K is converted after the V that
         // takes its place.
-        for (int j = 0; j < rounds && ok; ++j) {
-          for (int x = 0; x < 4; ++x) {
-            const int g = pair ? x >> 1 : x & 1, h = pair ? x & 1 : x >> 1;
-            ok = ok && issue_pv(j, g, h) && issue_s(j + 1, g, h);
+        if (pair) {
+          for (int j = 0; j < rounds && ok; ++j) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) ok = ok && issue_pv(j, x >> 1, x & 1) && issue_s(j + 1, x >> 1, x & 1);
+          }
+        } else {
+          for (int j = 0; j < rounds && ok; ++j) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) ok = ok && issue_pv(j, x & 1, x >> 1) && issue_s(j + 1, x & 1, x >> 1);
           }
         }
         tiles_done += n_tiles;
-        part.next(c, group);
-      } while (ok && part.more);
-      umma_commit(bar(L::kDrain));
+      } while (ok && next_part());
+      if (elect_one()) umma_commit(bar(L::kDrain));
+      __syncwarp();
       wait_out(bar(L::kDrain), 0, w);
     }
     __syncwarp();
