@@ -14,7 +14,7 @@
 //                cost again.  Registers and not TMA: a tile in flight takes no shared memory, which
 //                the fp16 buffers fill (with e4m3 tiles in shared memory V had one buffer, and its
 //                conversion, 1100 cycles, stood between two products: 608 us at 2048 x 16384 keys)
-//   warp 13      issues S = Q K^T and O += P V
+//   warps 13, 14 issue S = Q K^T and O += P V of a group each
 //   warps 0-3, 4-7   two softmax groups, a row to a thread.  With more than 128 rows group g has rows
 //                128 g .. and every key tile; otherwise both have the same rows and the key tiles
 //                alternate, and their sums are merged at the end (both lie in one lane of tensor memory).  Either way step i belongs to group
@@ -416,9 +416,9 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(L::kK16Full + i), 4);
-      mbar_init(bar(L::kK16Empty + i), 1);
+      mbar_init(bar(L::kK16Empty + i), 2);
       mbar_init(bar(L::kV16Full + i), 4);
-      mbar_init(bar(L::kV16Empty + i), 1);
+      mbar_init(bar(L::kV16Empty + i), 2);
       mbar_init(bar(L::kODone + i), 1);
       mbar_init(bar(L::kOFull + i), 1);
       mbar_init(bar(L::kQFull + i), kHalfRows);
@@ -429,9 +429,9 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
     }
     for (int i = 0; i < kTables; ++i) {
       mbar_init(bar(L::kTabFull + i), 1);
-      mbar_init(bar(L::kTabEmpty + i), 1);
+      mbar_init(bar(L::kTabEmpty + i), 2);
     }
-    mbar_init(bar(L::kDrain), 1);
+    mbar_init(bar(L::kDrain), 2);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -851,105 +851,104 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           if (lane == 0) mbar_arrive(bar(L::kTabFull + slot));
         }
       } while (ok && next_part());
-    } else if (warp == 13) {
-      // -------------------------------------------------------------- products
+    } else if (warp < 15) {
+      // -------------------------------------------------------------- products, a warp for each group
       // The whole warp walks the schedule and one lane issues: with every operand the same in all
-      // lanes the compiler keeps them in uniform registers, where the instructions want them.
+      // lanes the compiler keeps them in uniform registers, where the instructions want them.  Two
+      // warps, since the time from one product's issue to the next wait (about 500 cycles) is as long
+      // as the products.
       constexpr uint32_t kIdescS = idesc_mma(0, 128, kKeys / 2, false);
       constexpr uint32_t kIdescPV = idesc_mma(0, 128, D, true);
       constexpr uint32_t kHalfBytes = (kKeys / 2) * 128;  // 64 keys of a 128-byte chunk
+      const int g = __shfl_sync(0xffffffffu, warp - 13, 0);
       const uint32_t base = __shfl_sync(0xffffffffu, sbase, 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t s_tm = tm + L::kColS + g * 128, o_tm = tm + L::kColO + g * 128;
       const uint64_t q_desc = sdesc_sw128(base + L::kQ, 16, 1024);
       const uint64_t k_desc = sdesc_sw128(base + L::kK16, 16, 1024);
       const uint64_t v_desc = sdesc_sw128(base + L::kV16, L::kChunkBytes, 1024);
-      unsigned tiles_done = 0;
-      unsigned q_done[2] = {0, 0}, p_done[2] = {0, 0};  // p_done: tiles of group g
+      auto all = [](bool x) { return __all_sync(0xffffffffu, x); };
+      unsigned tiles_done = 0, my_tiles = 0, parts_done = 0, q1_done = 0;
       bool ok = true;
       do {
-        // Round j: each group's next tile, half by half.  With more than 128 rows both groups have
-        // the same tile, otherwise tiles 2 j and 2 j + 1.
+        // With more than 128 rows both groups have every tile, otherwise this one has tiles g, g + 2,
+        // ... and stands in for the other where both have to give a buffer back.
         const bool pair = __shfl_sync(0xffffffffu, static_cast<int>(part.pair), 0);
         const int n_tiles = __shfl_sync(0xffffffffu, part.n_tiles, 0);
-        const int rounds = pair ? (n_tiles + 1) / 2 : n_tiles;
-        auto all = [](bool x) { return __all_sync(0xffffffffu, x); };
-        auto issue_s = [&](int j, int g, int h) -> bool {
-          const int i = pair ? 2 * j + g : j;
-          if (j >= rounds || i >= n_tiles) return true;
+        const int step = pair ? 2 : 1;
+        const uint64_t qd = q_desc + (pair ? 0 : (g * L::kTile16) >> 4);
+        auto issue_s = [&](int i, int h) -> bool {
+          if (i >= n_tiles) return true;
           const unsigned tile = tiles_done + i;
           const int st = tile & 1;
-          if (h == 0 && (pair || g == 0)) {
+          if (h == 0) {
             if (!all(wait_or_abort(bar(L::kK16Full + st), (tile >> 1) & 1, w, kStKFull))) return false;
             tc_fence_after();
           }
-          const uint64_t qd = q_desc + (pair ? 0 : (g * L::kTile16) >> 4);
           const uint64_t kd = k_desc + ((st * L::kTile16 + h * kHalfBytes) >> 4);
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t off = (kk / 4) * L::kChunkBytes + (kk % 4) * 32;
-              umma_ss(tm + L::kColS + g * 128 + h * 64, qd + (off >> 4), kd + (off >> 4), kIdescS,
-                      kk > 0 ? 1u : 0u);
+              umma_ss(s_tm + h * 64, qd + (off >> 4), kd + (off >> 4), kIdescS, kk > 0 ? 1u : 0u);
             }
             umma_commit(bar(L::kSFull + 2 * g + h));
-            if (h == 1 && (pair || g == 1)) umma_commit(bar(L::kK16Empty + st));
+            if (h == 1) {
+              umma_commit(bar(L::kK16Empty + st));
+              if (pair) umma_commit(bar(L::kK16Empty + st));
+            }
           }
           __syncwarp();
           return true;
         };
-        auto issue_pv = [&](int j, int g, int h) -> bool {
-          const int i = pair ? 2 * j + g : j;
-          if (i >= n_tiles) return true;
+        auto issue_pv = [&](int i, int h) -> bool {
           const unsigned tile = tiles_done + i;
           const int st = tile & 1;
-          if (!all(wait_or_abort(bar(L::kPFull + 2 * g + h), p_done[g] & 1, w, kStPFull))) return false;
-          if (h == 0 && (pair || g == 0)) {
+          if (!all(wait_or_abort(bar(L::kPFull + 2 * g + h), my_tiles & 1, w, kStPFull))) return false;
+          if (h == 0) {
             if (!all(wait_or_abort(bar(L::kV16Full + st), (tile >> 1) & 1, w, kStVFull))) return false;
           }
           tc_fence_after();
           const uint64_t vd = v_desc + ((st * L::kTile16 + h * kHalfBytes) >> 4);
-          const bool last = j + 1 == rounds || (pair && i + 2 >= n_tiles);
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kKeys / 32; ++kk) {
-              umma_ts(tm + L::kColO + g * 128, tm + L::kColS + g * 128 + h * 64 + 8 * kk,
-                      vd + ((kk * 2048) >> 4), kIdescPV, (j > 0 || h > 0 || kk > 0) ? 1u : 0u);
+              umma_ts(o_tm, s_tm + h * 64 + 8 * kk, vd + ((kk * 2048) >> 4), kIdescPV,
+                      (i >= step || h > 0 || kk > 0) ? 1u : 0u);
             }
             umma_commit(bar(L::kODone + g));
             if (h == 1) {
-              if (last) umma_commit(bar(L::kOFull + g));
-              if (pair || g == 1) {
+              if (i + step >= n_tiles) umma_commit(bar(L::kOFull + g));
+              umma_commit(bar(L::kV16Empty + st));
+              // Both the weights and V's buffer of this tile are done with its table.
+              mbar_arrive(bar(L::kTabEmpty + tile % kTables));
+              if (pair) {
                 umma_commit(bar(L::kV16Empty + st));
-                // Both the weights and V's buffer of this tile are done with its table.
                 mbar_arrive(bar(L::kTabEmpty + tile % kTables));
               }
             }
           }
           __syncwarp();
-          if (h == 1) ++p_done[g];
+          if (h == 1) ++my_tiles;
           return true;
         };
+        const int first = pair ? g : 0;
         if (n_tiles > 0) {
-          ok = all(wait_or_abort(bar(L::kQFull), q_done[0]++ & 1, w, kStQFull));
-          if (ok && !pair) ok = all(wait_or_abort(bar(L::kQFull + 1), q_done[1]++ & 1, w, kStQFull));
+          // Group 0's Q even where this group reads its own: the barrier's phases count parts.
+          ok = all(wait_or_abort(bar(L::kQFull), parts_done & 1, w, kStQFull));
+          ++parts_done;
+          if (g == 1 && !pair) {
+            ok = ok && all(wait_or_abort(bar(L::kQFull + 1), q1_done & 1, w, kStQFull));
+            ++q1_done;
+          }
           tc_fence_after();
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) ok = ok && issue_s(0, x & 1, x >> 1);
+        ok = ok && issue_s(first, 0) && issue_s(first, 1);
         // S of the next tile follows the PV that read P from its columns: products that one thread
-        // issues execute in order.  Two groups on one tile take turns half by half.  With a tile each
-        // the first one's is finished first: the second one's next K is converted after the V that
-        // takes its place.
-        if (pair) {
-          for (int j = 0; j < rounds && ok; ++j) {
+        // issues execute in order.
+        for (int i = first; i < n_tiles && ok; i += step) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) ok = ok && issue_pv(j, x >> 1, x & 1) && issue_s(j + 1, x >> 1, x & 1);
-          }
-        } else {
-          for (int j = 0; j < rounds && ok; ++j) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) ok = ok && issue_pv(j, x & 1, x >> 1) && issue_s(j + 1, x & 1, x >> 1);
-          }
+          for (int h = 0; h < 2; ++h) ok = ok && issue_pv(i, h) && issue_s(i + step, h);
         }
         tiles_done += n_tiles;
       } while (ok && next_part());
