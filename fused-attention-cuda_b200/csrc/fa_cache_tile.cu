@@ -7,14 +7,14 @@
 // (one unit of work).  The units of all sequences are numbered and split evenly over one CTA for each
 // multiprocessor; a tile that several CTAs share leaves fp32 partials for fa_cache_tile_merge_kernel.
 //
-//   warp 12      looks pages and scales up
-//   warps 8-11   load e4m3 pages into registers, a tile ahead, and store them as fp16 in the swizzled
-//                layout of the products (exact; two buffers of K and of V): tcgen05 has no product of
-//                fp16 by e4m3, and rounding q and P to 8 bits would cost what the cache's own 8 bits
-//                cost again.  Registers and not TMA: a tile in flight takes no shared memory, which
+//   warp 16      looks pages and scales up
+//   warps 8-11   (K) and 12-15 (V) load e4m3 pages into registers, a tile ahead, and store them as
+//                fp16 in the swizzled layout of the products (exact; two buffers each): tcgen05 has
+//                no product of fp16 by e4m3, and rounding q and P to 8 bits would cost what the
+//                cache's own 8 bits cost again.  Registers and not TMA: a tile in flight takes no shared memory, which
 //                the fp16 buffers fill (with e4m3 tiles in shared memory V had one buffer, and its
 //                conversion, 1100 cycles, stood between two products: 608 us at 2048 x 16384 keys)
-//   warps 13, 14 issue S = Q K^T and O += P V of a group each
+//   warps 17, 18 issue S = Q K^T and O += P V of a group each
 //   warps 0-3, 4-7   two softmax groups, a row to a thread.  With more than 128 rows group g has rows
 //                128 g .. and every key tile; otherwise both have the same rows and the key tiles
 //                alternate, and their sums are merged at the end (both lie in one lane of tensor memory).  Either way step i belongs to group
@@ -33,7 +33,7 @@
 namespace fa_sm100 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr int kRows = 256;   // query rows of a tile
 constexpr int kHalfRows = 128;
 constexpr int kKeys = 128;   // keys of a unit
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   const long long u_begin = blockIdx.x * per;
   if (u_begin >= total) return;  // the whole block
   const long long n_units = min(total - u_begin, per);
-  if (warp == 13) {
+  if (warp == 17) {
     tmem_alloc(smem_u32(tmem_slot), L::kCols);
     tmem_relinquish();
   }
@@ -461,6 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
 
   if (warp < 8) {
     // ---------------------------------------------------------------- softmax groups
+    regs_alloc<136>();  // 256 x 136 + 256 x 72 + 128 x 64 = 640 x 96
     const int g = warp >> 2;
     const int r = tid & 127;  // tensor-memory lane
     const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -479,45 +480,39 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       float row_mul = a.scale * kLog2e;
       float m = -INFINITY, l = 0.f;
       if (part.n_tiles > 0 && ok) {
-        // This thread's row of Q as fp16, swizzled.
-        const T* src = static_cast<const T*>(a.q) + static_cast<long long>(q.t0 + token) * a.sq[0] +
-                       h * a.sq[1];
-        uint4 v[D / 8];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          v[i] = on ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-        }
+        // This thread's row of Q as fp16, swizzled.  Loops are kept short here and at the end of a
+        // part: code that runs once is fetched as it runs.
+        const uint4* src = reinterpret_cast<const uint4*>(
+            static_cast<const T*>(a.q) + static_cast<long long>(q.t0 + token) * a.sq[0] + h * a.sq[1]);
+        float div = 1.f;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          float big = 0.f;
-#pragma unroll
+          uint32_t big = 0;  // the largest magnitudes, as bits, of the two halves of a word
+#pragma unroll 4
           for (int i = 0; i < D / 8; ++i) {
-            const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = to_float2<T>(u[k]);
-              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
+            const uint4 v = on ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+            big = __vmaxu2(__vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)), big);
           }
-          const int e = big > 0.f && big < INFINITY
-                            ? min(119, max(-118, static_cast<int>(__float_as_uint(big) >> 23) - 127 - 8))
-                            : 0;
-          const float div = __int_as_float((127 - e) << 23);
+          const uint32_t top = max(big & 0xffffu, big >> 16);  // infinities and NaN: no division
+          const int e = top > 0 && top < 0x7f80u
+                            ? min(119, max(-118, static_cast<int>(top >> 7) - 127 - 8)) : 0;
+          div = __int_as_float((127 - e) << 23);
           row_mul *= __int_as_float((127 + e) << 23);
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            uint32_t* u = reinterpret_cast<uint32_t*>(&v[i]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = to_float2<T>(u[k]);
-              u[k] = from_float2<__half>(f.x * div, f.y * div);
-            }
-          }
         }
         if (!part.pair || g == 0) {
           const uint32_t dst = sbase + L::kQ + g * L::kTile16 + r * 128;
-#pragma unroll
+#pragma unroll 4
           for (int i = 0; i < D / 8; ++i) {
-            sts128(dst + (i >> 3) * L::kChunkBytes + (((i & 7) ^ (r & 7)) * 16), v[i]);
+            uint4 v = on ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+              uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = to_float2<T>(u[k]);
+                u[k] = from_float2<__half>(f.x * div, f.y * div);
+              }
+            }
+            sts128(dst + (i >> 3) * L::kChunkBytes + (((i & 7) ^ (r & 7)) * 16), v);
           }
           fence_proxy_async_smem();
           mbar_arrive(bar(L::kQFull + g));
@@ -531,13 +526,15 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         const unsigned at = tiles_done + i;
         const int slot = at % kTables;
         const RunScale* table = tables + slot * kGroups + half * (kGroups / 2);
-        ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull);
-        float mul[kGroups / 2], add[kGroups / 2];
+        if (half == 0) ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull);
+        float mul[kGroups / 2], add[kGroups / 2], inv[kGroups / 2];
         if (ok) {
 #pragma unroll
           for (int x = 0; x < kGroups / 2; ++x) {
-            mul[x] = fmaxf(table[x].mul * row_mul, 1.1754944e-38f);
-            add[x] = table[x].add;
+            const float4 sc = *reinterpret_cast<const float4*>(&table[x]);
+            mul[x] = fmaxf(sc.x * row_mul, 1.1754944e-38f);
+            add[x] = sc.y;
+            inv[x] = sc.z;
           }
           ok = wait_or_abort(bar(L::kSFull + 2 * g + half), (steps_done >> 1) & 1, w, kStSFull);
         }
@@ -594,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
               sum[j & 1] = f2_add(sum[j & 1], f2_pack(p0, p1));
             }
             const uint64_t both = f2_add(sum[0], sum[1]);
-            l = fmaf(f2_lo(both) + f2_hi(both), table[x + y].inv, l);
+            l = fmaf(f2_lo(both) + f2_hi(both), inv[x + y], l);
           }
           tmem_st16(col0 + 8 * x, pk);
         }
@@ -606,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kODone + g), (steps_done - 1) & 1, w, kStODone));
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
+#pragma unroll 1
           for (int col = 0; col < D; col += 32) {
             uint32_t o[32];
             tmem_ld32_wait(o_col + col, o);
@@ -660,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         const float inv = part.whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
         const long long at = static_cast<long long>(q.t0 + token) * a.H + h;
         float* slot = partials + (2ll * blockIdx.x + (first_part ? 0 : 1)) * L::kPartial;
-#pragma unroll
+#pragma unroll 1
         for (int col = 0; col < D; col += 32) {
           uint32_t u[32];
           __syncwarp();
@@ -705,78 +702,67 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       if (merge) pair_barrier();  // group 1's sums were read
       first_part = false;
     } while (next_part());
-  } else if (warp < 12) {
+  } else if (warp < 16) {
     // ---------------------------------------------------------------- conversion
+    regs_dealloc<72>();
     constexpr int kPieces = D / 16, kStep = 128 / kPieces;  // kStep rows at a time
+    const int is_v = warp >= 12;
     // Eight lanes that store together have two neighbouring rows and four pieces of one 128-byte
     // chunk: their swizzled places are in different banks.
     const int t = tid & 127;
     const int piece = (t & 3) + (D == 128 ? ((t >> 3) & 1) * 4 : 0);
     const int row0 = D == 128 ? ((t >> 2) & 1) + (t >> 4) * 2 : t >> 2;
-    const uint32_t spot = (piece >> 2) * L::kChunkBytes + row0 * 128;
-    const uint32_t lo = sbase + L::kK16 + spot + (((piece & 3) * 2) ^ (row0 & 7)) * 16;
-    const uint32_t hi = sbase + L::kK16 + spot + (((piece & 3) * 2 + 1) ^ (row0 & 7)) * 16;
-    const unsigned char* const k0 = c.k + (row0 & 15) * c.ks[2] + piece * 16;
-    const unsigned char* const v0 = c.v + (row0 & 15) * c.vs[2] + piece * 16;
+    const uint32_t spot = sbase + (is_v ? L::kV16 : L::kK16) + (piece >> 2) * L::kChunkBytes + row0 * 128;
+    const uint32_t lo = spot + (((piece & 3) * 2) ^ (row0 & 7)) * 16;
+    const uint32_t hi = spot + (((piece & 3) * 2 + 1) ^ (row0 & 7)) * 16;
+    const unsigned char* const base =
+        (is_v ? c.v : c.k) + (row0 & 15) * (is_v ? c.vs[2] : c.ks[2]) + piece * 16;
+    const int full = is_v ? L::kV16Full : L::kK16Full, empty = is_v ? L::kV16Empty : L::kK16Empty;
     unsigned n = 0;  // tiles stored
     bool ok = true;
     int i = 0, n_tiles = part.n_tiles;
-    uint4 kv[2][kPieces];
-    // This thread's pieces of K (which = 0) or V of tile i of the part, zeros where no key is.
-    auto fetch = [&](int which, unsigned at) {
+    uint4 kv[kPieces];
+    // This thread's pieces of tile i of the part, zeros where no key is.
+    auto fetch = [&](unsigned at) {
       const int slot = at % kTables;
-      const RunScale* table = tables + slot * kGroups + (row0 >> 4);
-      const unsigned char* base = which ? v0 : k0;
+      ok = __all_sync(0xffffffffu,
+                      wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull));
+      if (!ok) return;
+      const long long* from = &tables[slot * kGroups + (row0 >> 4)].k_at + is_v;
+      constexpr int kNext = sizeof(RunScale) / 8 * (kStep / 16);
       if (clean[slot]) {
 #pragma unroll
-        for (int x = 0; x < kPieces; ++x) {
-          const RunScale& run = table[x * kStep / 16];
-          kv[which][x] = ldg128(base + (which ? run.v_at : run.k_at));
-        }
+        for (int x = 0; x < kPieces; ++x) kv[x] = ldg128(base + from[x * kNext]);
       } else {  // behind the last key a page holds anything, and 0 times that must be 0
+        const RunScale* table = tables + slot * kGroups + (row0 >> 4);
         const int left = part.t.q.len - (part.tile0 + i) * kKeys;  // keys that are there
 #pragma unroll
         for (int x = 0; x < kPieces; ++x) {
-          const RunScale& run = table[x * kStep / 16];
-          kv[which][x] = make_uint4(0, 0, 0, 0);
-          if (row0 + x * kStep < left && run.page >= 0) {
-            kv[which][x] = ldg128(base + (which ? run.v_at : run.k_at));
+          kv[x] = make_uint4(0, 0, 0, 0);
+          if (row0 + x * kStep < left && table[x * kStep / 16].page >= 0) {
+            kv[x] = ldg128(base + from[x * kNext]);
           }
         }
       }
-    };
-    auto store = [&](int which, int st) {
-      const uint32_t to = (2 * which + st) * L::kTile16;
-#pragma unroll
-      for (int x = 0; x < kPieces; ++x) {
-        store_wide(lo + to + x * kStep * 128, hi + to + x * kStep * 128, kv[which][x]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar((which ? L::kV16Full : L::kK16Full) + st));
-    };
-    auto table_ready = [&](unsigned at) {
-      return wait_or_abort(bar(L::kTabFull + at % kTables), (at / kTables) & 1, w, kStKFull);
     };
     bool more = true;
     while (more && n_tiles == 0) {
       more = next_part();
       n_tiles = part.n_tiles;
     }
-    if (more) {
-      ok = __all_sync(0xffffffffu, table_ready(0));
-      if (ok) {
-        fetch(0, 0);
-        fetch(1, 0);
-      }
-    }
+    if (more) fetch(0);
     while (more && ok) {
       const int st = n & 1;
-      const uint32_t ph = (n >> 1) & 1;
-      ok = n < 2 || wait_or_abort(bar(L::kK16Empty + st), ph ^ 1, w, kStKVEmpty);
+      ok = n < 2 || wait_or_abort(bar(empty + st), ((n >> 1) & 1) ^ 1, w, kStKVEmpty);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      store(0, st);
+#pragma unroll
+      for (int x = 0; x < kPieces; ++x) {
+        store_wide(lo + st * L::kTile16 + x * kStep * 128, hi + st * L::kTile16 + x * kStep * 128, kv[x]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(full + st));
       // The tile after this one, in this part or a later one.
       if (++i == n_tiles) {
         i = 0;
@@ -785,19 +771,11 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           n_tiles = part.n_tiles;
         } while (more && n_tiles == 0);
       }
-      if (more) {
-        ok = __all_sync(0xffffffffu, table_ready(n + 1));
-        if (ok) fetch(0, n + 1);
-      }
-      ok = ok && (n < 2 || wait_or_abort(bar(L::kV16Empty + st), ph ^ 1, w, kStKVEmpty));
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      store(1, st);
-      if (more) fetch(1, n + 1);
-      ++n;
+      if (more) fetch(++n);
     }
   } else {
-    if (warp == 12) {
+    regs_dealloc<64>();
+    if (warp == 16) {
       // -------------------------------------------------------------- pages
       // Lane 8 b + x looks after 16 keys (run x) of tile b of four; pages are looked up four tiles
       // ahead, their scales a tile later.
@@ -851,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           if (lane == 0) mbar_arrive(bar(L::kTabFull + slot));
         }
       } while (ok && next_part());
-    } else if (warp < 15) {
+    } else if (warp < 19) {
       // -------------------------------------------------------------- products, a warp for each group
       // The whole warp walks the schedule and one lane issues: with every operand the same in all
       // lanes the compiler keeps them in uniform registers, where the instructions want them.  Two
@@ -860,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       constexpr uint32_t kIdescS = idesc_mma(0, 128, kKeys / 2, false);
       constexpr uint32_t kIdescPV = idesc_mma(0, 128, D, true);
       constexpr uint32_t kHalfBytes = (kKeys / 2) * 128;  // 64 keys of a 128-byte chunk
-      const int g = __shfl_sync(0xffffffffu, warp - 13, 0);
+      const int g = __shfl_sync(0xffffffffu, warp - 17, 0);
       const uint32_t base = __shfl_sync(0xffffffffu, sbase, 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t s_tm = tm + L::kColS + g * 128, o_tm = tm + L::kColO + g * 128;
@@ -961,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 13) tmem_dealloc(tmem, L::kCols);
+  if (warp == 17) tmem_dealloc(tmem, L::kCols);
 }
 
 // Merges the parts of a tile that several CTAs share.  Block i looks after the tile that CTA i's range
