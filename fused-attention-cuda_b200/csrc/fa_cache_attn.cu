@@ -35,7 +35,8 @@ template <int D, int NT>
 struct Layout {
   static constexpr int kRows = 8 * NT;
   static constexpr int kStages = D == 128 && NT == 1 ? 3 : 4;  // runs in flight for each warp
-  static constexpr int kPerSm = D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 5 : 4);  // CTAs
+  // CTAs on a multiprocessor: as many as the accumulators' registers leave room for.
+  static constexpr int kPerSm = NT > 2 ? 2 : D == 128 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 5 : 4);
   static constexpr int kHalf = kRun * D;  // K or V bytes of a run
   static constexpr int kStage = 2 * kHalf;
   static constexpr int kRing = kWarps * kStages * kStage;
@@ -600,9 +601,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
     }
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == w.tiles;
-    constexpr int kPer = kRows * D / kThreads;  // columns of one thread
-    const int row = tid / (D / kPer), col = (tid % (D / kPer)) * kPer;
-    if (row < rows) {
+#pragma unroll 1
+    for (int e = tid; e < rows * (D / 8); e += kThreads) {  // 8 columns of a row at a time
+      const int row = e / (D / 8), col = (e % (D / 8)) * 8;
       float top = merge_m[0][row], lsum = 0.f;
 #pragma unroll
       for (int i = 1; i < kWarps; ++i) top = fmaxf(top, merge_m[i][row]);
@@ -611,9 +612,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
         const float wm = merge_m[i][row], wl = merge_l[i][row];
         lsum += wm == -INFINITY ? (wl == wl ? 0.f : wl) : wl * ex2_approx(wm - top);
       }
-      float4 out[kPer / 4];
+      float4 out[2];
 #pragma unroll
-      for (int k = 0; k < kPer / 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         out[k] = *reinterpret_cast<const float4*>(sums + row * D + col + 4 * k);
 #pragma unroll
         for (int i = 1; i < kWarps; ++i) {
@@ -627,21 +628,17 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
         const long long at = static_cast<long long>(w.q.t0 + token) * a.H + head * group +
                              (row0 + row - token * group);
         const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-        T* o = static_cast<T*>(a.o) + at * D + col;
-#pragma unroll
-        for (int k = 0; k < kPer / 4; ++k) {
-          uint2 v;
-          v.x = from_float2<T>(out[k].x * inv, out[k].y * inv);
-          v.y = from_float2<T>(out[k].z * inv, out[k].w * inv);
-          *reinterpret_cast<uint2*>(o + 4 * k) = v;
-        }
+        uint4 v;
+        v.x = from_float2<T>(out[0].x * inv, out[0].y * inv);
+        v.y = from_float2<T>(out[0].z * inv, out[0].w * inv);
+        v.z = from_float2<T>(out[1].x * inv, out[1].y * inv);
+        v.w = from_float2<T>(out[1].z * inv, out[1].w * inv);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at * D + col) = v;
         if (col == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
       } else {
         float* part = partials + (2ll * blockIdx.x + (u == u_begin ? 0 : 1)) * L::kPartial;
-#pragma unroll
-        for (int k = 0; k < kPer / 4; ++k) {
-          *reinterpret_cast<float4*>(part + row * D + col + 4 * k) = out[k];
-        }
+        *reinterpret_cast<float4*>(part + row * D + col) = out[0];
+        *reinterpret_cast<float4*>(part + row * D + col + 4) = out[1];
         if (col == 0) {
           part[kRows * D + row] = top;
           part[kRows * D + kRows + row] = lsum;
@@ -688,9 +685,10 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   int split = 1;  // rows side by side; the warps of a row share its parts
-  while (split < rows) split *= 2;
-  const int row = warp % split, share = warp / split, shares = kCombineWarps / split;
+  while (split < rows && split < kCombineWarps) split *= 2;
+  const int share = warp / split, shares = kCombineWarps / split;
   const int last = static_cast<int>((end - 1) / per);  // the last CTA with a part
+  for (int row = warp % split; row - warp % split < rows; row += split) {
   float top = -INFINITY, lsum = 0.f, acc[kPer] = {};
   if (row < rows) {
     constexpr int kBatch = 4;  // parts in flight
@@ -731,9 +729,9 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
     lsums[warp] = lsum;
   }
   __syncthreads();
-  if (share > 0 || row >= rows) return;
+  if (share == 0 && row < rows) {
   for (int i = 1; i < shares; ++i) {
-    const int other = row + i * split;
+    const int other = warp + i * split;
     const float pm = tops[other], pl = lsums[other];
     if (pm == -INFINITY && pl == 0.f) continue;
     const float to = fmaxf(top, pm);
@@ -752,6 +750,9 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
 #pragma unroll
   for (int k = 0; k < kPer; k += 2) o[k / 2] = from_float2<T>(acc[k] * inv, acc[k + 1] * inv);
   if (lane == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
+  }
+  __syncthreads();  // the next rows' sums take the place of these
+  }
 }
 
 template <typename T, int D, int NT>
@@ -790,40 +791,47 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
                             static_cast<const float*>(partials));
 }
 
-// Tiles of 8 query rows where a sequence has no more on average, else of 16.
-bool narrow_tiles(int H, int Hkv, int T, int n_seqs) {
-  return static_cast<long long>(T) * (H / Hkv) <= 8ll * n_seqs;
-}
-
-// More than 16 rows on average go to the kernel on tcgen05 (fa_cache_tile.cu).
-bool wide_tiles(int H, int Hkv, int T, int n_seqs) {
-  return static_cast<long long>(T) * (H / Hkv) > 16ll * n_seqs;
+// Query rows of a tile in eights, by a sequence's mean; 0: the kernel on tcgen05 (fa_cache_tile.cu).
+int row_eights(int H, int Hkv, int T, int n_seqs) {
+  const long long rows = static_cast<long long>(T) * (H / Hkv);
+  return rows > 32ll * n_seqs ? 0 : static_cast<int>(std::max(1ll, (rows + 8ll * n_seqs - 1) / (8ll * n_seqs)));
 }
 
 template <typename T, int D>
 cudaError_t launch_d(const CacheAttnArgs& a, cudaStream_t stream) {
-  return narrow_tiles(a.H, a.c.Hkv, a.c.T, a.c.n_seqs) ? launch_t<T, D, 1>(a, stream)
-                                                       : launch_t<T, D, 2>(a, stream);
+  switch (row_eights(a.H, a.c.Hkv, a.c.T, a.c.n_seqs)) {
+    case 1: return launch_t<T, D, 1>(a, stream);
+    case 2: return launch_t<T, D, 2>(a, stream);
+    case 3: return launch_t<T, D, 3>(a, stream);
+    case 4: return launch_t<T, D, 4>(a, stream);
+    default: return launch_cache_tile(a, stream);
+  }
+}
+
+template <int D, int NT>
+size_t workspace_t(int sms) {
+  return 2ull * sms * Layout<D, NT>::kPerSm * Layout<D, NT>::kPartial * sizeof(float);
 }
 
 template <int D>
-size_t workspace_d(int H, int Hkv, int T, int n_seqs, int sms) {
-  const int floats = narrow_tiles(H, Hkv, T, n_seqs)
-                         ? Layout<D, 1>::kPerSm * Layout<D, 1>::kPartial
-                         : Layout<D, 2>::kPerSm * Layout<D, 2>::kPartial;
-  return 2ull * sms * floats * sizeof(float);
+size_t workspace_d(int eights, int sms) {
+  switch (eights) {
+    case 1: return workspace_t<D, 1>(sms);
+    case 2: return workspace_t<D, 2>(sms);
+    case 3: return workspace_t<D, 3>(sms);
+    case 4: return workspace_t<D, 4>(sms);
+    default: return cache_tile_workspace(D, sms);
+  }
 }
 
 }  // namespace
 
 size_t cache_attention_workspace(int H, int Hkv, int D, int T, int n_seqs, int sms) {
-  if (wide_tiles(H, Hkv, T, n_seqs)) return cache_tile_workspace(D, sms);
-  return D == 64 ? workspace_d<64>(H, Hkv, T, n_seqs, sms)
-                 : workspace_d<128>(H, Hkv, T, n_seqs, sms);
+  const int eights = row_eights(H, Hkv, T, n_seqs);
+  return D == 64 ? workspace_d<64>(eights, sms) : workspace_d<128>(eights, sms);
 }
 
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, cudaStream_t stream) {
-  if (wide_tiles(a.H, a.c.Hkv, a.c.T, a.c.n_seqs)) return launch_cache_tile(a, stream);
   if (a.dtype == FA_DTYPE_F16) {
     return a.D == 64 ? launch_d<__half, 64>(a, stream) : launch_d<__half, 128>(a, stream);
   }
