@@ -11,10 +11,13 @@
 // and its own exponent, and where it grows the earlier rows are rounded once more to the new step.
 // Scales are powers of two, so dividing by them is exact: the only rounding is the one to e4m3.
 //
-// The rotation is computed in 64 bits, where both products are exact (a 16-bit by a 24-bit
-// significand) and only the sum rounds, and then truncated to 32 bits with the lost bits or-ed into
-// the last one (rounding to odd).  A later rounding to 16 or 8 bits is then the rounding of the
-// exact value: the stored byte does not depend on the order of operations.
+// The rotation a c - b s is computed as an unevaluated sum of two floats: both products exactly (their
+// rounding errors by fma), the sum's rounding error by the two-sum of Knuth.  The sum is then rounded
+// to odd (the last bit set where it is inexact), so that the rounding to 16 or 8 bits that follows is
+// the rounding of the exact value: a stored byte does not depend on the order of operations.  In
+// 64-bit arithmetic the conversions, 16 a cycle, took longer than the memory (129 us against 47 for
+// 13613 tokens of 32 + 8 + 8 heads of 128).
+#include <algorithm>
 #include <cmath>
 
 #include "fa_cache_common.cuh"
@@ -27,10 +30,21 @@ constexpr int kMaxExp = 120;
 
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 
-// x in 32 bits, rounded to odd.
-__device__ __forceinline__ float round_to_odd(double x) {
-  const float f = __double2float_rz(x);
-  return static_cast<double>(f) != x ? __int_as_float(__float_as_int(f) | 1) : f;
+// a c - b s in 32 bits, rounded to odd.
+__device__ __forceinline__ float turn(float a, float c, float b, float s) {
+  const float p = __fmul_rn(a, c), q = __fmul_rn(b, s);
+  const float pe = __fmaf_rn(a, c, -p), qe = __fmaf_rn(b, s, -q);  // exact
+  const float d = __fsub_rn(p, q);
+  const float t = __fsub_rn(d, p);
+  const float de = __fadd_rn(__fsub_rn(p, __fsub_rn(d, t)), __fsub_rn(-q, t));  // p - q = d + de
+  const float e = __fadd_rn(de, __fsub_rn(pe, qe));
+  const float h = __fadd_rn(d, e);
+  const float lo = __fsub_rn(e, __fsub_rn(h, d));  // the exact value is h + lo, |lo| below h's step
+  const int bits = __float_as_int(h);
+  if (!(fabsf(d) < INFINITY)) return d;
+  // It lies between h and its neighbour on lo's side; one of the two is odd.
+  const int toward = (__float_as_int(lo) ^ bits) < 0 ? -1 : 1;
+  return lo != 0.f && (bits & 1) == 0 ? __int_as_float(bits + toward) : h;
 }
 
 __device__ __forceinline__ float finite_or_nan(float x) {
@@ -121,9 +135,9 @@ __device__ __forceinline__ void load_angles(Angles& a, const AppendArgs& p, int 
 
 // (a, b) -> the rotated pair, each rounded to odd in 32 bits.
 __device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s) {
-  const double da = a, db = b, dc = c, ds = s;
-  a = round_to_odd(da * dc - db * ds);
-  b = round_to_odd(db * dc + da * ds);
+  const float x = turn(a, c, b, s);
+  b = turn(b, c, -a, s);
+  a = x;
 }
 
 template <typename T>
@@ -203,7 +217,7 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
                           int tid, float* red) {
   constexpr int kLanes = D / 16;             // lanes for a row
   constexpr int kRows = WARPS * 32 / kLanes;  // rows of one sweep
-  constexpr int kKeep = 4;                   // sweeps whose rows stay in registers
+  constexpr int kKeep = 2;                   // sweeps whose rows stay in registers
   const CacheView& c = p.c;
   const int lane = tid & 31;
   const int head = job >> 1;
@@ -290,7 +304,7 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if constexpr (WARPS > 1) {
     if (lane == 0) red[tid >> 5] = amax;
-    __syncthreads();
+    __syncthreads();  // every job of the block comes here
     amax = red[0];
 #pragma unroll
     for (int i = 1; i < WARPS; ++i) amax = fmaxf(amax, red[i]);
@@ -384,9 +398,10 @@ __device__ void rotate_q(const AppendArgs& p, const Grid& g, long long group, in
   }
 }
 
-// Blocks [0, kv_blocks) fill pages, the others rotate q.  ITEM_WARPS warps share a page item.
+// Blocks [0, kv_blocks) fill pages, the others rotate q.  ITEM_WARPS warps share a job: a page item
+// of one head, k or v.
 template <typename T, int D, int THREADS, int ITEM_WARPS>
-__global__ void __launch_bounds__(THREADS) fa_cache_append_kernel(
+__global__ void __launch_bounds__(THREADS, 3) fa_cache_append_kernel(
     const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
   constexpr int kPerBlock = THREADS / 32 / ITEM_WARPS;
   __shared__ float red[THREADS / 32];
@@ -424,9 +439,12 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   }
   if (items > 0x7fffffffll) return cudaErrorInvalidValue;
   g.items = static_cast<int>(items);
-  const bool wide = mean >= 8;
-  const int threads = wide ? 256 : 128;
-  const int per_block = wide ? 1 : threads / 32;
+  // Few rows of a page come at a time: a warp for each job.  Else as many warps as hold a page's rows
+  // of one head in registers, 32 values a thread: with more, most of a block's time is its chain of
+  // lookups (eight warps for any page: 102 us for 16384 tokens of 12 heads of 64, pages of 32).
+  const int warps = mean < 8 ? 1 : std::min(8, page * D / 1024);
+  const int threads = 256;
+  const int per_block = threads / 32 / warps;
   const long long kv_blocks = (items * 2 * c.Hkv + per_block - 1) / per_block;
   long long q_blocks = 0;
   g.q_heads = 1;
@@ -441,10 +459,11 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   if (kv_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   g.kv_blocks = static_cast<int>(kv_blocks);
   const unsigned blocks = static_cast<unsigned>(kv_blocks + q_blocks);
-  if (wide) {
-    fa_cache_append_kernel<T, D, 256, 8><<<blocks, 256, 0, stream>>>(a, g);
-  } else {
-    fa_cache_append_kernel<T, D, 128, 1><<<blocks, 128, 0, stream>>>(a, g);
+  switch (warps) {
+    case 1: fa_cache_append_kernel<T, D, 256, 1><<<blocks, 256, 0, stream>>>(a, g); break;
+    case 2: fa_cache_append_kernel<T, D, 256, 2><<<blocks, 256, 0, stream>>>(a, g); break;
+    case 4: fa_cache_append_kernel<T, D, 256, 4><<<blocks, 256, 0, stream>>>(a, g); break;
+    default: fa_cache_append_kernel<T, D, 256, 8><<<blocks, 256, 0, stream>>>(a, g); break;
   }
   return cudaGetLastError();
 }
