@@ -11,16 +11,21 @@
 // and its own exponent, and where it grows the earlier rows are rounded once more to the new step.
 // Scales are powers of two, so dividing by them is exact: the only rounding is the one to e4m3.
 //
-// The rotation a c - b s is computed as an unevaluated sum of two floats: both products exactly (their
-// rounding errors by fma), the sum's rounding error by the two-sum of Knuth.  The sum is then rounded
-// to odd (the last bit set where it is inexact), so that the rounding to 16 or 8 bits that follows is
-// the rounding of the exact value: a stored byte does not depend on the order of operations.  In
-// 64-bit arithmetic the conversions, 16 a cycle, took longer than the memory (129 us against 47 for
-// 13613 tokens of 32 + 8 + 8 heads of 128).
+// The rotation a c + b s is computed as an unevaluated sum of two floats, two sums at a time: both
+// products exactly (their rounding errors by fma), the sum's rounding error by the two-sum of Knuth.
+// What is stored or returned is then the rounding of the exact value, whatever the order of
+// operations.  For k, which is rounded once its page's scale is known, the sum is rounded to odd in 32
+// bits (the last bit set where it is inexact): a later rounding to 8 bits is that of the exact value.
+// For q the first float, which is the exact value rounded, is rounded again at once; that differs only
+// where it lies halfway between two 16-bit values, one in 2^13 or 2^16, and those are done over by way
+// of the rounding to odd.  In 64-bit arithmetic the conversions, 16 a cycle, took 129 us for 13613
+// tokens of 32 + 8 + 8 heads of 128, and one sum at a time with every one rounded to odd 136 us; the
+// memory needs 47.
 #include <algorithm>
 #include <cmath>
 
 #include "fa_cache_common.cuh"
+#include "sm100_ptx.cuh"
 
 namespace fa_sm100 {
 namespace {
@@ -30,19 +35,31 @@ constexpr int kMaxExp = 120;
 
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 
-// a c - b s in 32 bits, rounded to odd.
-__device__ __forceinline__ float turn(float a, float c, float b, float s) {
-  const float p = __fmul_rn(a, c), q = __fmul_rn(b, s);
-  const float pe = __fmaf_rn(a, c, -p), qe = __fmaf_rn(b, s, -q);  // exact
-  const float d = __fsub_rn(p, q);
-  const float t = __fsub_rn(d, p);
-  const float de = __fadd_rn(__fsub_rn(p, __fsub_rn(d, t)), __fsub_rn(-q, t));  // p - q = d + de
-  const float e = __fadd_rn(de, __fsub_rn(pe, qe));
-  const float h = __fadd_rn(d, e);
-  const float lo = __fsub_rn(e, __fsub_rn(h, d));  // the exact value is h + lo, |lo| below h's step
+constexpr uint64_t kMinusOne2 = 0xbf800000bf800000ull;
+
+// a c + b s for two lanes of a packed pair: the nearest floats, and in `lo` what is left.
+struct Sum2 {
+  uint64_t hi, lo;
+};
+__device__ __forceinline__ Sum2 sum2(uint64_t a, uint64_t c, uint64_t b, uint64_t s) {
+  const uint64_t p = f2_mul(a, c), q = f2_mul(b, s);
+  const uint64_t minus_p = f2_mul(p, kMinusOne2);
+  const uint64_t pe = f2_fma(a, c, minus_p);                      // exact
+  const uint64_t qe = f2_fma(b, s, f2_mul(q, kMinusOne2));        // exact
+  const uint64_t d = f2_add(p, q);
+  const uint64_t t = f2_add(d, minus_p);
+  const uint64_t de = f2_add(f2_fma(f2_fma(t, kMinusOne2, d), kMinusOne2, p),
+                             f2_fma(t, kMinusOne2, q));           // p + q = d + de
+  const uint64_t e = f2_add(de, f2_add(pe, qe));
+  const uint64_t h = f2_add(d, e);
+  return Sum2{h, f2_fma(f2_fma(d, kMinusOne2, h), kMinusOne2, e)};
+}
+
+// h + lo rounded to odd; where h is not finite because of the steps above, `plain` is the value.
+__device__ __forceinline__ float to_odd(float h, float lo, float plain) {
   const int bits = __float_as_int(h);
-  if (!(fabsf(d) < INFINITY)) return d;
-  // It lies between h and its neighbour on lo's side; one of the two is odd.
+  if (!(fabsf(h) < INFINITY)) return plain;
+  // The value lies between h and its neighbour on lo's side; one of the two is odd.
   const int toward = (__float_as_int(lo) ^ bits) < 0 ? -1 : 1;
   return lo != 0.f && (bits & 1) == 0 ? __int_as_float(bits + toward) : h;
 }
@@ -115,8 +132,9 @@ __device__ __forceinline__ Unit unit_of(int u, int rot, bool interleaved) {
   return r;
 }
 
+// Eight angles in packed pairs.
 struct Angles {
-  float c[8], s[8];
+  uint64_t c[4], s[4];
 };
 
 __device__ __forceinline__ void load_angles(Angles& a, const AppendArgs& p, int pos, int col,
@@ -126,45 +144,112 @@ __device__ __forceinline__ void load_angles(Angles& a, const AppendArgs& p, int 
   for (int i = 0; i < 2; ++i) {
     const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at) + i);
     const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + at) + i);
-    a.c[4 * i] = c.x * mul, a.c[4 * i + 1] = c.y * mul;
-    a.c[4 * i + 2] = c.z * mul, a.c[4 * i + 3] = c.w * mul;
-    a.s[4 * i] = s.x * mul, a.s[4 * i + 1] = s.y * mul;
-    a.s[4 * i + 2] = s.z * mul, a.s[4 * i + 3] = s.w * mul;
+    a.c[2 * i] = f2_pack(c.x * mul, c.y * mul), a.c[2 * i + 1] = f2_pack(c.z * mul, c.w * mul);
+    a.s[2 * i] = f2_pack(s.x * mul, s.y * mul), a.s[2 * i + 1] = f2_pack(s.z * mul, s.w * mul);
   }
 }
 
-// (a, b) -> the rotated pair, each rounded to odd in 32 bits.
-__device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s) {
-  const float x = turn(a, c, b, s);
-  b = turn(b, c, -a, s);
-  a = x;
+// The pairs of a lane's 16 elements: first[j], second[j] are the two elements that angle j turns.
+__device__ __forceinline__ void split_pairs(const float (&x)[8], const float (&y)[8], bool interleaved,
+                                            uint64_t (&first)[4], uint64_t (&second)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (interleaved) {  // neighbours inside each run of 8
+      const float(&z)[8] = j < 2 ? x : y;
+      first[j] = f2_pack(z[4 * (j & 1)], z[4 * (j & 1) + 2]);
+      second[j] = f2_pack(z[4 * (j & 1) + 1], z[4 * (j & 1) + 3]);
+    } else {
+      first[j] = f2_pack(x[2 * j], x[2 * j + 1]);
+      second[j] = f2_pack(y[2 * j], y[2 * j + 1]);
+    }
+  }
+}
+__device__ __forceinline__ void join_pairs(float (&x)[8], float (&y)[8], bool interleaved,
+                                           const float (&first)[8], const float (&second)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (interleaved) {
+      float(&z)[8] = j < 4 ? x : y;
+      z[2 * (j & 3)] = first[j];
+      z[2 * (j & 3) + 1] = second[j];
+    } else {
+      x[j] = first[j];
+      y[j] = second[j];
+    }
+  }
 }
 
+// Turns a lane's elements, each rounded to odd.
+__device__ __forceinline__ void rotate_unit(float (&x)[8], float (&y)[8], const Angles& an,
+                                            bool interleaved) {
+  uint64_t a[4], b[4];
+  float fa[8], fb[8];
+  split_pairs(x, y, interleaved, a, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t minus_s = f2_mul(an.s[j], kMinusOne2);
+    const Sum2 u = sum2(a[j], an.c[j], b[j], minus_s), v = sum2(b[j], an.c[j], a[j], an.s[j]);
+    const uint64_t up = f2_fma(a[j], an.c[j], f2_mul(b[j], minus_s));
+    const uint64_t vp = f2_fma(b[j], an.c[j], f2_mul(a[j], an.s[j]));
+    fa[2 * j] = to_odd(f2_lo(u.hi), f2_lo(u.lo), f2_lo(up));
+    fa[2 * j + 1] = to_odd(f2_hi(u.hi), f2_hi(u.lo), f2_hi(up));
+    fb[2 * j] = to_odd(f2_lo(v.hi), f2_lo(v.lo), f2_lo(vp));
+    fb[2 * j + 1] = to_odd(f2_hi(v.hi), f2_hi(v.lo), f2_hi(vp));
+  }
+  join_pairs(x, y, interleaved, fa, fb);
+}
+
+// Turns a lane's elements to the nearest floats; false where one may not round on to T's nearest: it
+// lies halfway between two values of T, is subnormal there, or is not finite.
 template <typename T>
-__device__ __forceinline__ void load_unit(float (&x)[8], float (&y)[8], const T* row,
-                                          const Unit& u) {
-  const uint4 a = *reinterpret_cast<const uint4*>(row + u.lo);
-  const uint4 b = *reinterpret_cast<const uint4*>(row + u.hi);
-  const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+__device__ __forceinline__ bool rotate_unit_fast(float (&x)[8], float (&y)[8], const Angles& an,
+                                                 bool interleaved) {
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr uint32_t kBits = kHalf ? 0x1fffu : 0xffffu;  // those that the rounding takes off
+  constexpr uint32_t kTie = kHalf ? 0x1000u : 0x8000u;
+  uint64_t a[4], b[4], poison = 0;
+  float fa[8], fb[8];
+  uint32_t tie = 0xffffffffu, small = 0xffffffffu;
+  split_pairs(x, y, interleaved, a, b);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint64_t minus_s = f2_mul(an.s[j], kMinusOne2);
+    const uint64_t u = sum2(a[j], an.c[j], b[j], minus_s).hi;
+    const uint64_t v = sum2(b[j], an.c[j], a[j], an.s[j]).hi;
+    poison = f2_fma(u, 0ull, poison);  // 0 times what is not finite
+    poison = f2_fma(v, 0ull, poison);
+    const uint32_t w[4] = {static_cast<uint32_t>(u), static_cast<uint32_t>(u >> 32),
+                           static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32)};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      tie = min(tie, (w[k] & kBits) ^ kTie);
+      if (kHalf) small = min(small, w[k] & 0x7fffffffu);
+    }
+    fa[2 * j] = f2_lo(u), fa[2 * j + 1] = f2_hi(u);
+    fb[2 * j] = f2_lo(v), fb[2 * j + 1] = f2_hi(v);
+  }
+  const bool sure = tie != 0 && f2_lo(poison) == 0.f && f2_hi(poison) == 0.f &&
+                    (!kHalf || small >= 0x38800000u);  // 2^-14
+  if (sure) join_pairs(x, y, interleaved, fa, fb);
+  return sure;
+}
+
+// A lane's 16 elements as they lie in memory.
+struct Raw {
+  uint4 a, b;
+};
+template <typename T>
+__device__ __forceinline__ Raw load_unit(const T* row, const Unit& u) {
+  return Raw{*reinterpret_cast<const uint4*>(row + u.lo), *reinterpret_cast<const uint4*>(row + u.hi)};
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Raw& r, float (&x)[8], float (&y)[8]) {
+  const uint32_t wa[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, wb[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 fa = to_float2<T>(wa[i]), fb = to_float2<T>(wb[i]);
     x[2 * i] = fa.x, x[2 * i + 1] = fa.y;
     y[2 * i] = fb.x, y[2 * i + 1] = fb.y;
-  }
-}
-
-__device__ __forceinline__ void rotate_unit(float (&x)[8], float (&y)[8], const Angles& a,
-                                            bool interleaved) {
-  if (interleaved) {  // the pairs are neighbours inside each run of 8
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      rotate_pair(x[2 * i], x[2 * i + 1], a.c[i], a.s[i]);
-      rotate_pair(y[2 * i], y[2 * i + 1], a.c[4 + i], a.s[4 + i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) rotate_pair(x[i], y[i], a.c[i], a.s[i]);
   }
 }
 
@@ -270,7 +355,7 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
   float x[kKeep][8], y[kKeep][8];
   float amax = 0.f;
   auto fetch = [&](int slot, float(&fx)[8], float(&fy)[8]) {
-    load_unit<T>(fx, fy, base + slot * st[0], u);
+    widen<T>(load_unit<T>(base + slot * st[0], u), fx, fy);
     if (u.angle >= 0) {
       Angles an;
       load_angles(an, p, static_cast<int>(page_pos) + slot, u.angle, half);
@@ -382,11 +467,16 @@ __device__ void rotate_q(const AppendArgs& p, const Grid& g, long long group, in
   const T* src = static_cast<const T*>(p.q) + t * p.sq[0];
   T* dst = static_cast<T*>(p.q_out) + static_cast<long long>(t) * p.H * D;
   const int h1 = min(p.H, h0 + g.q_heads);
+  Raw next = {};
+  if (pos >= 0) next = load_unit<T>(src + h0 * p.sq[1], u);
+#pragma unroll 1
   for (int h = h0; h < h1; ++h) {
-    float x[8] = {}, y[8] = {};
-    if (pos >= 0) {
-      load_unit<T>(x, y, src + h * p.sq[1], u);
-      if (u.angle >= 0) rotate_unit(x, y, an, p.interleaved);
+    float x[8], y[8];
+    const Raw raw = next;  // zeros without a position
+    if (pos >= 0 && h + 1 < h1) next = load_unit<T>(src + (h + 1) * p.sq[1], u);
+    widen<T>(raw, x, y);
+    if (pos >= 0 && u.angle >= 0 && !rotate_unit_fast<T>(x, y, an, p.interleaved)) {
+      rotate_unit(x, y, an, p.interleaved);
     }
     uint4 a, b;
     a.x = from_float2<T>(x[0], x[1]), a.y = from_float2<T>(x[2], x[3]);
