@@ -11,16 +11,15 @@
 // and its own exponent, and where it grows the earlier rows are rounded once more to the new step.
 // Scales are powers of two, so dividing by them is exact: the only rounding is the one to e4m3.
 //
-// The rotation a c + b s is computed as an unevaluated sum of two floats, two sums at a time: both
-// products exactly (their rounding errors by fma), the sum's rounding error by the two-sum of Knuth.
-// What is stored or returned is then the rounding of the exact value, whatever the order of
-// operations.  For k, which is rounded once its page's scale is known, the sum is rounded to odd in 32
-// bits (the last bit set where it is inexact): a later rounding to 8 bits is that of the exact value.
-// For q the first float, which is the exact value rounded, is rounded again at once; that differs only
-// where it lies halfway between two 16-bit values, one in 2^13 or 2^16, and those are done over by way
-// of the rounding to odd.  In 64-bit arithmetic the conversions, 16 a cycle, took 129 us for 13613
-// tokens of 32 + 8 + 8 heads of 128, and one sum at a time with every one rounded to odd 136 us; the
-// memory needs 47.
+// What is stored or returned is the rounding of the exact rotated value, whatever the order of
+// operations: a c + b s is computed in 32 bits with a bound w on its error, and where a c + b s - w and
+// a c + b s + w round to the same 8 or 16 bits, that is it.  Where they do not (a value next to a border:
+// one of some 2^12 for bf16, 2^9 for fp16, 2^18 for e4m3) the sum is done over as an unevaluated
+// sum of two floats, both products exactly (their errors by fma), the sum's error by the two-sum of
+// Knuth, rounded to odd in 32 bits (the last bit set where it is inexact), so that the rounding that
+// follows is that of the exact value.  A page's scale is settled likewise, by bounds on its largest
+// magnitude.  13613 tokens of 32 + 8 + 8 heads of 128, where the memory needs 47 us: 64-bit arithmetic
+// 129 us (conversions, 16 a cycle), every sum as two floats 105 us.
 #include <algorithm>
 #include <cmath>
 
@@ -30,6 +29,7 @@
 namespace fa_sm100 {
 namespace {
 
+constexpr int kThreads = 256;
 constexpr int kMinExp = -64;
 constexpr int kMaxExp = 120;
 
@@ -84,6 +84,11 @@ __device__ __forceinline__ int stored_exp(float s) {
   return max(kMinExp, min(kMaxExp, e));
 }
 
+// Two values; what is not finite has to be NaN before (infinities saturate).
+__device__ __forceinline__ uint32_t to_e4m3x2(uint64_t v) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(f2_lo(v), f2_hi(v)), __NV_SATFINITE, __NV_E4M3);
+}
+
 __device__ __forceinline__ uint2 to_e4m3x8(const float (&y)[8], float mul) {
   uint2 r;
   unsigned short h[4];
@@ -132,21 +137,28 @@ __device__ __forceinline__ Unit unit_of(int u, int rot, bool interleaved) {
   return r;
 }
 
-// Eight angles in packed pairs.
+// Eight angles in packed pairs, and 3.125 * 2^-24 of the largest |cos| or |sin| among them.
 struct Angles {
-  uint64_t c[4], s[4];
+  uint64_t c[4], s[4], minus_s[4];
+  float eps;
 };
 
 __device__ __forceinline__ void load_angles(Angles& a, const AppendArgs& p, int pos, int col,
                                             float mul) {
   const long long at = static_cast<long long>(pos) * (p.rot_dim / 2) + col;
+  float big = 0.f;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at) + i);
     const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + at) + i);
     a.c[2 * i] = f2_pack(c.x * mul, c.y * mul), a.c[2 * i + 1] = f2_pack(c.z * mul, c.w * mul);
     a.s[2 * i] = f2_pack(s.x * mul, s.y * mul), a.s[2 * i + 1] = f2_pack(s.z * mul, s.w * mul);
+    big = fmax3(big, fmax3(fabsf(c.x), fabsf(c.y), fmaxf(fabsf(c.z), fabsf(c.w))),
+                fmax3(fabsf(s.x), fabsf(s.y), fmaxf(fabsf(s.z), fabsf(s.w))));
   }
+  a.eps = big * mul * 0x1.9p-23f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) a.minus_s[j] = f2_mul(a.s[j], kMinusOne2);
 }
 
 // The pairs of a lane's 16 elements: first[j], second[j] are the two elements that angle j turns.
@@ -164,74 +176,62 @@ __device__ __forceinline__ void split_pairs(const float (&x)[8], const float (&y
     }
   }
 }
-__device__ __forceinline__ void join_pairs(float (&x)[8], float (&y)[8], bool interleaved,
-                                           const float (&first)[8], const float (&second)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (interleaved) {
-      float(&z)[8] = j < 4 ? x : y;
-      z[2 * (j & 3)] = first[j];
-      z[2 * (j & 3) + 1] = second[j];
-    } else {
-      x[j] = first[j];
-      y[j] = second[j];
-    }
-  }
+__device__ __forceinline__ uint64_t f2_abs(uint64_t x) { return x & 0x7fffffff7fffffffull; }
+
+// Pair j turned in plain 32 bits, and a bound on how far the values and the values +- w are off: a
+// product, the fma and the sum with w round once each, 2^-24 (|b s| + 2 |a c + b s|) in all, which is at
+// most 3 * 2^-24 (|a| + |b|) times the largest |c| or |s|.
+struct Bounded {
+  uint64_t x, y, w;
+};
+__device__ __forceinline__ Bounded turn_bounded(uint64_t a, uint64_t b, const Angles& an, int j) {
+  return Bounded{f2_fma(a, an.c[j], f2_mul(b, an.minus_s[j])), f2_fma(b, an.c[j], f2_mul(a, an.s[j])),
+                 f2_mul(f2_add(f2_abs(a), f2_abs(b)), f2_pack(an.eps, an.eps))};
 }
 
-// Turns a lane's elements, each rounded to odd.
-__device__ __forceinline__ void rotate_unit(float (&x)[8], float (&y)[8], const Angles& an,
-                                            bool interleaved) {
-  uint64_t a[4], b[4];
-  float fa[8], fb[8];
-  split_pairs(x, y, interleaved, a, b);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint64_t minus_s = f2_mul(an.s[j], kMinusOne2);
-    const Sum2 u = sum2(a[j], an.c[j], b[j], minus_s), v = sum2(b[j], an.c[j], a[j], an.s[j]);
-    const uint64_t up = f2_fma(a[j], an.c[j], f2_mul(b[j], minus_s));
-    const uint64_t vp = f2_fma(b[j], an.c[j], f2_mul(a[j], an.s[j]));
-    fa[2 * j] = to_odd(f2_lo(u.hi), f2_lo(u.lo), f2_lo(up));
-    fa[2 * j + 1] = to_odd(f2_hi(u.hi), f2_hi(u.lo), f2_hi(up));
-    fb[2 * j] = to_odd(f2_lo(v.hi), f2_lo(v.lo), f2_lo(vp));
-    fb[2 * j + 1] = to_odd(f2_hi(v.hi), f2_hi(v.lo), f2_hi(vp));
-  }
-  join_pairs(x, y, interleaved, fa, fb);
+// The same rounded to odd.
+__device__ __forceinline__ void turn_odd(uint64_t a, uint64_t b, const Angles& an, int j, float (&fa)[2],
+                                         float (&fb)[2]) {
+  const Sum2 u = sum2(a, an.c[j], b, an.minus_s[j]), v = sum2(b, an.c[j], a, an.s[j]);
+  const Bounded p = turn_bounded(a, b, an, j);
+  fa[0] = to_odd(f2_lo(u.hi), f2_lo(u.lo), f2_lo(p.x));
+  fa[1] = to_odd(f2_hi(u.hi), f2_hi(u.lo), f2_hi(p.x));
+  fb[0] = to_odd(f2_lo(v.hi), f2_lo(v.lo), f2_lo(p.y));
+  fb[1] = to_odd(f2_hi(v.hi), f2_hi(v.lo), f2_hi(p.y));
 }
 
-// Turns a lane's elements to the nearest floats; false where one may not round on to T's nearest: it
-// lies halfway between two values of T, is subnormal there, or is not finite.
 template <typename T>
-__device__ __forceinline__ bool rotate_unit_fast(float (&x)[8], float (&y)[8], const Angles& an,
-                                                 bool interleaved) {
-  constexpr bool kHalf = std::is_same<T, __half>::value;
-  constexpr uint32_t kBits = kHalf ? 0x1fffu : 0xffffu;  // those that the rounding takes off
-  constexpr uint32_t kTie = kHalf ? 0x1000u : 0x8000u;
-  uint64_t a[4], b[4], poison = 0;
-  float fa[8], fb[8];
-  uint32_t tie = 0xffffffffu, small = 0xffffffffu;
+__device__ __forceinline__ uint32_t narrow2(uint64_t v) {
+  return from_float2<T>(f2_lo(v), f2_hi(v));
+}
+
+// Turns a lane's elements and rounds them to T: the words of its two runs.
+template <typename T>
+__device__ __forceinline__ void rotate_to(const float (&x)[8], const float (&y)[8], const Angles& an,
+                                          bool interleaved, uint32_t (&wx)[4], uint32_t (&wy)[4]) {
+  uint64_t a[4], b[4];
   split_pairs(x, y, interleaved, a, b);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint64_t minus_s = f2_mul(an.s[j], kMinusOne2);
-    const uint64_t u = sum2(a[j], an.c[j], b[j], minus_s).hi;
-    const uint64_t v = sum2(b[j], an.c[j], a[j], an.s[j]).hi;
-    poison = f2_fma(u, 0ull, poison);  // 0 times what is not finite
-    poison = f2_fma(v, 0ull, poison);
-    const uint32_t w[4] = {static_cast<uint32_t>(u), static_cast<uint32_t>(u >> 32),
-                           static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32)};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      tie = min(tie, (w[k] & kBits) ^ kTie);
-      if (kHalf) small = min(small, w[k] & 0x7fffffffu);
+    const Bounded t = turn_bounded(a[j], b[j], an, j);
+    uint32_t fu = narrow2<T>(f2_add(t.x, t.w)), fv = narrow2<T>(f2_add(t.y, t.w));
+    const uint32_t gu = narrow2<T>(f2_fma(t.w, kMinusOne2, t.x));
+    const uint32_t gv = narrow2<T>(f2_fma(t.w, kMinusOne2, t.y));
+    if (((fu ^ gu) | (fv ^ gv)) != 0) {
+      float p[2], q[2];
+      turn_odd(a[j], b[j], an, j, p, q);
+      fu = from_float2<T>(p[0], p[1]);
+      fv = from_float2<T>(q[0], q[1]);
     }
-    fa[2 * j] = f2_lo(u), fa[2 * j + 1] = f2_hi(u);
-    fb[2 * j] = f2_lo(v), fb[2 * j + 1] = f2_hi(v);
+    if (interleaved) {
+      uint32_t(&w)[4] = j < 2 ? wx : wy;
+      w[2 * (j & 1)] = __byte_perm(fu, fv, 0x5410);
+      w[2 * (j & 1) + 1] = __byte_perm(fu, fv, 0x7632);
+    } else {
+      wx[j] = fu;
+      wy[j] = fv;
+    }
   }
-  const bool sure = tie != 0 && f2_lo(poison) == 0.f && f2_hi(poison) == 0.f &&
-                    (!kHalf || small >= 0x38800000u);  // 2^-14
-  if (sure) join_pairs(x, y, interleaved, fa, fb);
-  return sure;
 }
 
 // A lane's 16 elements as they lie in memory.
@@ -291,14 +291,14 @@ __device__ __forceinline__ int find_item_seq(const CacheView& c, int i, int lane
 struct Grid {
   int items;         // page items of one (head, k or v)
   int seq_items;     // of one sequence when all have the same number of new tokens
-  int kv_blocks;     // blocks that fill pages; the rest rotate q
+  int kv_blocks;     // blocks that fill pages; in one launch the rest rotate q
   int q_heads;       // heads of q that one lane group takes
   int q_groups;      // lane groups for one token
 };
 
 // One page item: the new rows of one page, kv head, and k or v, by WARPS warps together.
-template <typename T, int D, int WARPS>
-__device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job, bool active,
+template <typename T, int D, int WARPS, bool ROTATES>
+__device__ __forceinline__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job, bool active,
                           int tid, float* red) {
   constexpr int kLanes = D / 16;             // lanes for a row
   constexpr int kRows = WARPS * 32 / kLanes;  // rows of one sweep
@@ -334,7 +334,7 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
   const int page = active ? page_of(c, s, static_cast<int>(index)) : -1;
   active = active && page >= 0;
   if (!active) b = a;
-  const int rot = !is_v && p.cos != nullptr ? p.rot_dim : 0;
+  const int rot = ROTATES && !is_v ? p.rot_dim : 0;
   if (p.cos != nullptr && active && page_pos + b > p.table_rows) {
     report_cache_index(c);  // positions that the table does not have are not stored
     const long long rows = p.table_rows - page_pos;
@@ -349,50 +349,104 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
   const T* base = src + (t0 + page_pos - begin) * st[0] + head * st[1];  // of slot 0
 
   // Two bf16 values near the type's largest can rotate past the range of 32 bits: rotated rows are
-  // held at half their size.
+  // taken at half their size.
   const int up = rot > 0 ? 1 : 0;
   const float half = rot > 0 ? 0.5f : 1.f;
-  float x[kKeep][8], y[kKeep][8];
-  float amax = 0.f;
-  auto fetch = [&](int slot, float(&fx)[8], float(&fy)[8]) {
-    widen<T>(load_unit<T>(base + slot * st[0], u), fx, fy);
-    if (u.angle >= 0) {
+  const bool turns = ROTATES && u.angle >= 0;
+  Raw kept[kKeep] = {};
+  float amax = 0.f, off = 0.f;  // the largest magnitude, and a bound on its error
+  auto look = [&](int slot, const Raw& raw) {
+    float x[8], y[8];
+    widen<T>(raw, x, y);
+    if (turns) {
       Angles an;
       load_angles(an, p, static_cast<int>(page_pos) + slot, u.angle, half);
-      rotate_unit(fx, fy, an, p.interleaved);
+      uint64_t pa[4], pb[4];
+      split_pairs(x, y, p.interleaved, pa, pb);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Bounded t = turn_bounded(pa[j], pb[j], an, j);
+        amax = fmax3(amax, fabsf(f2_lo(t.x)), fabsf(f2_hi(t.x)));  // passes over NaN
+        amax = fmax3(amax, fabsf(f2_lo(t.y)), fabsf(f2_hi(t.y)));
+        off = fmax3(off, f2_lo(t.w), f2_hi(t.w));
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        fx[i] *= half;
-        fy[i] *= half;
+        const float fx = fabsf(finite_or_nan(x[i] * half)), fy = fabsf(finite_or_nan(y[i] * half));
+        amax = fmax3(amax, fx, fy);
       }
     }
+  };
+  // The same exactly, where the bounds leave the scale open or a value is not finite.
+  auto look_again = [&](int slot, const Raw& raw) {
+    float x[8], y[8];
+    widen<T>(raw, x, y);
+    if (turns) {
+      Angles an;
+      load_angles(an, p, static_cast<int>(page_pos) + slot, u.angle, half);
+      uint64_t pa[4], pb[4];
+      split_pairs(x, y, p.interleaved, pa, pb);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      fx[i] = finite_or_nan(fx[i]);
-      fy[i] = finite_or_nan(fy[i]);
-      amax = fmaxf(amax, fmaxf(fabsf(fx[i]), fabsf(fy[i])));  // fmaxf passes over NaN
+      for (int j = 0; j < 4; ++j) {
+        float fa[2], fb[2];
+        turn_odd(pa[j], pb[j], an, j, fa, fb);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          amax = fmax3(amax, fabsf(finite_or_nan(fa[k])), fabsf(finite_or_nan(fb[k])));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float fx = fabsf(finite_or_nan(x[i] * half)), fy = fabsf(finite_or_nan(y[i] * half));
+        amax = fmax3(amax, fx, fy);
+      }
     }
   };
 #pragma unroll
   for (int w = 0; w < kKeep; ++w) {
     const int slot = a + row + w * kRows;
-    if (slot < b) fetch(slot, x[w], y[w]);
+    if (slot < b) kept[w] = load_unit<T>(base + slot * st[0], u);
   }
+#pragma unroll
+  for (int w = 0; w < kKeep; ++w) {
+    const int slot = a + row + w * kRows;
+    if (slot < b) look(slot, kept[w]);
+  }
+#pragma unroll 1
   for (int slot = a + row + kKeep * kRows; slot < b; slot += kRows) {
-    float fx[8], fy[8];
-    fetch(slot, fx, fy);
+    look(slot, load_unit<T>(base + slot * st[0], u));
   }
   float* scale = (is_v ? c.v_scale : c.k_scale) + (active ? page : 0) * static_cast<long long>(c.Hkv) + head;
   const float old = active && a > 0 ? *scale : 0.f;
+  auto group_max = [&](float v) {  // over the job's warps; the block comes here together
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if constexpr (WARPS > 1) {
-    if (lane == 0) red[tid >> 5] = amax;
-    __syncthreads();  // every job of the block comes here
-    amax = red[0];
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if constexpr (WARPS > 1) {
+      __syncthreads();  // the last values were read
+      if (lane == 0) red[tid >> 5] = v;
+      __syncthreads();
+      v = red[0];
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) amax = fmaxf(amax, red[i]);
+      for (int i = 1; i < WARPS; ++i) v = fmaxf(v, red[i]);
+    }
+    return v;
+  };
+  amax = group_max(amax);
+  if (ROTATES) {
+    off = group_max(off);
+    // amax + off may be infinite, which no exponent equals.
+    const bool open = needed_exp(amax + off, up) != needed_exp(fmaxf(amax - off, 0.f), up) ||
+                      !(amax + off < INFINITY);
+    if (WARPS > 1 ? __syncthreads_or(open) : __any_sync(0xffffffffu, open)) {
+      if (open) amax = 0.f;
+#pragma unroll 1
+      for (int slot = a + row; slot < b && open; slot += kRows) {
+        look_again(slot, load_unit<T>(base + slot * st[0], u));
+      }
+      amax = group_max(amax);
+    }
   }
   if (!active) return;
   int e = needed_exp(amax, up);
@@ -416,31 +470,83 @@ __device__ void fill_page(const AppendArgs& p, const Grid& g, int item, int job,
       *at = v;
     }
   }
-  auto put = [&](int slot, const float(&fx)[8], const float(&fy)[8]) {
+  auto put = [&](int slot, const Raw& raw) {
     unsigned char* at = dst + slot * dt;
-    *reinterpret_cast<uint2*>(at + u.lo) = to_e4m3x8(fx, mul);
-    *reinterpret_cast<uint2*>(at + u.hi) = to_e4m3x8(fy, mul);
+    float x[8], y[8];
+    widen<T>(raw, x, y);
+    uint2 wx, wy;
+    if (turns) {
+      Angles an;
+      load_angles(an, p, static_cast<int>(page_pos) + slot, u.angle, half);
+      uint64_t pa[4], pb[4];
+      split_pairs(x, y, p.interleaved, pa, pb);
+      const uint64_t mul2 = f2_pack(mul, mul);
+      uint32_t h[8];  // pairs of bytes: run lo, then run hi
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Bounded t = turn_bounded(pa[j], pb[j], an, j);
+        uint32_t f = to_e4m3x2(f2_mul(f2_add(t.x, t.w), mul2));
+        uint32_t g2 = to_e4m3x2(f2_mul(f2_add(t.y, t.w), mul2));
+        const uint32_t f1 = to_e4m3x2(f2_mul(f2_fma(t.w, kMinusOne2, t.x), mul2));
+        const uint32_t g1 = to_e4m3x2(f2_mul(f2_fma(t.w, kMinusOne2, t.y), mul2));
+        if (((f ^ f1) | (g2 ^ g1)) != 0) {
+          float fa[2], fb[2];
+          turn_odd(pa[j], pb[j], an, j, fa, fb);
+          f = to_e4m3x2(f2_pack(finite_or_nan(fa[0]) * mul, finite_or_nan(fa[1]) * mul));
+          g2 = to_e4m3x2(f2_pack(finite_or_nan(fb[0]) * mul, finite_or_nan(fb[1]) * mul));
+        }
+        if (p.interleaved) {
+          h[2 * j] = __byte_perm(f, g2, 0x0040);      // bytes f0, g0
+          h[2 * j + 1] = __byte_perm(f, g2, 0x0051);  // f1, g1
+        } else {
+          h[j] = f;
+          h[4 + j] = g2;
+        }
+      }
+      wx = make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
+      wy = make_uint2(__byte_perm(h[4], h[5], 0x5410), __byte_perm(h[6], h[7], 0x5410));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = finite_or_nan(x[i] * half);
+        y[i] = finite_or_nan(y[i] * half);
+      }
+      wx = to_e4m3x8(x, mul);
+      wy = to_e4m3x8(y, mul);
+    }
+    *reinterpret_cast<uint2*>(at + u.lo) = wx;
+    *reinterpret_cast<uint2*>(at + u.hi) = wy;
   };
 #pragma unroll
   for (int w = 0; w < kKeep; ++w) {
     const int slot = a + row + w * kRows;
-    if (slot < b) put(slot, x[w], y[w]);
+    if (slot < b) put(slot, kept[w]);
   }
+#pragma unroll 1
   for (int slot = a + row + kKeep * kRows; slot < b; slot += kRows) {
-    float fx[8], fy[8];
-    fetch(slot, fx, fy);
-    put(slot, fx, fy);
+    put(slot, load_unit<T>(base + slot * st[0], u));
   }
 }
 
 // g.q_heads heads of one packed row of q, by D / 16 lanes.
 template <typename T, int D>
-__device__ void rotate_q(const AppendArgs& p, const Grid& g, long long group, int lane) {
+__device__ __forceinline__ void rotate_q(const AppendArgs& p, const Grid& g, long long group, int lane) {
   constexpr int kLanes = D / 16;
   const CacheView& c = p.c;
   const long long t_ll = group / g.q_groups;
   const int t = t_ll < c.T ? static_cast<int>(t_ll) : c.T;
   const int h0 = static_cast<int>(group - t_ll * g.q_groups) * g.q_heads;
+  const Unit u = unit_of(lane % kLanes, p.rot_dim, p.interleaved);
+  const T* src = static_cast<const T*>(p.q) + t * p.sq[0];
+  T* dst = static_cast<T*>(p.q_out) + static_cast<long long>(t) * p.H * D;
+  const int h1 = t < c.T ? min(p.H, h0 + g.q_heads) : h0;
+  // Four heads' rows in flight, the first ones while the row's position is looked up.
+  constexpr int kAhead = 4;
+  Raw ring[kAhead] = {};
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    if (h0 + i < h1) ring[i] = load_unit<T>(src + (h0 + i) * p.sq[1], u);
+  }
   const int live = live_rows(c);
   int pos = -1;
   // The lanes of a warp hold up to 32 / kLanes rows: find the first one's sequence, then step on.
@@ -461,54 +567,83 @@ __device__ void rotate_q(const AppendArgs& p, const Grid& g, long long group, in
       pos = -1;
     }
   }
-  const Unit u = unit_of(lane % kLanes, p.rot_dim, p.interleaved);
   Angles an;
   if (pos >= 0 && u.angle >= 0) load_angles(an, p, pos, u.angle, 1.f);
-  const T* src = static_cast<const T*>(p.q) + t * p.sq[0];
-  T* dst = static_cast<T*>(p.q_out) + static_cast<long long>(t) * p.H * D;
-  const int h1 = min(p.H, h0 + g.q_heads);
-  Raw next = {};
-  if (pos >= 0) next = load_unit<T>(src + h0 * p.sq[1], u);
 #pragma unroll 1
-  for (int h = h0; h < h1; ++h) {
-    float x[8], y[8];
-    const Raw raw = next;  // zeros without a position
-    if (pos >= 0 && h + 1 < h1) next = load_unit<T>(src + (h + 1) * p.sq[1], u);
-    widen<T>(raw, x, y);
-    if (pos >= 0 && u.angle >= 0 && !rotate_unit_fast<T>(x, y, an, p.interleaved)) {
-      rotate_unit(x, y, an, p.interleaved);
+  for (int hb = h0; hb < h1; hb += kAhead) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int h = hb + i;
+      if (h >= h1) break;
+      const Raw raw = ring[i];
+      if (h + kAhead < h1) ring[i] = load_unit<T>(src + (h + kAhead) * p.sq[1], u);
+      uint32_t wx[4] = {raw.a.x, raw.a.y, raw.a.z, raw.a.w};
+      uint32_t wy[4] = {raw.b.x, raw.b.y, raw.b.z, raw.b.w};
+      if (pos < 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wx[k] = wy[k] = 0;
+      } else if (u.angle >= 0) {
+        float x[8], y[8];
+        widen<T>(raw, x, y);
+        rotate_to<T>(x, y, an, p.interleaved, wx, wy);
+      }
+      *reinterpret_cast<uint4*>(dst + h * D + u.lo) = make_uint4(wx[0], wx[1], wx[2], wx[3]);
+      *reinterpret_cast<uint4*>(dst + h * D + u.hi) = make_uint4(wy[0], wy[1], wy[2], wy[3]);
     }
-    uint4 a, b;
-    a.x = from_float2<T>(x[0], x[1]), a.y = from_float2<T>(x[2], x[3]);
-    a.z = from_float2<T>(x[4], x[5]), a.w = from_float2<T>(x[6], x[7]);
-    b.x = from_float2<T>(y[0], y[1]), b.y = from_float2<T>(y[2], y[3]);
-    b.z = from_float2<T>(y[4], y[5]), b.w = from_float2<T>(y[6], y[7]);
-    *reinterpret_cast<uint4*>(dst + h * D + u.lo) = a;
-    *reinterpret_cast<uint4*>(dst + h * D + u.hi) = b;
   }
 }
 
-// Blocks [0, kv_blocks) fill pages, the others rotate q.  ITEM_WARPS warps share a job: a page item
-// of one head, k or v.
-template <typename T, int D, int THREADS, int ITEM_WARPS>
-__global__ void __launch_bounds__(THREADS, 3) fa_cache_append_kernel(
+// ITEM_WARPS warps share a job: a page item of one head, k or v.
+template <typename T, int D, int ITEM_WARPS, bool ROTATES>
+__device__ __forceinline__ void fill_block(const AppendArgs& p, const Grid& g, int block) {
+  constexpr int kPerBlock = kThreads / 32 / ITEM_WARPS;
+  __shared__ float red[kThreads / 32];
+  const int sub = threadIdx.x / (32 * ITEM_WARPS);
+  const long long id = static_cast<long long>(block) * kPerBlock + sub;
+  const int jobs = 2 * p.c.Hkv;
+  const long long item = id / jobs;
+  const bool active = item < g.items;
+  fill_page<T, D, ITEM_WARPS, ROTATES>(p, g, active ? static_cast<int>(item) : 0,
+                                       static_cast<int>(id - item * jobs), active,
+                                       threadIdx.x % (32 * ITEM_WARPS), red + sub * ITEM_WARPS);
+}
+template <typename T, int D>
+__device__ __forceinline__ void rotate_block(const AppendArgs& p, const Grid& g, int block) {
+  rotate_q<T, D>(p, g, (static_cast<long long>(block) * kThreads + threadIdx.x) / (D / 16),
+                 threadIdx.x & 31);
+}
+
+// Few tokens: one launch, blocks [0, kv_blocks) fill pages, the others rotate q.
+template <typename T, int D, bool ROTATES>
+__global__ void __launch_bounds__(kThreads) fa_cache_append_kernel(
     const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
-  constexpr int kPerBlock = THREADS / 32 / ITEM_WARPS;
-  __shared__ float red[THREADS / 32];
-  const int tid = threadIdx.x;
-  if (blockIdx.x < static_cast<unsigned>(g.kv_blocks)) {
-    const int sub = tid / (32 * ITEM_WARPS);
-    const long long id = static_cast<long long>(blockIdx.x) * kPerBlock + sub;
-    const int jobs = 2 * p.c.Hkv;
-    const long long item = id / jobs;
-    const bool active = item < g.items;
-    fill_page<T, D, ITEM_WARPS>(p, g, active ? static_cast<int>(item) : 0,
-                                static_cast<int>(id - item * jobs), active,
-                                tid % (32 * ITEM_WARPS), red + sub * ITEM_WARPS);
+  const int block = blockIdx.x;
+  if (block < g.kv_blocks) {
+    fill_block<T, D, 1, ROTATES>(p, g, block);
+  } else if (ROTATES) {
+    rotate_block<T, D>(p, g, block - g.kv_blocks);
+  }
+}
+
+// Many: a launch each, with the registers that each needs (one kernel for both spilled at 80, and at
+// 128 had too few warps for the loads' latency).
+template <typename T, int D, int ITEM_WARPS, bool ROTATES>
+__global__ void __launch_bounds__(kThreads, 3) fa_cache_fill_kernel(
+    const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
+  fill_block<T, D, ITEM_WARPS, ROTATES>(p, g, blockIdx.x);
+}
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) fa_cache_turn_kernel(
+    const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
+  rotate_block<T, D>(p, g, blockIdx.x);
+}
+
+template <typename T, int D, int WARPS>
+void launch_fill(const AppendArgs& a, const Grid& g, unsigned blocks, cudaStream_t stream) {
+  if (a.cos != nullptr) {
+    fa_cache_fill_kernel<T, D, WARPS, true><<<blocks, kThreads, 0, stream>>>(a, g);
   } else {
-    const long long group =
-        (static_cast<long long>(blockIdx.x - g.kv_blocks) * THREADS + tid) / (D / 16);
-    rotate_q<T, D>(p, g, group, tid & 31);
+    fa_cache_fill_kernel<T, D, WARPS, false><<<blocks, kThreads, 0, stream>>>(a, g);
   }
 }
 
@@ -532,9 +667,9 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   // Few rows of a page come at a time: a warp for each job.  Else as many warps as hold a page's rows
   // of one head in registers, 32 values a thread: with more, most of a block's time is its chain of
   // lookups (eight warps for any page: 102 us for 16384 tokens of 12 heads of 64, pages of 32).
-  const int warps = mean < 8 ? 1 : std::min(8, page * D / 1024);
-  const int threads = 256;
-  const int per_block = threads / 32 / warps;
+  const bool few = mean < 8;
+  const int warps = few ? 1 : std::min(8, page * D / 1024);
+  const int per_block = kThreads / 32 / warps;
   const long long kv_blocks = (items * 2 * c.Hkv + per_block - 1) / per_block;
   long long q_blocks = 0;
   g.q_heads = 1;
@@ -542,18 +677,33 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   if (a.q != nullptr) {
     const long long rows = static_cast<long long>(c.T) * a.H;
     const long long fill = static_cast<long long>(multiprocessors()) * 1024 / kLanes;
-    while (g.q_heads < 8 && g.q_heads < a.H && rows / (2 * g.q_heads) >= fill) g.q_heads *= 2;
+    while (g.q_heads < a.H && rows / (2 * g.q_heads) >= fill) g.q_heads *= 2;
     g.q_groups = (a.H + g.q_heads - 1) / g.q_heads;
-    q_blocks = (static_cast<long long>(c.T) * g.q_groups * kLanes + threads - 1) / threads;
+    q_blocks = (static_cast<long long>(c.T) * g.q_groups * kLanes + kThreads - 1) / kThreads;
   }
   if (kv_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   g.kv_blocks = static_cast<int>(kv_blocks);
-  const unsigned blocks = static_cast<unsigned>(kv_blocks + q_blocks);
+  const bool turns = a.cos != nullptr;
+  if (few) {
+    const unsigned blocks = static_cast<unsigned>(kv_blocks + q_blocks);
+    if (turns) {
+      fa_cache_append_kernel<T, D, true><<<blocks, kThreads, 0, stream>>>(a, g);
+    } else {
+      fa_cache_append_kernel<T, D, false><<<blocks, kThreads, 0, stream>>>(a, g);
+    }
+    return cudaGetLastError();
+  }
+  const unsigned blocks = static_cast<unsigned>(kv_blocks);
   switch (warps) {
-    case 1: fa_cache_append_kernel<T, D, 256, 1><<<blocks, 256, 0, stream>>>(a, g); break;
-    case 2: fa_cache_append_kernel<T, D, 256, 2><<<blocks, 256, 0, stream>>>(a, g); break;
-    case 4: fa_cache_append_kernel<T, D, 256, 4><<<blocks, 256, 0, stream>>>(a, g); break;
-    default: fa_cache_append_kernel<T, D, 256, 8><<<blocks, 256, 0, stream>>>(a, g); break;
+    case 1: launch_fill<T, D, 1>(a, g, blocks, stream); break;
+    case 2: launch_fill<T, D, 2>(a, g, blocks, stream); break;
+    case 4: launch_fill<T, D, 4>(a, g, blocks, stream); break;
+    default: launch_fill<T, D, 8>(a, g, blocks, stream); break;
+  }
+  if (q_blocks > 0) {
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    fa_cache_turn_kernel<T, D><<<static_cast<unsigned>(q_blocks), kThreads, 0, stream>>>(a, g);
   }
   return cudaGetLastError();
 }
