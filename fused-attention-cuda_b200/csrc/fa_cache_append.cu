@@ -626,16 +626,18 @@ __global__ void __launch_bounds__(kThreads) fa_cache_append_kernel(
 }
 
 // Many: a launch each, with the registers that each needs (one kernel for both spilled at 80, and at
-// 128 had too few warps for the loads' latency).
+// 128 had too few warps for the loads' latency).  They need nothing of each other and run together.
 template <typename T, int D, int ITEM_WARPS, bool ROTATES>
 __global__ void __launch_bounds__(kThreads, 3) fa_cache_fill_kernel(
     const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   fill_block<T, D, ITEM_WARPS, ROTATES>(p, g, blockIdx.x);
 }
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) fa_cache_turn_kernel(
     const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
   rotate_block<T, D>(p, g, blockIdx.x);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // done only when the pages are
 }
 
 template <typename T, int D, int WARPS>
@@ -676,7 +678,7 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   g.q_groups = 1;
   if (a.q != nullptr) {
     const long long rows = static_cast<long long>(c.T) * a.H;
-    const long long fill = static_cast<long long>(multiprocessors()) * 1024 / kLanes;
+    const long long fill = static_cast<long long>(multiprocessors()) * 512 / kLanes;
     while (g.q_heads < a.H && rows / (2 * g.q_heads) >= fill) g.q_heads *= 2;
     g.q_groups = (a.H + g.q_heads - 1) / g.q_heads;
     q_blocks = (static_cast<long long>(c.T) * g.q_groups * kLanes + kThreads - 1) / kThreads;
@@ -703,7 +705,16 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   if (q_blocks > 0) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    fa_cache_turn_kernel<T, D><<<static_cast<unsigned>(q_blocks), kThreads, 0, stream>>>(a, g);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(q_blocks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fa_cache_turn_kernel<T, D>, a, g);
   }
   return cudaGetLastError();
 }
