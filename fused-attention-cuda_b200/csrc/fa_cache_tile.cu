@@ -33,14 +33,13 @@
 namespace fa_sm100 {
 namespace {
 
-constexpr int kThreads = 896;
+constexpr int kThreads = 640;
 constexpr int kRows = 256;   // query rows of a tile
 constexpr int kHalfRows = 128;
 constexpr int kKeys = 128;   // keys of a unit
 constexpr int kGroups = kKeys / 16;
 constexpr int kTables = 8;   // scale tables in flight: more than the tiles between load and softmax
-constexpr int kPairBarrier = 1;   // named barrier of both softmax groups
-constexpr int kGroupBarrier = 2;  // of group g: + g
+constexpr int kPairBarrier = 1;  // named barrier of the two softmax groups
 constexpr float kLazy = 8.0f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -56,9 +55,9 @@ struct Layout {
   static constexpr int kTable = kV16 + 2 * kTile16;
   static constexpr int kBars = kTable + kTables * kGroups * 32;
   // Barriers.
-  // kSFull, kPFull, kBaton: group g, half h at + 2 g + h.
+  // kSFull, kPFull: group g, half h at + 2 g + h.
   static constexpr int kK16Full = 0, kK16Empty = 2, kV16Full = 4, kV16Empty = 6, kSFull = 8,
-                       kPFull = 12, kODone = 16, kOFull = 18, kQFull = 20, kBaton = 22, kTabFull = 26,
+                       kPFull = 12, kODone = 16, kOFull = 18, kQFull = 20, kTabFull = 22,
                        kTabEmpty = kTabFull + kTables, kDrain = kTabEmpty + kTables,
                        kCount = kDrain + 1;
   static constexpr int kMisc = kBars + 8 * kCount;
@@ -379,21 +378,9 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-__device__ __forceinline__ void named_barrier(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
-// 16 columns of 32-bit tensor memory, one lane to a thread.
-__device__ __forceinline__ void tmem_ld16_wait(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+// The 256 threads of the two softmax groups.
+__device__ __forceinline__ void pair_barrier() {
+  asm volatile("bar.sync %0, 256;" ::"n"(kPairBarrier) : "memory");
 }
 
 template <typename T, int D>
@@ -406,7 +393,6 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   unsigned char* smem = smem_raw + (sbase - raw);
   __shared__ Finder finder;
   __shared__ Part parts[kThreads / 32];
-  __shared__ float row_m[2][kHalfRows], row_l[2][2][kHalfRows];  // of the softmax groups' rows
   RunScale* tables = reinterpret_cast<RunScale*>(smem + L::kTable);
   volatile int* clean = reinterpret_cast<volatile int*>(smem + L::kClean);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
@@ -435,12 +421,11 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       mbar_init(bar(L::kV16Empty + i), 2);
       mbar_init(bar(L::kODone + i), 1);
       mbar_init(bar(L::kOFull + i), 1);
-      mbar_init(bar(L::kQFull + i), 2 * kHalfRows);
+      mbar_init(bar(L::kQFull + i), kHalfRows);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(bar(L::kSFull + i), 1);
       mbar_init(bar(L::kPFull + i), kHalfRows);
-      mbar_init(bar(L::kBaton + i), kHalfRows);
     }
     for (int i = 0; i < kTables; ++i) {
       mbar_init(bar(L::kTabFull + i), 1);
@@ -455,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   const long long u_begin = blockIdx.x * per;
   if (u_begin >= total) return;  // the whole block
   const long long n_units = min(total - u_begin, per);
-  if (warp == 25) {
+  if (warp == 17) {
     tmem_alloc(smem_u32(tmem_slot), L::kCols);
     tmem_relinquish();
   }
@@ -474,34 +459,31 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
     return part.more;
   };
 
-  if (warp < 16) {
-    // ---------------------------------------------------------------- softmax: group g, half h
-    regs_alloc<80>();  // 512 x 80 + 256 x 64 + 128 x 56 = 896 x 72
-    const int g = warp >> 3, h = (warp >> 2) & 1;
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax groups
+    regs_alloc<136>();  // 256 x 136 + 256 x 72 + 128 x 64 = 640 x 96
+    const int g = warp >> 2;
     const int r = tid & 127;  // tensor-memory lane
     const uint32_t tl = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_col = tl + L::kColS + g * 128 + 64 * h, o_col = tl + L::kColO + g * 128;
-    volatile float* const my_m = &row_m[g][r];
-    unsigned my_tiles = 0, tiles_done = 0, parts_done = 0;
+    const uint32_t s_col = tl + L::kColS + g * 128, o_col = tl + L::kColO + g * 128;
+    unsigned steps_done = 0, tiles_done = 0, parts_done = 0;
     bool ok = true;
     bool first_part = true;
     do {
-      const bool pair = part.pair;
-      const int n_tiles = part.n_tiles;
       const SeqInfo q = part.t.q;
-      const int row = pair ? r : g * kHalfRows + r;
+      const int row = part.pair ? r : g * kHalfRows + r;
       const bool on = row < part.rows;
       const int token = on ? (part.row0 + row) / group : 0;
-      const int head = part.p.head * group + (on ? part.row0 + row - token * group : 0);
+      const int h = part.p.head * group + (on ? part.row0 + row - token * group : 0);
       const int limit = on ? (a.causal ? max(0, q.len - q.n + token + 1) : q.len) : 0;
-      const int tiles = pair ? (n_tiles - g + 1) / 2 : n_tiles;  // of this group
+      const int my_steps = 2 * (part.pair ? (part.n_tiles - g + 1) / 2 : part.n_tiles);  // halves
       float row_mul = a.scale * kLog2e;
       float m = -INFINITY, l = 0.f;
-      if (n_tiles > 0 && ok) {
-        // This thread's row of Q as fp16, swizzled, half of it; the row's other thread has the rest.
-        // Loops are kept short here and at the end of a part: code that runs once is fetched as it runs.
+      if (part.n_tiles > 0 && ok) {
+        // This thread's row of Q as fp16, swizzled.  Loops are kept short here and at the end of a
+        // part: code that runs once is fetched as it runs.
         const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const T*>(a.q) + static_cast<long long>(q.t0 + token) * a.sq[0] + head * a.sq[1]);
+            static_cast<const T*>(a.q) + static_cast<long long>(q.t0 + token) * a.sq[0] + h * a.sq[1]);
         float div = 1.f;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
           uint32_t big = 0;  // the largest magnitudes, as bits, of the two halves of a word
@@ -517,10 +499,10 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           div = __int_as_float((127 - e) << 23);
           row_mul *= __int_as_float((127 + e) << 23);
         }
-        if (!pair || g == 0) {
+        if (!part.pair || g == 0) {
           const uint32_t dst = sbase + L::kQ + g * L::kTile16 + r * 128;
-#pragma unroll 2
-          for (int i = h * (D / 16); i < (h + 1) * (D / 16); ++i) {
+#pragma unroll 4
+          for (int i = 0; i < D / 8; ++i) {
             uint4 v = on ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
               uint32_t* u = reinterpret_cast<uint32_t*>(&v);
@@ -536,85 +518,72 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           mbar_arrive(bar(L::kQFull + g));
         }
       }
-      // The first key that some row of this group does not see.
-      const int first_row = pair ? 0 : min(g * kHalfRows, part.rows - 1);
+      // The first key that some row of this half does not see.
+      const int first_row = part.pair ? 0 : min(g * kHalfRows, part.rows - 1);
       const int all_see = a.causal ? q.len - q.n + (part.row0 + first_row) / group + 1 : q.len;
-      const int tile0 = part.tile0;
-      for (int k = 0; k < tiles && ok; ++k) {
-        const int i = pair ? 2 * k + g : k;
+      for (int k = 0; k < my_steps && ok; ++k) {
+        const int half = k & 1, i = part.pair ? 2 * (k >> 1) + g : k >> 1;
         const unsigned at = tiles_done + i;
         const int slot = at % kTables;
-        const RunScale* table = tables + slot * kGroups + h * (kGroups / 2);
-        ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull) &&
-             wait_or_abort(bar(L::kSFull + 2 * g + h), my_tiles & 1, w, kStSFull);
+        const RunScale* table = tables + slot * kGroups + half * (kGroups / 2);
+        if (half == 0) ok = wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull);
+        float mul[kGroups / 2], add[kGroups / 2], inv[kGroups / 2];
+        if (ok) {
+#pragma unroll
+          for (int x = 0; x < kGroups / 2; ++x) {
+            const float4 sc = *reinterpret_cast<const float4*>(&table[x]);
+            mul[x] = fmaxf(sc.x * row_mul, 1.1754944e-38f);
+            add[x] = sc.y;
+            inv[x] = sc.z;
+          }
+          ok = wait_or_abort(bar(L::kSFull + 2 * g + half), (steps_done >> 1) & 1, w, kStSFull);
+        }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const int key0 = (tile0 + i) * kKeys + 64 * h;
-        const bool masked = key0 + 64 > all_see || !clean[slot];
-        uint32_t u[32];
-        auto load = [&](int part32) {  // 32 of the 64 scores
-          tmem_ld32_wait(s_col + 32 * part32, u);
-          if (masked) {
-            const int lim = limit - key0 - 32 * part32;
+        const uint32_t col0 = s_col + 64 * half;
+        const int key0 = (part.tile0 + i) * kKeys + 64 * half;
+        uint32_t u[64];
+        tmem_ld64_wait(col0, u);
+        if (key0 + 64 > all_see || !clean[slot]) {
+          const int lim = limit - key0;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int lx = table[2 * part32 + x].page < 0 ? 0 : lim;
+          for (int x = 0; x < kGroups / 2; ++x) {
+            const int lx = table[x].page < 0 ? 0 : lim;
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                if (16 * x + j >= lx) u[16 * x + j] = 0xff800000u;  // -inf
-              }
+            for (int j = 0; j < 16; ++j) {
+              if (16 * x + j >= lx) u[16 * x + j] = 0xff800000u;  // -inf
             }
           }
-        };
-        float top = -INFINITY;
-        auto maximum = [&](int part32) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            float b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              b[j] = fmaxf(__uint_as_float(u[16 * x + 4 * j]), __uint_as_float(u[16 * x + 4 * j + 1]));
-              b[j] = fmax3(b[j], __uint_as_float(u[16 * x + 4 * j + 2]),
-                           __uint_as_float(u[16 * x + 4 * j + 3]));
-            }
-            const RunScale& sc = table[2 * part32 + x];
-            top = fmaxf(top, fmaf(fmax3(b[0], b[1], fmaxf(b[2], b[3])),
-                                  fmaxf(sc.mul * row_mul, 1.1754944e-38f), sc.add));
-          }
-        };
-        load(1);
-        maximum(1);
-        load(0);
-        maximum(0);
-        // The two halves take turns at the row's maximum: this one's follows the other's last.
-        float before = -INFINITY;
-        if (k > 0 || h == 1) {
-          ok = wait_or_abort(bar(L::kBaton + 2 * g + h), (my_tiles - (h == 0 ? 1 : 0)) & 1, w, kStPFree);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          before = *my_m;
-          if (before != m) l *= m == -INFINITY ? 0.f : ex2_approx(m - before);
         }
-        const bool moved = top > before + kLazy || (before == -INFINITY && top != -INFINITY);
-        m = moved ? top : before;
-        *my_m = m;
-        mbar_arrive(bar(L::kBaton + 2 * g + (h ^ 1)));
-        const float alpha = moved ? (before == -INFINITY ? 0.f : ex2_approx(before - m)) : 1.f;
+        float top = m;
+#pragma unroll
+        for (int x = 0; x < kGroups / 2; ++x) {
+          float b[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            b[j] = fmaxf(__uint_as_float(u[16 * x + 4 * j]), __uint_as_float(u[16 * x + 4 * j + 1]));
+            b[j] = fmax3(b[j], __uint_as_float(u[16 * x + 4 * j + 2]),
+                         __uint_as_float(u[16 * x + 4 * j + 3]));
+          }
+          top = fmaxf(top, fmaf(fmax3(b[0], b[1], fmaxf(b[2], b[3])), mul[x], add[x]));
+        }
+        const bool moved = top > m + kLazy || (m == -INFINITY && top != -INFINITY);
+        const float alpha = moved ? (m == -INFINITY ? 0.f : ex2_approx(m - top)) : 1.f;
+        if (moved) m = top;
         const float ref = m == -INFINITY ? 0.f : m;
         l *= alpha;
-        auto weigh = [&](int part32) {  // P over scores that are no longer needed
+#pragma unroll
+        for (int x = 0; x < kGroups / 2; x += 2) {
           uint32_t pk[16];
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const float4 sc = *reinterpret_cast<const float4*>(&table[2 * part32 + y]);
-            const float mul = fmaxf(sc.x * row_mul, 1.1754944e-38f);
-            const uint64_t mul2 = f2_pack(mul, mul);
-            const uint64_t add2 = f2_pack(sc.y - ref, sc.y - ref);
+            const uint64_t mul2 = f2_pack(mul[x + y], mul[x + y]);
+            const uint64_t add2 = f2_pack(add[x + y] - ref, add[x + y] - ref);
             uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              const int at2 = 16 * y + 2 * j;
+              const int at2 = 16 * (x + y) + 2 * j;
               const uint64_t z =
                   f2_fma(f2_pack(__uint_as_float(u[at2]), __uint_as_float(u[at2 + 1])), mul2, add2);
               const float p0 = ex2_approx(f2_lo(z)), p1 = ex2_approx(f2_hi(z));
@@ -622,101 +591,94 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
               sum[j & 1] = f2_add(sum[j & 1], f2_pack(p0, p1));
             }
             const uint64_t both = f2_add(sum[0], sum[1]);
-            l = fmaf(f2_lo(both) + f2_hi(both), sc.z, l);
+            l = fmaf(f2_lo(both) + f2_hi(both), inv[x + y], l);
           }
-          tmem_st16(s_col + 16 * part32, pk);
-        };
-        weigh(0);
-        load(1);
-        weigh(1);
+          tmem_st16(col0 + 8 * x, pk);
+        }
         tmem_st_wait();
-        if ((k > 0 || h == 1) && __any_sync(0xffffffffu, moved)) {
-          // O follows the maximum once the step before, the other half's, has been added to it.  The
-          // barrier counts the group's steps: it cannot pass this one, whose P is still to come, and
-          // has passed the last but one, which this step's S comes after.
-          const unsigned step = 2 * my_tiles + h;
-          ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kODone + g), (step - 1) & 1, w, kStODone));
+        if (k > 0 && __any_sync(0xffffffffu, moved)) {
+          // O follows the maximum once the step before has been added to it.  The barrier counts this
+          // group's steps: it cannot pass this one, whose P is still to come, and has passed the last
+          // but one, which this step's S comes after.
+          ok = __all_sync(0xffffffffu, wait_or_abort(bar(L::kODone + g), (steps_done - 1) & 1, w, kStODone));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll 1
           for (int col = 0; col < D; col += 32) {
-            tmem_ld32_wait(o_col + col, u);
+            uint32_t o[32];
+            tmem_ld32_wait(o_col + col, o);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) u[j] = __float_as_uint(__uint_as_float(u[j]) * alpha);
-            tmem_st32(o_col + col, u);
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            tmem_st32(o_col + col, o);
           }
           tmem_st_wait();
         }
-        ++my_tiles;
+        ++steps_done;
         tc_fence_before();
-        mbar_arrive(bar(L::kPFull + 2 * g + h));
+        mbar_arrive(bar(L::kPFull + 2 * g + half));
       }
-      tiles_done += n_tiles;
-      if (tiles > 0 && ok) {
+      tiles_done += part.n_tiles;
+      if (my_steps > 0 && ok) {
         // A barrier of its own: of the last two steps' phases of kODone either may be the current one.
         ok = wait_or_abort(bar(L::kOFull + g), parts_done & 1, w, kStODone);
         ++parts_done;
-        if (h == 0) {  // the last step was the other half's
-          ok = ok && wait_or_abort(bar(L::kBaton + 2 * g), (my_tiles - 1) & 1, w, kStPFree);
-          const float last = *my_m;
-          if (last != m) l *= m == -INFINITY ? 0.f : ex2_approx(m - last);
-          m = last;
-        }
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
-      // Each half's sum of a row.  With alternating tiles group 0 merges: both groups' sums of a row lie
-      // in one lane of tensor memory.  Every thread comes to each of these barriers, whatever went wrong.
-      auto together = [&]() {
-        if (pair) {
-          named_barrier(kPairBarrier, 4 * kHalfRows);
-        } else {
-          named_barrier(kGroupBarrier + g, 2 * kHalfRows);
+      // Alternating tiles: group 0 merges.  Both groups' sums of a row are in one lane of tensor
+      // memory; (m, l) of group 1 go there too, over its scores.  Both groups come to each of these
+      // barriers, whatever went wrong.
+      const bool merge = part.pair && part.n_tiles > 1;
+      float m1 = -INFINITY, l1 = 0.f;
+      if (merge) {
+        if (g == 1) {
+          const uint32_t ml[8] = {__float_as_uint(m), __float_as_uint(l), 0, 0, 0, 0, 0, 0};
+          tmem_st8(s_col, ml);
+          tmem_st_wait();
+          tc_fence_before();
         }
-      };
-      row_l[g][h][r] = l;
-      if (h == 0) *my_m = m;
-      tc_fence_before();
-      together();
-      tc_fence_after();
-      const bool merge = pair && n_tiles > 1;
-      const float m1 = merge ? row_m[1][r] : -INFINITY;
-      const float l1 = merge ? row_l[1][0][r] + row_l[1][1][r] : 0.f;
-      l = row_l[g][0][r] + row_l[g][1][r];
+        pair_barrier();
+        if (g == 0) {
+          tc_fence_after();
+          uint32_t ml[32];
+          tmem_ld32_wait(tl + L::kColS + 128, ml);
+          m1 = __uint_as_float(ml[0]);
+          l1 = __uint_as_float(ml[1]);
+        }
+      }
       // Tensor-memory loads are by the warp: rows that are off take part and store nothing.
-      if (ok && (!pair || g == 0)) {
+      if (ok && (!part.pair || g == 0)) {
         const float top = fmaxf(m, m1);
         const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - top);
         const float f1 = m1 == -INFINITY ? 0.f : ex2_approx(m1 - top);
         // A row whose scores are all NaN has no maximum but a sum that is NaN.
         const float lsum = (m == -INFINITY ? l : l * f0) + (m1 == -INFINITY ? l1 : l1 * f1);
         const float w0 = lsum != lsum ? lsum : f0, w1 = lsum != lsum ? lsum : f1;
-        const bool whole = part.whole;
-        const float inv = whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
-        const long long at = static_cast<long long>(q.t0 + token) * a.H + head;
+        const float inv = part.whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
+        const long long at = static_cast<long long>(q.t0 + token) * a.H + h;
         float* slot = partials + (2ll * blockIdx.x + (first_part ? 0 : 1)) * L::kPartial;
 #pragma unroll 1
-        for (int col = h * (D / 2); col < (h + 1) * (D / 2); col += 16) {
-          uint32_t u[16];
-          float o[16];
+        for (int col = 0; col < D; col += 32) {
+          uint32_t u[32];
           __syncwarp();
-          if (tiles > 0) {
-            tmem_ld16_wait(o_col + col, u);
+          if (my_steps > 0) {
+            tmem_ld32_wait(o_col + col, u);
           } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) u[j] = 0;
+            for (int j = 0; j < 32; ++j) u[j] = 0;
           }
+          float o[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = __uint_as_float(u[j]) * w0;
+          for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(u[j]) * w0;
           if (merge) {
-            tmem_ld16_wait(o_col + 128 + col, u);
+            tmem_ld32_wait(o_col + 128 + col, u);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = fmaf(__uint_as_float(u[j]), w1, o[j]);
+            for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(u[j]), w1, o[j]);
           }
-          if (on && whole) {
+          if (on && part.whole) {
             uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at * D + col);
 #pragma unroll
-            for (int j = 0; j < 16; j += 8) {
+            for (int j = 0; j < 32; j += 8) {
               uint4 x;
               x.x = from_float2<T>(o[j] * inv, o[j + 1] * inv);
               x.y = from_float2<T>(o[j + 2] * inv, o[j + 3] * inv);
@@ -727,27 +689,24 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           } else if (on) {
             float4* dst = reinterpret_cast<float4*>(slot + row * D + col);
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) dst[j / 4] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            for (int j = 0; j < 32; j += 4) dst[j / 4] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
           }
         }
-        if (on && h == 0) {
-          if (whole) {
-            a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
-          } else {
-            slot[kRows * D + row] = top;
-            slot[kRows * D + kRows + row] = lsum;
-          }
+        if (on && part.whole) {
+          a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
+        } else if (on) {
+          slot[kRows * D + row] = top;
+          slot[kRows * D + kRows + row] = lsum;
         }
       }
-      tc_fence_before();
-      together();  // sums and O were read
+      if (merge) pair_barrier();  // group 1's sums were read
       first_part = false;
     } while (next_part());
-  } else if (warp < 24) {
+  } else if (warp < 16) {
     // ---------------------------------------------------------------- conversion
-    regs_dealloc<64>();
+    regs_dealloc<72>();
     constexpr int kPieces = D / 16, kStep = 128 / kPieces;  // kStep rows at a time
-    const int is_v = warp >= 20;
+    const int is_v = warp >= 12;
     // Eight lanes that store together have two neighbouring rows and four pieces of one 128-byte
     // chunk: their swizzled places are in different banks.
     const int t = tid & 127;
@@ -815,8 +774,8 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       if (more) fetch(++n);
     }
   } else {
-    regs_dealloc<56>();
-    if (warp == 24) {
+    regs_dealloc<64>();
+    if (warp == 16) {
       // -------------------------------------------------------------- pages
       // Lane 8 b + x looks after 16 keys (run x) of tile b of four; pages are looked up four tiles
       // ahead, their scales a tile later.
@@ -870,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
           if (lane == 0) mbar_arrive(bar(L::kTabFull + slot));
         }
       } while (ok && next_part());
-    } else if (warp < 27) {
+    } else if (warp < 19) {
       // -------------------------------------------------------------- products, a warp for each group
       // The whole warp walks the schedule and one lane issues: with every operand the same in all
       // lanes the compiler keeps them in uniform registers, where the instructions want them.  Two
@@ -879,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       constexpr uint32_t kIdescS = idesc_mma(0, 128, kKeys / 2, false);
       constexpr uint32_t kIdescPV = idesc_mma(0, 128, D, true);
       constexpr uint32_t kHalfBytes = (kKeys / 2) * 128;  // 64 keys of a 128-byte chunk
-      const int g = __shfl_sync(0xffffffffu, warp - 25, 0);
+      const int g = __shfl_sync(0xffffffffu, warp - 17, 0);
       const uint32_t base = __shfl_sync(0xffffffffu, sbase, 0);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t s_tm = tm + L::kColS + g * 128, o_tm = tm + L::kColO + g * 128;
@@ -980,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 25) tmem_dealloc(tmem, L::kCols);
+  if (warp == 17) tmem_dealloc(tmem, L::kCols);
 }
 
 // Merges the parts of a tile that several CTAs share.  Block i looks after the tile that CTA i's range
