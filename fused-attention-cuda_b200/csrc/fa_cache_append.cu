@@ -637,7 +637,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) fa_cache_turn_kernel(
     const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
   rotate_block<T, D>(p, g, blockIdx.x);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // done only when the pages are
+  wait_for_parts();  // done only when the pages are
 }
 
 template <typename T, int D, int WARPS>

@@ -672,17 +672,20 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
   long long incl;
   const long long total = finder.total(c, group, &w, &incl);
   const long long per = units_per_cta(total), begin = me * per;
-  if (me == 0 || begin >= total) return;
+  if (me == 0 || begin >= total) {
+    wait_for_parts();
+    return;
+  }
   finder.find(c, group, w, incl, begin);
   const long long seq_first = finder.at.first;
   w = work_of<kRows>(finder.at.q, group);
   const long long tuple = (begin - seq_first) / w.tiles;
   const long long first = seq_first + tuple * w.tiles, end = first + w.tiles;
+  wait_for_parts();
   if (first == begin || begin - per > first) return;
   const int head = static_cast<int>(tuple / w.row_tiles);
   const int row0 = static_cast<int>(tuple - static_cast<long long>(head) * w.row_tiles) * kRows;
   const int rows = min(kRows, w.q.n * group - row0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   int split = 1;  // rows side by side; the warps of a row share its parts
   while (split < rows && split < kCombineWarps) split *= 2;

@@ -68,6 +68,12 @@ __device__ __forceinline__ int page_of(const CacheView& c, int s, int i) {
   return p;
 }
 
+// In a kernel launched while the one before it runs: until that one's results are there.  Every block
+// of such a kernel comes here, so that its end is the end of both.
+__device__ __forceinline__ void wait_for_parts() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ float2 to_float2(uint32_t u);
 template <>

@@ -11,19 +11,28 @@
 //   warps 8-11   (K) and 12-15 (V) load e4m3 pages into registers, a tile ahead, and store them as
 //                fp16 in the swizzled layout of the products (exact; two buffers each): tcgen05 has
 //                no product of fp16 by e4m3, and rounding q and P to 8 bits would cost what the
-//                cache's own 8 bits cost again.  Registers and not TMA: a tile in flight takes no shared memory, which
-//                the fp16 buffers fill (with e4m3 tiles in shared memory V had one buffer, and its
-//                conversion, 1100 cycles, stood between two products: 608 us at 2048 x 16384 keys)
+//                cache's own 8 bits cost again.  Registers and not TMA: a tile in flight takes no
+//                shared memory, which the fp16 buffers fill.  (With e4m3 tiles in shared memory V had
+//                one buffer, and its conversion, 1100 cycles, stood between two products.)
 //   warps 17, 18 issue S = Q K^T and O += P V of a group each
 //   warps 0-3, 4-7   two softmax groups, a row to a thread.  With more than 128 rows group g has rows
 //                128 g .. and every key tile; otherwise both have the same rows and the key tiles
-//                alternate, and their sums are merged at the end (both lie in one lane of tensor memory).  Either way step i belongs to group
-//                i & 1, and the tensor core works for one group while the other exponentiates.
+//                alternate, and their sums are merged at the end (both lie in one lane of tensor
+//                memory).  Either way the tensor core works for one group while the other
+//                exponentiates.
 //
 // A key tile goes through in two halves of 64 keys: S_g has two buffers of 64 columns in tensor memory,
 // P_g (fp16) overwrites the first 32 of its own, O_g takes D.  While a group exponentiates one half
-// the products of the other are under way.  (With one S of 128 columns a group waited for its PV and its
-// next S, 1800 of 5900 cycles.)
+// the products of the other are under way.
+//
+// What bounds it: 2048 new tokens of 32 heads over 16384 keys of 8 heads of 128 take 640 us, 800 TFLOP/s,
+// about 4600 cycles for 256 rows by 128 keys where the products alone need 2048.  A group's softmax of
+// 64 keys takes 2250 cycles (maximum 500, exponentials 1000, the rest loads, stores and hand-offs), and
+// the products, S reading both operands from shared memory and sharing it with the conversion's stores,
+// 3400 of the 4600.  Measured and not kept: one S of 128 columns (a group waits for its products, 5900
+// cycles), four softmax groups with a row's maximum handed from half to half (650 us), a quarter of the
+// exponentials as polynomials on the FMA pipes (638 us), products issued by one lane of a diverged warp
+// (738 us: operands have to move to uniform registers one by one).
 #include <algorithm>
 #include <cmath>
 
@@ -957,14 +966,13 @@ __global__ void __launch_bounds__(kThreads) fa_cache_tile_merge_kernel(
   long long per;
   const long long total = finder.find(c, group, a.causal, me, &per);
   const long long begin = me * per;
-  if (me == 0 || begin >= total) return;
   const Place p = finder.at;
-  if (p.tile == 0 || p.tile > per) return;
+  wait_for_parts();
+  if (me == 0 || begin >= total || p.tile == 0 || p.tile > per) return;
   const SeqTiles t = tiles_of(finder.q, group, a.causal);
   const long long first = begin - p.tile, end = first + t.of(p.j, group);
   const int last = static_cast<int>((end - 1) / per);  // the last CTA with a part
   const int row0 = p.j * kRows, rows = min(kRows, t.rows - row0);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int row = warp; row < rows; row += kWarps) {
     float top = -INFINITY, lsum = 0.f, acc[kPer] = {};
     for (int i0 = me - 1; i0 <= last; i0 += kBatch) {

@@ -400,6 +400,167 @@ def test_attention_random_batches(seed):
     check_attention(s, causal=r.random() < 0.7, scale=r.choice([None, 0.02, 0.5]))
 
 
+# ---- the same with many rows a sequence, which another kernel serves ----
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("lens,new", [([300], [300]), ([129, 128, 127], [60, 128, 127]), ([700, 40], [90, 33]),
+                                      ([64, 500, 1], [64, 1, 1])], ids=str)
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+def test_many_rows(lens, new, causal, dtype, D):
+    check_attention(Setup(lens, new, H=8, Hkv=2, D=D, dtype=dtype, page=32, seed=41, tail=2), causal)
+
+
+@pytest.mark.parametrize("H,Hkv", [(3, 3), (7, 1), (130, 1), (300, 1)])
+def test_many_rows_groups(H, Hkv):
+    """Groups that do not divide a tile, up to more heads than a tile has rows."""
+    check_attention(Setup([90, 200], [40, 3], H=H, Hkv=Hkv, D=64, page=64, seed=42, dtype=torch.float16))
+
+
+def test_many_rows_without_keys():
+    s = Setup([20, 0, 50], [60, 40, 50], H=8, Hkv=1, seed=43)
+    o, lse = s.attend()
+    check_attention(s, o=o, lse=lse)
+    assert bool((lse[:40] == math.inf).all()) and bool((lse[60:100] == math.inf).all()) and not bool(o[:40].any())
+
+
+def test_many_rows_scales_and_garbage():
+    """Scales over twenty binades, NaN behind every sequence and in unused pages."""
+    s = Setup([333, 64, 200], [30, 64, 41], H=8, Hkv=2, seed=44, page=32, dtype=torch.bfloat16)
+    s.k_scale.copy_(torch.exp2(3 * torch.randn(s.P, s.Hkv, generator=s.g) - 8))
+    s.v_scale.copy_(torch.exp2(5 * torch.randn(s.P, s.Hkv, generator=s.g)).clamp(2**-10, 2**10))
+    used = torch.zeros(s.P, s.page, dtype=torch.bool)
+    for seq, n in enumerate(s.lens):
+        for pos in range(n):
+            used[s.table[seq, pos // s.page], pos % s.page] = True
+    dead = ~used[:, None, :, None].expand(s.P, s.Hkv, s.page, s.D).cuda()
+    for c, sc in ((s.k_cache, s.k_scale), (s.v_cache, s.v_scale)):
+        c.view(torch.uint8).masked_fill_(dead, 0x7F)
+        sc[~used.any(1).cuda()] = math.nan
+    clean = s.pages()
+    for x in clean[:2]:
+        x.nan_to_num_()
+    for x in clean[2:]:
+        x.nan_to_num_(1.0)
+    s.pages = lambda: clean
+    check_attention(s)
+
+
+def test_many_rows_long_chunk_against_64_bits():
+    """Tiles that several CTAs share, over many key tiles, against fp64 on the GPU."""
+    for D, H, Hkv, n, L in ((128, 8, 2, 300, 20000), (64, 4, 1, 77, 90001), (128, 16, 1, 5, 70000)):
+        page = 64
+        counts = -(-L // page)
+        g = torch.Generator(device="cuda").manual_seed(45)
+        pools = [torch.randn(counts, Hkv, page, D, generator=g, device="cuda").to(E4M3) for _ in range(2)]
+        scales = [torch.exp2(torch.randint(-2, 3, (counts, Hkv), generator=g, device="cuda").float()) for _ in "kv"]
+        table = torch.randperm(counts, generator=g, device="cuda").int()[None]
+        q = torch.randn(n, H, D, generator=g, device="cuda").bfloat16()
+        lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+        o, lse = fused_attn.cache_attention(q, *pools, *scales, table, lens, return_lse=True)
+        assert fused_attn.last_device_error() == (0, 0)
+        ids = table[0].long()
+        k, v = ((x.view(torch.uint8)[ids].view(E4M3).double() * sc[ids].double()[..., None, None]).transpose(0, 1)
+                .reshape(Hkv, -1, D)[:, :L] for x, sc in zip(pools, scales))
+        hidden = torch.arange(L, device="cuda")[None] > torch.arange(n, device="cuda")[:, None] + (L - n)
+        for h in range(H):
+            a = (q[:, h].double() @ k[h * Hkv // H].T / D**0.5).masked_fill_(hidden, -math.inf)
+            p = torch.softmax(a, -1)
+            want = p @ v[h * Hkv // H]
+            room = p @ v[h * Hkv // H].abs() * 2.0**-10 + want.abs() * 2.0**-8 + 1e-6
+            assert bool(((o[:, h].double() - want).abs() <= room).all())
+            assert bool(((lse[:, h].double() - torch.logsumexp(a, -1)).abs() < 1e-4).all())
+
+
+def test_many_rows_repeat_bit_for_bit():
+    s = Setup([1500, 40, 700], [200, 40, 333], H=8, Hkv=2, seed=46, page=64)
+    o, lse = s.attend()
+    for _ in range(10):
+        o2, lse2 = s.attend()
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("new", [1, 40], ids=["tokens", "rows"])
+def test_many_sequences(new):
+    """More sequences than a block has threads, some without new tokens, some without keys."""
+    r = random.Random(7)
+    S = 1400
+    n = [0 if i % 97 == 5 else r.choice([1, new]) if new > 1 else 1 for i in range(S)]
+    lens = [0 if i % 131 == 7 else m + r.choice([0, 3, 150]) for i, m in enumerate(n)]
+    s = Setup(lens, n, H=4, Hkv=1, D=64, page=32, rot=64, seed=47, dtype=torch.float16)
+    before = s.pages()
+    q = s.append()
+    s.q = q
+    o, lse = s.attend()
+    # tokens in front of the cache (sequences that hold nothing) are reported, the others stored
+    assert fused_attn.last_device_error()[0] in (0, 1)
+    picks = sorted({0, 5, 7, 8, 700, 701, S - 1, *(r.randrange(S) for _ in range(20))})
+    after = s.pages()
+    for i in picks:
+        rows = slice(s.cu[i], s.cu[i + 1])
+        sub = [0, s.cu[i + 1] - s.cu[i]]
+        table = [s.table[i].tolist()]
+        page_ids = [p for p in table[0] if p >= 0]
+        want = ref.Pages(*(x.clone() for x in before))
+        ref.append(want, s.k[rows], s.v[rows], table, [lens[i]], sub, cos=s.cos, sin=s.sin)
+        for a, b in zip(after, want):
+            assert torch.equal(a[page_ids], b[page_ids])
+        got = ref.attention(after, q[rows], table, [lens[i]], sub)
+        half = torch.finfo(torch.float16).eps / 2
+        assert bool(((o[rows].cpu().double() - got.o).abs() <= got.o_room * 1.01 + got.o.abs() * half + 1e-7).all())
+        fin = torch.isfinite(got.lse)
+        assert bool(((lse[rows].cpu().double() - got.lse)[fin].abs() <= got.lse_room[fin]).all())
+        assert bool((lse[rows].cpu()[~fin] == math.inf).all())
+
+
+def test_bad_device_values_with_many_rows():
+    def fresh():
+        return Setup([120, 233], [64, 50], H=4, Hkv=2, seed=48, page=32)
+
+    for what in ("page", "length", "negative length", "offsets", "offset order"):
+        s, good = fresh(), fresh()
+        if what == "page":
+            s.table_d[0, 1] = s.P
+        elif what == "length":
+            s.lens_d[0] = 10**6
+        elif what == "negative length":
+            s.lens_d[0] = -5
+        elif what == "offsets":
+            s.cu_d[2] = 1000
+        elif what == "offset order":
+            s.cu_d[0] = 70
+        o, _ = s.attend()
+        torch.cuda.synchronize()
+        assert fused_attn.last_device_error() == (1, 1 << 11), what
+        o_good, _ = good.attend()
+        if what in ("page", "length", "negative length"):  # the second sequence is as it should be
+            assert bool(((o[64:] - o_good[64:]).abs().float() <= 0.02 * o_good[64:].abs().float() + 0.02).all())
+        assert fused_attn.last_device_error() == (0, 0)
+
+
+def test_many_rows_in_a_graph_on_another_stream():
+    s = Setup([150, 300], [100, 60], H=8, Hkv=2, rot=128, seed=49, page=64)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        q = s.append()
+        s.attend(q=q)
+        with torch.cuda.graph(g, stream=side):
+            q = s.append()
+            o, lse = s.attend(q=q)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(3):
+        o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        kept, s.q = s.q, q
+        check_attention(s, o=o, lse=lse)
+        s.q = kept
+    del g
+
+
 # ---- together, and how they are called ----
 
 
