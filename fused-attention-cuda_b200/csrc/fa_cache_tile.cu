@@ -165,8 +165,9 @@ struct Place {
 };
 
 // All CTAs add up the units of the sequences and find the place that their own range begins at.
+template <int THREADS>
 struct Finder {
-  long long warp[kThreads / 32];
+  long long warp[THREADS / 32];
   SeqInfo q;
   long long first;
   Place at;
@@ -183,7 +184,7 @@ struct Finder {
     __syncthreads();
     *sum = 0;
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) {
+    for (int i = 0; i < THREADS / 32; ++i) {
       if (i < wid) x += warp[i];
       *sum += warp[i];
     }
@@ -198,7 +199,7 @@ struct Finder {
       first = 0;
     }
     long long mine = 0, incl = 0, total = 0, sum;
-    for (int base = 0; base < c.n_seqs; base += kThreads) {
+    for (int base = 0; base < c.n_seqs; base += THREADS) {
       const int s = base + threadIdx.x;
       mine = s < c.n_seqs ? tiles_of(seq_info(c, s), group, causal).units * c.Hkv : 0;
       incl = total + scan(mine, &sum);
@@ -208,9 +209,9 @@ struct Finder {
     const long long unit = cta * *per;
     if (unit < total) {
       long long run = 0;
-      for (int base = 0; base < c.n_seqs; base += kThreads) {
+      for (int base = 0; base < c.n_seqs; base += THREADS) {
         const int s = base + threadIdx.x;
-        if (c.n_seqs > kThreads) {
+        if (c.n_seqs > THREADS) {
           mine = s < c.n_seqs ? tiles_of(seq_info(c, s), group, causal).units * c.Hkv : 0;
           incl = run + scan(mine, &sum);
           run += sum;
@@ -262,7 +263,8 @@ struct Part {
   bool whole;
   bool more;         // false behind the last part
 
-  __device__ void start(const Finder& f, int group, bool causal, long long units) {
+  template <int THREADS>
+  __device__ void start(const Finder<THREADS>& f, int group, bool causal, long long units) {
     t = tiles_of(f.q, group, causal);
     p = f.at;
     left = units;
@@ -347,6 +349,14 @@ __device__ __forceinline__ uint4 ldg128(const unsigned char* p) {
                : "l"(p));
   return v;
 }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z),
                "r"(v.w)
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t sbase = (raw + 1023u) & ~1023u;
   unsigned char* smem = smem_raw + (sbase - raw);
-  __shared__ Finder finder;
+  __shared__ Finder<kThreads> finder;
   __shared__ Part parts[kThreads / 32];
   RunScale* tables = reinterpret_cast<RunScale*>(smem + L::kTable);
   volatile int* clean = reinterpret_cast<volatile int*>(smem + L::kClean);
@@ -489,40 +499,58 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       float row_mul = a.scale * kLog2e;
       float m = -INFINITY, l = 0.f;
       if (part.n_tiles > 0 && ok) {
-        // This thread's row of Q as fp16, swizzled.  Loops are kept short here and at the end of a
-        // part: code that runs once is fetched as it runs.
-        const uint4* src = reinterpret_cast<const uint4*>(
-            static_cast<const T*>(a.q) + static_cast<long long>(q.t0 + token) * a.sq[0] + h * a.sq[1]);
-        float div = 1.f;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          uint32_t big = 0;  // the largest magnitudes, as bits, of the two halves of a word
-#pragma unroll 4
-          for (int i = 0; i < D / 8; ++i) {
-            const uint4 v = on ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-            big = __vmaxu2(__vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
-                                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)), big);
-          }
-          const uint32_t top = max(big & 0xffffu, big >> 16);  // infinities and NaN: no division
-          const int e = top > 0 && top < 0x7f80u
-                            ? min(119, max(-118, static_cast<int>(top >> 7) - 127 - 8)) : 0;
-          div = __int_as_float((127 - e) << 23);
-          row_mul *= __int_as_float((127 + e) << 23);
-        }
-        if (!part.pair || g == 0) {
-          const uint32_t dst = sbase + L::kQ + g * L::kTile16 + r * 128;
-#pragma unroll 4
-          for (int i = 0; i < D / 8; ++i) {
-            uint4 v = on ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-              uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+        // The warp's 32 rows of Q as fp16, swizzled: neighbouring lanes have neighbouring 16 bytes of a
+        // row (a row to a thread touched 32 lines with every load), all loads first.
+        constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
+        const int sub = lane / kLanes, piece = lane % kLanes;
+        const int r0 = (warp & 3) * 32 + sub;
+        const int row1 = part.pair ? r0 : g * kHalfRows + r0;
+        int token1 = (part.row0 + row1) / group;
+        int h1 = part.row0 + row1 - token1 * group;
+        const int rows_left = part.rows - row1;
+        const T* const q0 = static_cast<const T*>(a.q) + static_cast<long long>(q.t0) * a.sq[0] +
+                            static_cast<long long>(part.p.head) * group * a.sq[1] + piece * 8;
+        uint4 v[kLanes];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 f = to_float2<T>(u[k]);
-                u[k] = from_float2<__half>(f.x * div, f.y * div);
-              }
-            }
-            sts128(dst + (i >> 3) * L::kChunkBytes + (((i & 7) ^ (r & 7)) * 16), v);
+        for (int i = 0; i < kLanes; ++i) {
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (i * kRowsAtOnce < rows_left) {
+            v[i] = __ldg(reinterpret_cast<const uint4*>(q0 + token1 * a.sq[0] + h1 * a.sq[1]));
           }
+          for (h1 += kRowsAtOnce; h1 >= group; h1 -= group) ++token1;
+        }
+        int e_own = 0;
+#pragma unroll
+        for (int i = 0; i < kLanes; ++i) {
+          const int r1 = r0 + i * kRowsAtOnce;
+          if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            uint32_t big = __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                                    __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o /= 2) {
+              big = __vmaxu2(big, __shfl_xor_sync(0xffffffffu, big, o));
+            }
+            const uint32_t top = max(big & 0xffffu, big >> 16);  // infinities and NaN: no division
+            const int e = top > 0 && top < 0x7f80u
+                              ? min(119, max(-118, static_cast<int>(top >> 7) - 127 - 8)) : 0;
+            const float div = __int_as_float((127 - e) << 23);
+            uint32_t* u = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = to_float2<T>(u[k]);
+              u[k] = from_float2<__half>(f.x * div, f.y * div);
+            }
+            const int got = __shfl_sync(0xffffffffu, e, (lane % kRowsAtOnce) * kLanes);
+            if (lane / kRowsAtOnce == i) e_own = got;
+          }
+          if (!part.pair || g == 0) {
+            sts128(sbase + L::kQ + g * L::kTile16 + r1 * 128 + (piece >> 3) * L::kChunkBytes +
+                       (((piece & 7) ^ (r1 & 7)) * 16),
+                   v[i]);
+          }
+        }
+        row_mul *= __int_as_float((127 + e_own) << 23);
+        if (!part.pair || g == 0) {
           fence_proxy_async_smem();
           mbar_arrive(bar(L::kQFull + g));
         }
@@ -666,6 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         const float inv = part.whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
         const long long at = static_cast<long long>(q.t0 + token) * a.H + h;
         float* slot = partials + (2ll * blockIdx.x + (first_part ? 0 : 1)) * L::kPartial;
+        const uint32_t stage = sbase + L::kQ + g * L::kTile16 + (warp & 3) * 4096;
 #pragma unroll 1
         for (int col = 0; col < D; col += 32) {
           uint32_t u[32];
@@ -684,22 +713,46 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(u[j]), w1, o[j]);
           }
-          if (on && part.whole) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at * D + col);
+          // Through shared memory (Q's, which every S has read), so that neighbouring lanes store
+          // neighbouring 16 bytes of a row.
+          if (part.whole) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
+            for (int j = 0; j < 4; ++j) {
               uint4 x;
-              x.x = from_float2<T>(o[j] * inv, o[j + 1] * inv);
-              x.y = from_float2<T>(o[j + 2] * inv, o[j + 3] * inv);
-              x.z = from_float2<T>(o[j + 4] * inv, o[j + 5] * inv);
-              x.w = from_float2<T>(o[j + 6] * inv, o[j + 7] * inv);
-              dst[j / 8] = x;
+              x.x = from_float2<T>(o[8 * j] * inv, o[8 * j + 1] * inv);
+              x.y = from_float2<T>(o[8 * j + 2] * inv, o[8 * j + 3] * inv);
+              x.z = from_float2<T>(o[8 * j + 4] * inv, o[8 * j + 5] * inv);
+              x.w = from_float2<T>(o[8 * j + 6] * inv, o[8 * j + 7] * inv);
+              sts128(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16), x);
             }
-          } else if (on) {
-            float4* dst = reinterpret_cast<float4*>(slot + row * D + col);
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) dst[j / 4] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+            for (int i = 0; i < 4; ++i) {
+              const int r1 = 8 * i + (lane >> 2), piece = lane & 3;
+              const uint4 x = lds128(stage + r1 * 64 + ((piece ^ ((r1 >> 1) & 3)) * 16));
+              const long long at1 = __shfl_sync(0xffffffffu, at, r1);
+              if (row - lane + r1 < part.rows) {
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at1 * D + col + 8 * piece) = x;
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              sts128(stage + lane * 128 + ((j ^ (lane & 7)) * 16),
+                     make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
+                                __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3])));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r1 = 4 * i + (lane >> 3), piece = lane & 7;
+              const uint4 x = lds128(stage + r1 * 128 + ((piece ^ (r1 & 7)) * 16));
+              if (row - lane + r1 < part.rows) {
+                *reinterpret_cast<uint4*>(slot + (row - lane + r1) * D + col + 4 * piece) = x;
+              }
+            }
           }
+          __syncwarp();
         }
         if (on && part.whole) {
           a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
@@ -952,13 +1005,15 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
 }
 
 // Merges the parts of a tile that several CTAs share.  Block i looks after the tile that CTA i's range
-// begins inside of, if no earlier CTA's does too; a warp for each row.
+// begins inside of, if no earlier CTA's does too; a warp for each row, kMergeBlocks blocks for a tile (one:
+// 26 us where CTAs share 147 tiles of 256 rows).
+constexpr int kMergeBlocks = 4, kMergeThreads = 256;
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) fa_cache_tile_merge_kernel(
+__global__ void __launch_bounds__(kMergeThreads) fa_cache_tile_merge_kernel(
     const __grid_constant__ CacheAttnArgs a, const float* partials) {
   using L = Layout<D>;
-  constexpr int kPer = D / 32, kWarps = kThreads / 32, kBatch = 4;
-  __shared__ Finder finder;
+  constexpr int kPer = D / 32, kWarps = kMergeThreads / 32, kBatch = 4;
+  __shared__ Finder<kMergeThreads> finder;
   const CacheView& c = a.c;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = a.H / c.Hkv;
@@ -973,7 +1028,7 @@ __global__ void __launch_bounds__(kThreads) fa_cache_tile_merge_kernel(
   const long long first = begin - p.tile, end = first + t.of(p.j, group);
   const int last = static_cast<int>((end - 1) / per);  // the last CTA with a part
   const int row0 = p.j * kRows, rows = min(kRows, t.rows - row0);
-  for (int row = warp; row < rows; row += kWarps) {
+  for (int row = blockIdx.y * kWarps + warp; row < rows; row += gridDim.y * kWarps) {
     float top = -INFINITY, lsum = 0.f, acc[kPer] = {};
     for (int i0 = me - 1; i0 <= last; i0 += kBatch) {
       float pm[kBatch], pl[kBatch], v[kBatch][kPer];
@@ -1034,8 +1089,8 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   if (units == 1) return cudaSuccess;  // no tile has two units
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(ctas, kMergeBlocks);
+  cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = stream;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
