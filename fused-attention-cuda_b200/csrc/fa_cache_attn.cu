@@ -252,17 +252,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
   const int group = a.H / c.Hkv;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // Rows behind the last sequence.
-  {
-    const int live = live_rows(c);
-    const long long n = static_cast<long long>(c.T - live) * a.H;
-    T* o = static_cast<T*>(a.o) + static_cast<long long>(live) * a.H * D;
-    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + tid; i < n * (D / 8);
-         i += static_cast<long long>(gridDim.x) * kThreads) {
-      reinterpret_cast<uint4*>(o)[i] = make_uint4(0, 0, 0, 0);
-      if (i % (D / 8) == 0) a.lse[static_cast<long long>(live) * a.H + i / (D / 8)] = 0.f;
-    }
-  }
+  zero_stray_rows<T, D, kThreads>(a);
 
   SeqWork w;
   long long incl;

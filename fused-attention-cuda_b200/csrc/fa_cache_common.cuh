@@ -21,13 +21,18 @@ __device__ __forceinline__ void report_cache_index(const CacheView& c) {
   atomicOr(c.status, kStCacheIndex);
 }
 
+// The packed rows of sequence s lie in the batch, and those of the first one begin it.
+__device__ __forceinline__ bool offsets_ok(const CacheView& c, int s, int t0, int end) {
+  return t0 >= 0 && end >= t0 && end <= c.T && (s > 0 || t0 == 0);
+}
+
 __device__ __forceinline__ SeqInfo seq_info(const CacheView& c, int s) {
   SeqInfo q;
   int len = c.seq_lens[s];
   if (c.cu_seqlens != nullptr) {
     q.t0 = c.cu_seqlens[s];
     const int end = c.cu_seqlens[s + 1];
-    if (q.t0 < 0 || end < q.t0 || end > c.T) {
+    if (!offsets_ok(c, s, q.t0, end)) {
       report_cache_index(c);
       q.t0 = 0;
       q.n = 0;
@@ -52,6 +57,35 @@ __device__ __forceinline__ int live_rows(const CacheView& c) {
   if (c.cu_seqlens == nullptr) return c.T;
   const int end = c.cu_seqlens[c.n_seqs];
   return end < 0 ? 0 : (end > c.T ? c.T : end);
+}
+
+// Zeros in the rows of attention's outputs that belong to no sequence, by all threads of all blocks:
+// those behind the last one or, where an offset is out of order, each row that no sequence has.
+template <typename T, int D, int THREADS>
+__device__ __forceinline__ void zero_stray_rows(const CacheAttnArgs& a) {
+  const CacheView& c = a.c;
+  if (c.cu_seqlens == nullptr) return;
+  const int live = live_rows(c);
+  bool bad = false;
+  for (int s = threadIdx.x; s < c.n_seqs; s += THREADS) {
+    bad |= !offsets_ok(c, s, c.cu_seqlens[s], c.cu_seqlens[s + 1]);
+  }
+  bad = __syncthreads_or(bad);
+  for (int t = (bad ? 0 : live) + static_cast<int>(blockIdx.x); t < c.T; t += gridDim.x) {
+    bool stray = true;
+    if (bad) {
+      for (int s = threadIdx.x; s < c.n_seqs; s += THREADS) {
+        const int t0 = c.cu_seqlens[s], end = c.cu_seqlens[s + 1];
+        stray &= !(offsets_ok(c, s, t0, end) && t >= t0 && t < end);
+      }
+      stray = __syncthreads_and(stray);
+    }
+    if (!stray) continue;
+    const long long at = static_cast<long long>(t) * a.H;
+    uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + at * D);
+    for (int i = threadIdx.x; i < a.H * (D / 8); i += THREADS) o[i] = make_uint4(0, 0, 0, 0);
+    for (int h = threadIdx.x; h < a.H; h += THREADS) a.lse[at + h] = 0.f;
+  }
 }
 
 // The page of sequence s that holds its keys [i << page_shift, ...), or -1 (reported).

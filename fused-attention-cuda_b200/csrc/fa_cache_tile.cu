@@ -422,16 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   const int group = a.H / c.Hkv;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  {  // rows behind the last sequence
-    const int live = live_rows(c);
-    const long long n = static_cast<long long>(c.T - live) * a.H;
-    T* o = static_cast<T*>(a.o) + static_cast<long long>(live) * a.H * D;
-    for (long long i = static_cast<long long>(blockIdx.x) * kThreads + tid; i < n * (D / 8);
-         i += static_cast<long long>(gridDim.x) * kThreads) {
-      reinterpret_cast<uint4*>(o)[i] = make_uint4(0, 0, 0, 0);
-      if (i % (D / 8) == 0) a.lse[static_cast<long long>(live) * a.H + i / (D / 8)] = 0.f;
-    }
-  }
+  zero_stray_rows<T, D, kThreads>(a);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(L::kK16Full + i), 4);

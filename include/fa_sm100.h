@@ -129,8 +129,9 @@ size_t fa_noalloc_scratch_bytes(void);
  * last ones of their sequences: new token i of n sits at position len - n + i.  These arrays live
  * in device memory and are checked there: a page, length, offset or position out of range is
  * skipped and reported by fa_last_device_error (cudaErrorInvalidValue), never followed.  Entries
- * of block_table behind a sequence's last page are not read.  Rows of the packed tensors behind
- * cu_seqlens[n_seqs] belong to no sequence: nothing is stored for them, and outputs get zeros. */
+ * of block_table behind a sequence's last page are not read.  cu_seqlens begins with 0.  Rows of the
+ * packed tensors that belong to no sequence -- behind cu_seqlens[n_seqs], or of a sequence whose
+ * offsets are out of order -- store nothing, and outputs get zeros there. */
 typedef struct fa_cache {
   void* k;
   void* v;

@@ -677,6 +677,27 @@ def test_bad_device_values_are_skipped_and_reported():
         fused_attn.last_device_error()
 
 
+@pytest.mark.parametrize("new", [[4, 3, 2], [40, 33, 50]])
+@pytest.mark.parametrize("offset,value,skipped", [(0, 2, [0]), (1, -1, [0, 1]), (1, 10**6, [0, 1]), (3, 10**6, [2])])
+def test_rows_of_sequences_with_bad_offsets_are_zero(new, offset, value, skipped):
+    s = Setup([60, 70, 80], new, rot=128, seed=26)
+    rows = sum(new)
+    bounds = s.cu_d.tolist()
+    s.cu_d[offset] = value
+    garbage = torch.full((rows * s.H * s.D * 4,), float("nan"), device="cuda")  # what a reused block may hold
+    del garbage
+    q = s.append()
+    o, lse = s.attend()
+    torch.cuda.synchronize()
+    assert fused_attn.last_device_error() == (1, 1 << 11)
+    assert bool(torch.isfinite(o).all()) and bool(torch.isfinite(lse).all())
+    for i in range(len(new)):
+        part = slice(bounds[i], bounds[i + 1])
+        zero = i in skipped
+        assert bool((o[part] == 0).all()) == zero and bool((lse[part] == 0).all()) == zero
+        assert bool((q[part] == 0).all()) == zero
+
+
 def test_refusals_of_the_op():
     s = Setup([20, 33], [4, 3], rot=128, seed=24)
     args = dict(k=s.k, v=s.v, k_cache=s.k_cache, v_cache=s.v_cache, k_scale=s.k_scale, v_scale=s.v_scale,
