@@ -19,7 +19,8 @@
 // Knuth, rounded to odd in 32 bits (the last bit set where it is inexact), so that the rounding that
 // follows is that of the exact value.  A page's scale is settled likewise, by bounds on its largest
 // magnitude.  13613 tokens of 32 + 8 + 8 heads of 128, where the memory needs 47 us: 64-bit arithmetic
-// 129 us (conversions, 16 a cycle), every sum as two floats 105 us.
+// 129 us (conversions, 16 a cycle), every sum as two floats or these bounds 105 to 113 us (q alone 54, k
+// and v 59, of which the rotation 36: instructions bound it, not the memory).
 #include <algorithm>
 #include <cmath>
 
@@ -613,7 +614,7 @@ __device__ __forceinline__ void rotate_block(const AppendArgs& p, const Grid& g,
                  threadIdx.x & 31);
 }
 
-// Few tokens: one launch, blocks [0, kv_blocks) fill pages, the others rotate q.
+// One launch, a warp for each job: blocks [0, kv_blocks) fill pages, the others rotate q.
 template <typename T, int D, bool ROTATES>
 __global__ void __launch_bounds__(kThreads) fa_cache_append_kernel(
     const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
@@ -625,8 +626,7 @@ __global__ void __launch_bounds__(kThreads) fa_cache_append_kernel(
   }
 }
 
-// Many: a launch each, with the registers that each needs (one kernel for both spilled at 80, and at
-// 128 had too few warps for the loads' latency).  They need nothing of each other and run together.
+// A launch each, several warps for a job.  They need nothing of each other and run together.
 template <typename T, int D, int ITEM_WARPS, bool ROTATES>
 __global__ void __launch_bounds__(kThreads, 3) fa_cache_fill_kernel(
     const __grid_constant__ AppendArgs p, const __grid_constant__ Grid g) {
@@ -666,13 +666,18 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   }
   if (items > 0x7fffffffll) return cudaErrorInvalidValue;
   g.items = static_cast<int>(items);
-  // Few rows of a page come at a time: a warp for each job.  Else as many warps as hold a page's rows
-  // of one head in registers, 32 values a thread: with more, most of a block's time is its chain of
-  // lookups (eight warps for any page: 102 us for 16384 tokens of 12 heads of 64, pages of 32).
-  const bool few = mean < 8;
-  const int warps = few ? 1 : std::min(8, page * D / 1024);
+  // A job (a page item of one head, k or v) costs its warps a chain of lookups and then its rows one
+  // sweep after the other.  With many jobs for their rows a warp for each, and q in the same launch:
+  // the chains of many jobs hide each other, and a block waits for nothing.  With few, as many warps as
+  // hold a page's rows in registers, 32 values a thread, and a launch for q.  Measured, us, a warp / more:
+  // 16 x 1024 tokens of 12 heads of 64, pages of 32 (12672 jobs) 18 / 24; 64 x 64 of 32 + 8 heads of 128,
+  // pages of 64 (2048) 32 / 41; 2048, pages of 32 (1072) 18 / 20, of 64 (544) 26 / 19, of 128 (288) 48 / 20;
+  // 64 x 128, pages of 128 (2048) 81 / 69.  A job's time goes with its rows and D, and so does the border.
+  const long long jobs = items * 2 * c.Hkv;
+  const bool one_launch = mean < 8 || jobs >= static_cast<long long>(std::min(mean, page)) * D / 4;
+  const int warps = one_launch ? 1 : std::min(8, page * D / 1024);
   const int per_block = kThreads / 32 / warps;
-  const long long kv_blocks = (items * 2 * c.Hkv + per_block - 1) / per_block;
+  const long long kv_blocks = (jobs + per_block - 1) / per_block;
   long long q_blocks = 0;
   g.q_heads = 1;
   g.q_groups = 1;
@@ -686,7 +691,7 @@ cudaError_t launch_t(const AppendArgs& a, cudaStream_t stream) {
   if (kv_blocks + q_blocks > 0x7fffffffll) return cudaErrorInvalidValue;
   g.kv_blocks = static_cast<int>(kv_blocks);
   const bool turns = a.cos != nullptr;
-  if (few) {
+  if (one_launch) {
     const unsigned blocks = static_cast<unsigned>(kv_blocks + q_blocks);
     if (turns) {
       fa_cache_append_kernel<T, D, true><<<blocks, kThreads, 0, stream>>>(a, g);
