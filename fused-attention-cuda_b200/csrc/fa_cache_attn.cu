@@ -13,6 +13,24 @@
 //
 // bf16 queries enter the products as fp16 after division by a power of two for each row: 8
 // significant bits fit in fp16's 11, so this is exact but for values 2^-23 below the row's largest.
+//
+// A query row is (token, head of the group), so a kv head's keys are read once for all of its heads.
+// Up to 32 rows of a sequence go through mma.sync with the keys as M and 8 rows as N: tcgen05's 128
+// rows would be mostly padding, and the bytes of the cache, not the products, bound these calls.  Each
+// warp takes runs of 16 keys from a ring that TMA fills, with its own maximum and sum; nothing in the
+// loop waits for another warp.  All sequences' units of 64 keys are numbered and split evenly over the
+// CTAs (lengths live on the device, so a captured call follows them); tiles that several CTAs share
+// leave fp32 partials, which a second kernel, launched while the first runs, merges.
+//
+// What bounds it: 64 sequences of 97 to 8191 keys of 8 heads of 128, one token of 32 heads each, 554 MB,
+// take 113 us (84 at the measured copy rate), one of 131071 keys 63 us (41): about 6.5 TB/s and some
+// 15 us that do not depend on the length (the table's and the first page's latency, the merge).  5 tokens
+// of 32 heads, 20 rows, take 70 us for 153 MB: the products' instructions and the softmax of 24 rows.
+// 777 keys take 12.6 us, two kernels of some 7 us that are chains of latencies.  One sequence's tables
+// were looked up by each run before (142 us for the first of these), rows as M (171 us).
+//
+// A stored value that is NaN makes all output rows NaN that are computed in one product with a row that
+// sees its key: rows with the same heads and tokens next to each other, whether they see it or not.
 #include <algorithm>
 #include <cmath>
 
@@ -682,69 +700,69 @@ __global__ void __launch_bounds__(32 * kCombineWarps) fa_cache_combine_kernel(
   const int share = warp / split, shares = kCombineWarps / split;
   const int last = static_cast<int>((end - 1) / per);  // the last CTA with a part
   for (int row = warp % split; row - warp % split < rows; row += split) {
-  float top = -INFINITY, lsum = 0.f, acc[kPer] = {};
-  if (row < rows) {
-    constexpr int kBatch = 4;  // parts in flight
-    for (int i0 = me - 1 + share; i0 <= last; i0 += kBatch * shares) {
-      float pm[kBatch], pl[kBatch], v[kBatch][kPer];
+    float top = -INFINITY, lsum = 0.f, acc[kPer] = {};
+    if (row < rows) {
+      constexpr int kBatch = 4;  // parts in flight
+      for (int i0 = me - 1 + share; i0 <= last; i0 += kBatch * shares) {
+        float pm[kBatch], pl[kBatch], v[kBatch][kPer];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int i = i0 + b * shares;
-        pm[b] = -INFINITY;
-        pl[b] = 0.f;
-        if (i <= last) {
-          // Its first part, unless it is the one that this tuple starts inside of.
-          const int slot = i * per >= first ? 0 : 1;
-          const float* part = partials + (2ll * i + slot) * L::kPartial;
-          pm[b] = part[kRows * D + row];
-          pl[b] = part[kRows * D + kRows + row];
+        for (int b = 0; b < kBatch; ++b) {
+          const int i = i0 + b * shares;
+          pm[b] = -INFINITY;
+          pl[b] = 0.f;
+          if (i <= last) {
+            // Its first part, unless it is the one that this tuple starts inside of.
+            const int slot = i * per >= first ? 0 : 1;
+            const float* part = partials + (2ll * i + slot) * L::kPartial;
+            pm[b] = part[kRows * D + row];
+            pl[b] = part[kRows * D + kRows + row];
 #pragma unroll
-          for (int k = 0; k < kPer; ++k) v[b][k] = part[row * D + lane * kPer + k];
+            for (int k = 0; k < kPer; ++k) v[b][k] = part[row * D + lane * kPer + k];
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          if (pm[b] == -INFINITY && pl[b] == 0.f) continue;
+          const float to = fmaxf(top, pm[b]);
+          const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - to);
+          const float f1 = pm[b] == -INFINITY ? 1.f : ex2_approx(pm[b] - to);
+          top = to;
+          lsum = lsum * f0 + pl[b] * f1;
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f0 + v[b][k] * f1;
         }
       }
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        if (pm[b] == -INFINITY && pl[b] == 0.f) continue;
-        const float to = fmaxf(top, pm[b]);
-        const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - to);
-        const float f1 = pm[b] == -INFINITY ? 1.f : ex2_approx(pm[b] - to);
-        top = to;
-        lsum = lsum * f0 + pl[b] * f1;
-#pragma unroll
-        for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f0 + v[b][k] * f1;
-      }
     }
-  }
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) sums[warp][lane * kPer + k] = acc[k];
-  if (lane == 0) {
-    tops[warp] = top;
-    lsums[warp] = lsum;
-  }
-  __syncthreads();
-  if (share == 0 && row < rows) {
-  for (int i = 1; i < shares; ++i) {
-    const int other = warp + i * split;
-    const float pm = tops[other], pl = lsums[other];
-    if (pm == -INFINITY && pl == 0.f) continue;
-    const float to = fmaxf(top, pm);
-    const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - to);
-    const float f1 = pm == -INFINITY ? 1.f : ex2_approx(pm - to);
-    top = to;
-    lsum = lsum * f0 + pl * f1;
+    for (int k = 0; k < kPer; ++k) sums[warp][lane * kPer + k] = acc[k];
+    if (lane == 0) {
+      tops[warp] = top;
+      lsums[warp] = lsum;
+    }
+    __syncthreads();
+    if (share == 0 && row < rows) {
+      for (int i = 1; i < shares; ++i) {
+        const int other = warp + i * split;
+        const float pm = tops[other], pl = lsums[other];
+        if (pm == -INFINITY && pl == 0.f) continue;
+        const float to = fmaxf(top, pm);
+        const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - to);
+        const float f1 = pm == -INFINITY ? 1.f : ex2_approx(pm - to);
+        top = to;
+        lsum = lsum * f0 + pl * f1;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f0 + sums[other][lane * kPer + k] * f1;
-  }
-  const int token = (row0 + row) / group;
-  const long long at = static_cast<long long>(w.q.t0 + token) * a.H + head * group +
-                       (row0 + row - token * group);
-  const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
-  uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + at * D + lane * kPer);
+        for (int k = 0; k < kPer; ++k) acc[k] = acc[k] * f0 + sums[other][lane * kPer + k] * f1;
+      }
+      const int token = (row0 + row) / group;
+      const long long at = static_cast<long long>(w.q.t0 + token) * a.H + head * group +
+                           (row0 + row - token * group);
+      const float inv = lsum == 0.f ? 0.f : 1.f / lsum;
+      uint32_t* o = reinterpret_cast<uint32_t*>(static_cast<T*>(a.o) + at * D + lane * kPer);
 #pragma unroll
-  for (int k = 0; k < kPer; k += 2) o[k / 2] = from_float2<T>(acc[k] * inv, acc[k + 1] * inv);
-  if (lane == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
-  }
-  __syncthreads();  // the next rows' sums take the place of these
+      for (int k = 0; k < kPer; k += 2) o[k / 2] = from_float2<T>(acc[k] * inv, acc[k + 1] * inv);
+      if (lane == 0) a.lse[at] = lsum == 0.f ? INFINITY : (top + log2f(lsum)) * kLn2;
+    }
+    __syncthreads();  // the next rows' sums take the place of these
   }
 }
 
@@ -785,6 +803,9 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
 }
 
 // Query rows of a tile in eights, by a sequence's mean; 0: the kernel on tcgen05 (fa_cache_tile.cu).
+// 32 sequences of 500 to 4003 keys, rows: this kernel / the other, us.  32 + 8 heads of 128: 16: 58 / 107,
+// 32: 93 / 110, 36: 157 / 112, 64: 172 / 113; 16 + 4 heads of 64: 32: 37 / 52, 36: 52 / 52, 64: 55 / 53,
+// 128: 99 / 58.
 int row_eights(int H, int Hkv, int T, int n_seqs) {
   const long long rows = static_cast<long long>(T) * (H / Hkv);
   return rows > 32ll * n_seqs ? 0 : static_cast<int>(std::max(1ll, (rows + 8ll * n_seqs - 1) / (8ll * n_seqs)));
