@@ -25,12 +25,9 @@
 // What bounds it: 64 sequences of 97 to 8191 keys of 8 heads of 128, one token of 32 heads each, 554 MB,
 // take 113 us (84 at the measured copy rate), one of 131071 keys 63 us (41): about 6.5 TB/s and some
 // 15 us that do not depend on the length (the table's and the first page's latency, the merge).  5 tokens
-// of 32 heads, 20 rows, take 70 us for 153 MB: the products' instructions and the softmax of 24 rows.
+// of 32 heads, 20 rows, take 74 us for 153 MB: the products' instructions and the softmax of 24 rows.
 // 777 keys take 12.6 us, two kernels of some 7 us that are chains of latencies.  One sequence's tables
 // were looked up by each run before (142 us for the first of these), rows as M (171 us).
-//
-// A stored value that is NaN makes all output rows NaN that are computed in one product with a row that
-// sees its key: rows with the same heads and tokens next to each other, whether they see it or not.
 #include <algorithm>
 #include <cmath>
 
@@ -447,6 +444,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
       l[x][0] = l[x][1] = 0.f;
     }
 
+    uint32_t nans = 0;  // V's NaN that were taken out (nan_columns)
     for (int i = 0; i < n_runs; ++i) {
       const int stage = taken % L::kStages;
       if (alive) alive = wait_copy(bars + 8 * stage, (taken / L::kStages) & 1, a);
@@ -485,7 +483,8 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
       }
       const int key0 = first_key + i * kTile;
       const bool ragged = key0 + kRun > w.q.len || sc.page < 0;
-      if (key0 + kRun > all_see || sc.page < 0) {
+      const bool masked = key0 + kRun > all_see || sc.page < 0;
+      if (masked) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -551,6 +550,14 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) vw[k][j] = 0;
         }
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const uint32_t n = nan_bytes(vw[k][j]);
+            vw[k][j] &= ~n;
+            nans |= n;
+          }
+        }
       }
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {  // columns 4j .. 4j + 3 of the lane's
@@ -586,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
         }
       }
     }
-    __syncthreads();  // and no warp reads its ring any more
+    const bool spoiled = __syncthreads_or(nans != 0);  // and no warp reads its ring any more
     float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
@@ -631,8 +638,21 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
           out[k].x += x.x, out[k].y += x.y, out[k].z += x.z, out[k].w += x.w;
         }
       }
+      const int token = (row0 + row) / group;
+      if (spoiled) {
+        const int see = a.causal ? max(0, w.q.len - w.q.n + token + 1) : w.q.len;
+        const uint32_t bits = nan_columns<8>(c, s, head, max(tile0 * kTile, all_see & ~(kRun - 1)),
+                                             min(see, tile1 * kTile), col);
+        const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (bits >> (4 * k) & 1) out[k].x = nan;
+          if (bits >> (4 * k) & 2) out[k].y = nan;
+          if (bits >> (4 * k) & 4) out[k].z = nan;
+          if (bits >> (4 * k) & 8) out[k].w = nan;
+        }
+      }
       if (whole) {
-        const int token = (row0 + row) / group;
         const long long at = static_cast<long long>(w.q.t0 + token) * a.H + head * group +
                              (row0 + row - token * group);
         const float inv = lsum == 0.f ? 0.f : 1.f / lsum;

@@ -102,6 +102,34 @@ __device__ __forceinline__ int page_of(const CacheView& c, int s, int i) {
   return p;
 }
 
+// A key that some rows of a tile see and others do not has weight 0 in the latter, but 0 times NaN is
+// NaN.  Where a tile's rows differ in what they see, the kernels therefore take V's NaN out (e4m3 has
+// no infinities), note it, and at the end put NaN where it belongs: the columns of nan_columns in the
+// rows that see the key.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t v) {  // 0xff in the bytes that are NaN
+  return __vcmpeq4(v & 0x7f7f7f7fu, 0x7f7f7f7fu);
+}
+
+// Bit i: column col + i (col, COLS multiples of 4) of V is NaN in one of the keys [lo, hi).
+template <int COLS>
+__device__ __forceinline__ uint32_t nan_columns(const CacheView& c, int s, int head, int lo, int hi,
+                                                int col) {
+  uint32_t bits = 0;
+#pragma unroll 1
+  for (int key = lo; key < hi; ++key) {
+    const int page = page_of(c, s, key >> c.page_shift);
+    if (page < 0) continue;
+    const unsigned char* at = c.v + page * c.vs[0] + head * c.vs[1] +
+                              (key & ((1 << c.page_shift) - 1)) * c.vs[2] + col;
+#pragma unroll
+    for (int i = 0; i < COLS / 4; ++i) {
+      const uint32_t n = nan_bytes(*reinterpret_cast<const uint32_t*>(at + 4 * i)) & 0x08040201u;
+      bits |= ((n | n >> 8 | n >> 16 | n >> 24) & 15u) << (4 * i);
+    }
+  }
+  return bits;
+}
+
 // In a kernel launched while the one before it runs: until that one's results are there.  Every block
 // of such a kernel comes here, so that its end is the end of both.
 __device__ __forceinline__ void wait_for_parts() {

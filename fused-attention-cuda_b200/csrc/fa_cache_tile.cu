@@ -25,14 +25,15 @@
 // P_g (fp16) overwrites the first 32 of its own, O_g takes D.  While a group exponentiates one half
 // the products of the other are under way.
 //
-// What bounds it: 2048 new tokens of 32 heads over 16384 keys of 8 heads of 128 take 640 us, 800 TFLOP/s,
-// about 4600 cycles for 256 rows by 128 keys where the products alone need 2048.  A group's softmax of
+// What bounds it: 2048 new tokens of 32 heads over 16384 keys of 8 heads of 128 take 650 us, 790 TFLOP/s,
+// about 4700 cycles for 256 rows by 128 keys where the products alone need 2048.  A group's softmax of
 // 64 keys takes 2250 cycles (maximum 500, exponentials 1000, the rest loads, stores and hand-offs), and
 // the products, S reading both operands from shared memory and sharing it with the conversion's stores,
-// 3400 of the 4600.  Measured and not kept: one S of 128 columns (a group waits for its products, 5900
+// 3400 of the 4700.  Measured and not kept: one S of 128 columns (a group waits for its products, 5900
 // cycles), four softmax groups with a row's maximum handed from half to half (650 us), a quarter of the
 // exponentials as polynomials on the FMA pipes (638 us), products issued by one lane of a diverged warp
-// (738 us: operands have to move to uniform registers one by one).
+// (738 us: operands have to move to uniform registers one by one).  Taking V's NaN out of the tiles on the
+// diagonal is 10 of the 650.
 #include <algorithm>
 #include <cmath>
 
@@ -416,6 +417,8 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
   volatile int* clean = reinterpret_cast<volatile int*>(smem + L::kClean);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  // One more than the last tile that NaN were taken out of V of (see nan_columns).
+  unsigned* last_nan = reinterpret_cast<unsigned*>(smem + L::kMisc + 8);
   auto bar = [sbase](int i) -> uint32_t { return sbase + L::kBars + 8u * i; };
   const CacheView& c = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -443,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
     }
     mbar_init(bar(L::kDrain), 2);
     *abort_flag = 0;
+    *last_nan = 0;
     fence_mbar_init();
   }
   long long per;
@@ -645,6 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         tc_fence_before();
         mbar_arrive(bar(L::kPFull + 2 * g + half));
       }
+      const unsigned first_tile = tiles_done;
       tiles_done += part.n_tiles;
       if (my_steps > 0 && ok) {
         // A barrier of its own: of the last two steps' phases of kODone either may be the current one.
@@ -686,6 +691,8 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
         const long long at = static_cast<long long>(q.t0 + token) * a.H + h;
         float* slot = partials + (2ll * blockIdx.x + (first_part ? 0 : 1)) * L::kPartial;
         const uint32_t stage = sbase + L::kQ + g * L::kTile16 + (warp & 3) * 4096;
+        // A later part's tiles may be counted already: then the search finds nothing.
+        const bool spoiled = *reinterpret_cast<volatile unsigned*>(last_nan) > first_tile;
 #pragma unroll 1
         for (int col = 0; col < D; col += 32) {
           uint32_t u[32];
@@ -703,6 +710,16 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
             tmem_ld32_wait(o_col + 128 + col, u);
 #pragma unroll
             for (int j = 0; j < 32; ++j) o[j] = fmaf(__uint_as_float(u[j]), w1, o[j]);
+          }
+          if (spoiled && part.n_tiles > 0) {
+            const int diag = max(0, q.len - q.n + part.row0 / group + 1) & ~(kKeys - 1);
+            const uint32_t bits = nan_columns<32>(
+                c, part.p.s, part.p.head, max(part.tile0 * kKeys, diag),
+                min(limit, (part.tile0 + part.n_tiles) * kKeys), col);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (bits >> j & 1) o[j] = __int_as_float(0x7fffffff);
+            }
           }
           // Through shared memory (Q's, which every S has read), so that neighbouring lanes store
           // neighbouring 16 bytes of a row.
@@ -776,8 +793,11 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
     int i = 0, n_tiles = part.n_tiles;
     uint4 kv[kPieces];
     // This thread's pieces of tile i of the part, zeros where no key is.
+    bool masked = false;  // V of a tile that not all rows see all of
     auto fetch = [&](unsigned at) {
       const int slot = at % kTables;
+      const long long tokens = (part.tile0 + i + 1ll) * kKeys - (part.t.q.len - part.t.q.n) - 1;
+      masked = is_v && a.causal && tokens * group > part.row0;
       ok = __all_sync(0xffffffffu,
                       wait_or_abort(bar(L::kTabFull + slot), (at / kTables) & 1, w, kStKFull));
       if (!ok) return;
@@ -809,6 +829,17 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       ok = n < 2 || wait_or_abort(bar(empty + st), ((n >> 1) & 1) ^ 1, w, kStKVEmpty);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      if (masked) {
+        uint32_t nans = 0;
+#pragma unroll
+        for (int x = 0; x < kPieces; ++x) {
+          const uint4 f = make_uint4(nan_bytes(kv[x].x), nan_bytes(kv[x].y), nan_bytes(kv[x].z),
+                                     nan_bytes(kv[x].w));
+          nans |= f.x | f.y | f.z | f.w;
+          kv[x] = make_uint4(kv[x].x & ~f.x, kv[x].y & ~f.y, kv[x].z & ~f.z, kv[x].w & ~f.w);
+        }
+        if (nans != 0) atomicMax(last_nan, n + 1);
+      }
 #pragma unroll
       for (int x = 0; x < kPieces; ++x) {
         store_wide(lo + st * L::kTile16 + x * kStep * 128, hi + st * L::kTile16 + x * kStep * 128, kv[x]);

@@ -319,6 +319,31 @@ def test_attention_nan_in_a_visible_key_reaches_its_rows_only():
     assert bool(torch.isfinite(o[0, 2:]).all()) and bool(torch.isfinite(o[1]).all())
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,new", [([50, 40], [8, 3]), ([700, 300], [5, 7]), ([300, 180], [200, 60]),
+                                      ([2600, 40], [300, 40])])
+def test_attention_nan_in_a_value_stays_with_the_rows_that_see_it(lens, new, D):
+    """A value that is NaN behind a causal row's own position does not reach it: 0 weights and NaN."""
+    s = Setup(lens, new, D=D, seed=27)
+    clean_o, clean_lse = s.attend()
+    first = 0
+    want = torch.zeros(sum(new), s.H, D, dtype=torch.bool)
+    group = s.H // s.Hkv
+    for i, (length, n) in enumerate(zip(lens, new)):
+        for back, head, col in ((n // 2, 0, 5), (1, 1, D - 1), (n - 1, 1, 33)):
+            key = length - back  # new token n - back
+            s.v_cache.view(torch.uint8)[s.table[i, key // s.page].item(), head, key % s.page, col] = 0xFF
+            want[first + n - back:first + n, head * group:(head + 1) * group, col] = True
+        first += n
+    o, lse = s.attend()
+    torch.cuda.synchronize()
+    assert torch.equal(torch.isnan(o).cpu(), want)
+    assert torch.equal(lse, clean_lse)
+    keep = ~want.cuda()
+    assert torch.equal(o[keep], clean_o[keep])
+    assert fused_attn.last_device_error() == (0, 0)
+
+
 def test_attention_layouts_agree():
     """Token-major pools, strided q, wider tables: the same numbers, the same bits."""
     a = Setup([100, 37, 260], [2, 1, 5], seed=18)
