@@ -25,7 +25,7 @@
 // What bounds it: 64 sequences of 97 to 8191 keys of 8 heads of 128, one token of 32 heads each, 554 MB,
 // take 113 us (84 at the measured copy rate), one of 131071 keys 63 us (41): about 6.5 TB/s and some
 // 15 us that do not depend on the length (the table's and the first page's latency, the merge).  5 tokens
-// of 32 heads, 20 rows, take 74 us for 153 MB: the products' instructions and the softmax of 24 rows.
+// of 32 heads, 20 rows, take 71 us for 153 MB: the products' instructions and the softmax of 24 rows.
 // 777 keys take 12.6 us, two kernels of some 7 us that are chains of latencies.  One sequence's tables
 // were looked up by each run before (142 us for the first of these), rows as M (171 us).
 #include <algorithm>
@@ -482,7 +482,6 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
         for (int e = 0; e < 4; ++e) t[x][e] = fmaf(sacc[x][0][e] + sacc[x][1][e], mul[e & 1], sc.add);
       }
       const int key0 = first_key + i * kTile;
-      const bool ragged = key0 + kRun > w.q.len || sc.page < 0;
       const bool masked = key0 + kRun > all_see || sc.page < 0;
       if (masked) {
 #pragma unroll
@@ -546,15 +545,15 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
           const uint2 v = lds64(vb + key * D + ((r >> 1) ^ ((key >> 1) & 3)) * 16 + (r & 1) * 8);
           vw[k][0] = v.x, vw[k][1] = v.y;
         }
-        if (ragged && (sc.page < 0 || key0 + key >= w.q.len)) {  // a page's tail holds anything
+      }
+      if (masked) {
 #pragma unroll
-          for (int j = 0; j < D / 32; ++j) vw[k][j] = 0;
-        }
-        if (masked) {
+        for (int k = 0; k < 4; ++k) {  // a page's tail holds anything
+          const bool there = sc.page >= 0 && key0 + 2 * cq + (k & 1) + 8 * (k >> 1) < w.q.len;
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
-            const uint32_t n = nan_bytes(vw[k][j]);
-            vw[k][j] &= ~n;
+            const uint32_t v = there ? vw[k][j] : 0, n = nan_bytes(v);
+            vw[k][j] = v & ~n;
             nans |= n;
           }
         }
