@@ -143,8 +143,8 @@ def cache_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale
 
     Scales are powers of two, the least that hold a page's largest magnitude (448 * scale).  A page
     that held earlier tokens keeps them: its scale only grows, and where it does they are rounded
-    to the new step.  Values that are not finite are stored as NaN.  Two sequences must not append
-    to one page in one call.  Pages, lengths, offsets and positions live on the device and are
+    to the new step.  Values that are not finite are stored as NaN.  A call must not append to
+    one page twice (two sequences, or two entries of the table).  Pages, lengths, offsets and positions live on the device and are
     checked there: what is out of range is skipped and reported by ``last_device_error`` as (1, bits).
     """
     _require_ext()

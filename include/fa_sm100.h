@@ -175,15 +175,17 @@ typedef struct fa_append {
 /* Writes T new tokens (fp16 or bf16) into their pages.  A page whose first new token is not its
  * first slot keeps its earlier rows: its scale only grows, and where it does they are rounded to
  * the new step; rows behind the last token stay as they are.  Stored values are the rotated ones
- * rounded once, to nearest even; values that are not finite are stored as NaN.  Two sequences must
- * not append to one page in one call.  q_out must not overlap q. */
+ * rounded once, to nearest even; values that are not finite are stored as NaN.  A call must not
+ * append to one page twice, by two sequences or two entries of the table: what that page then holds
+ * is undefined.  q_out must not overlap q. */
 int fa_cache_append(int dtype, const fa_cache_t* cache, const fa_append_t* p, int T,
                     cudaStream_t stream);
 
 /* Attention of T new query rows q [T, H, D] (fp16 or bf16, H % Hkv == 0, element strides of
  * (token, head)) over the cache; o [T, H, D] (contiguous, q's type) and lse [T, H] (fp32, natural
  * log) are written.  causal: a query sees the keys up to its own position; else all of its
- * sequence's.  A query without a key gets o = 0, lse = +inf.  `workspace` (16-byte aligned) holds
+ * sequence's.  A query without a key gets o = 0, lse = +inf; a key or value that is NaN reaches the
+ * queries that see it and no others.  `workspace` (16-byte aligned) holds
  * fa_cache_attention_workspace_bytes(cache, H, T) bytes, belongs to this call until it has run, and
  * needs no initial value. */
 size_t fa_cache_attention_workspace_bytes(const fa_cache_t* cache, int H, int T);
