@@ -9,7 +9,6 @@ table [S, max_pages], and the lengths after the step.  Each sequence's new token
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -24,7 +23,6 @@ _E4M3_MAX = 448.0
 _MIN_EXP, _MAX_EXP = -64, 120
 
 
-@functools.cache
 def _fused_attn():
     package = str(Path(__file__).resolve().parents[1] / "fused-attention-cuda_b200")
     if package not in sys.path:
