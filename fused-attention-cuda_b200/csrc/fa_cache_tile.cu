@@ -110,28 +110,29 @@ __device__ __forceinline__ long long sum_floors(unsigned n, unsigned m, unsigned
   }
 }
 
-// The tiles of one (sequence, kv head).  Tile j's last row is a query that sees
-//   past + floor((256 j + 255) / group) + 1
-// keys (causal), so it has floor((2 j + base) / group) units, base = floor((255 + group (past + 128))
-// / 128), and the units in front of tile j have a closed form.  The last tile ends with the last row.
+// The tiles of one (sequence, kv head).  With past = len - n, which is negative where queries lie in front
+// of the keys, tile j's last row is a query that sees past + floor((256 j + 255) / group) + 1 keys (causal),
+// so the tile has max(1, floor((2 j + base) / group)) units, base = floor((255 + group (past + 128)) / 128):
+// one in each of the first `flat` tiles, and behind them a sum with a closed form.  The last tile ends
+// with the last row, which sees every key; no tile has more units than the keys make.
 struct SeqTiles {
   SeqInfo q;
   int rows, tiles;
   bool causal;
-  int full;        // not causal: units of each tile
-  int last;        // units of the last tile
-  long long base;  // causal, see above
+  int full;        // units of the last tile; not causal: of each
+  int flat;        // causal: tiles in front that see at most one unit's keys ...
+  long long base;  // ... see above
   long long units;  // of one kv head
 
   __device__ long long before(int j, int group) const {
     if (!causal) return static_cast<long long>(j) * full;
-    if (j <= 0) return 0;
-    const long long whole = base / group;
-    return whole * j + sum_floors(j, group, static_cast<unsigned>(base - whole * group));
+    if (j <= flat) return j;
+    const long long at = base + 2ll * flat, whole = at / group;
+    return flat + whole * (j - flat) + sum_floors(j - flat, group, static_cast<unsigned>(at - whole * group));
   }
   __device__ int of(int j, int group) const {
-    if (j == tiles - 1) return last;
-    return causal ? static_cast<int>((2ll * j + base) / group) : full;
+    if (j == tiles - 1 || !causal) return full;
+    return j < flat ? 1 : static_cast<int>((2ll * j + base) / group);
   }
 };
 
@@ -142,17 +143,16 @@ __device__ __forceinline__ SeqTiles tiles_of(const SeqInfo& q, int group, bool c
   t.rows = q.n * group;
   t.tiles = (t.rows + kRows - 1) / kRows;
   t.full = max(1, (q.len + kKeys - 1) / kKeys);
-  t.last = t.full;
+  t.flat = 0;
   t.base = 0;
   t.units = 0;
   if (t.tiles == 0) return t;
   if (causal) {
-    // Queries in front of the cache count as if they saw their own keys: a few units too many.
-    const long long past = max(0, q.len - q.n);
-    t.base = (255 + group * (past + kKeys)) / kKeys;
-    t.last = static_cast<int>((t.rows - 1 + group * (past + kKeys)) / (static_cast<long long>(kKeys) * group));
+    t.base = (255 + group * (static_cast<long long>(q.len) - q.n + kKeys)) >> 7;
+    static_assert(kKeys == 1 << 7, "floors of negative numbers by shifts");
+    t.flat = static_cast<int>(min(static_cast<long long>(t.tiles), max(0ll, (group - t.base + 1) >> 1)));
   }
-  t.units = t.before(t.tiles - 1, group) + t.last;
+  t.units = t.before(t.tiles - 1, group) + t.full;
   return t;
 }
 
@@ -1109,7 +1109,7 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   fa_cache_tile_kernel<T, D><<<ctas, kThreads, L::kBytes, stream>>>(a, partials);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  if (units == 1) return cudaSuccess;  // no tile has two units
+  if (units == 1) return cudaSuccess;  // no tile has two units: none has more than its sequence's keys
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas, kMergeBlocks);
   cfg.blockDim = dim3(kMergeThreads);

@@ -1,0 +1,68 @@
+"""The paged 8-bit cache at the ends of what its documents allow, against the 64-bit oracle (oracle/cache.py)."""
+
+from __future__ import annotations
+
+import math
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+import fused_attn
+from fused_attn import abi
+from oracle import cache as ref
+from test_cache_gpu import E4M3, Setup, check_append, check_attention, narrow, same_pages
+
+pytestmark = pytest.mark.gpu
+
+BAD_INDEX = (1, 1 << 11)
+
+
+@pytest.fixture(autouse=True)
+def _available():
+    if not fused_attn.is_available() or not fused_attn.impl_supports(5, torch.float16, 128):
+        pytest.skip("kernels not available")
+    fused_attn.last_device_error()
+    yield
+
+
+def attend_into_nan(s: Setup, causal=True):
+    """The C entry point on outputs and a workspace that hold NaN: what is not written shows."""
+    P, Hkv, page, D = s.k_cache.shape
+    strides = [tuple(c.stride(i) for i in range(3)) for c in (s.k_cache, s.v_cache)]
+    c = abi.FaCache(s.k_cache.data_ptr(), s.v_cache.data_ptr(), s.k_scale.data_ptr(), s.v_scale.data_ptr(), P, page,
+                    Hkv, D, *strides, s.table_d.data_ptr(), s.table_d.stride(0), s.table_d.shape[1],
+                    s.lens_d.data_ptr(), s.cu_d.data_ptr(), len(s.lens))
+    T = s.q.shape[0]
+    o = torch.full((T, s.H, D), math.nan, dtype=s.dtype, device="cuda")
+    lse = torch.full((T, s.H), math.nan, device="cuda")
+    ws = torch.full((abi.cache_attention_workspace_bytes(c, s.H, T),), 0xFF, dtype=torch.uint8, device="cuda")
+    err = abi.cache_attention(abi.dtype_code(s.dtype), c, s.q.data_ptr(), (s.q.stride(0), s.q.stride(1)), o.data_ptr(),
+                              lse.data_ptr(), ws.data_ptr(), T, s.H, 1 / math.sqrt(D), causal,
+                              torch.cuda.current_stream().cuda_stream)
+    assert err == 0
+    torch.cuda.synchronize()
+    return o, lse
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("H,Hkv,D,page,lens,new", [
+    (8, 2, 128, 64, [64], [300]), (1, 1, 64, 128, [128], [1000]), (1, 1, 64, 128, [100], [300]),
+    (6, 2, 64, 16, [16, 3, 0], [500, 90, 200]), (7, 1, 128, 32, [129, 250], [300, 250]), (300, 1, 64, 16, [5], [9])],
+    ids=str)
+def test_more_queries_than_keys(H, Hkv, D, page, lens, new, causal):
+    """Many new tokens over a table with room for few keys: every row is written, those in front of the keys too."""
+    s = Setup(lens, new, H=H, Hkv=Hkv, D=D, page=page, seed=61)
+    o, lse = attend_into_nan(s, causal)
+    check_attention(s, causal, o=o, lse=lse)
+
+
+def test_a_length_above_the_tables_room_with_many_rows():
+    """It counts as the room, and every row is written."""
+    s = Setup([64, 40], [300, 30], H=4, Hkv=1, D=64, page=64, seed=62)
+    s.lens_d[0] = 10**6
+    o, lse = attend_into_nan(s)
+    assert fused_attn.last_device_error() == BAD_INDEX
+    check_attention(s, o=o, lse=lse)
