@@ -9,7 +9,10 @@
 //   O = sum_j P_j vq_j / l,   l = sum_j P_j / sv_j,   LSE = (m + log2 l) ln 2.
 // Folding V's scale into the exponent keeps P in 16 bits' range whatever the scales are, leaves the
 // products to plain e4m3 values (exact in fp16, so one fp16 product form serves fp16 and bf16
-// queries), and costs one term for a run of 16 keys, since a run never leaves its page.
+// queries), and costs one term for a run of 16 keys, since a run never leaves its page.  In return P is
+// rounded relative to the row's largest P sv: 11 bits down to 2^-14 of it, and below 2^-25 of it a key is
+// in the denominator alone.  The denominator is a sum in 32 bits; P has to stay above 2^-126 for it, so
+// value scales have a range (value_scale) and those of one sequence lie within 2^96 of each other.
 //
 // bf16 queries enter the products as fp16 after division by a power of two for each row: 8
 // significant bits fit in fp16's 11, so this is exact but for values 2^-23 below the row's largest.
@@ -220,16 +223,6 @@ struct RunScale {
   int page;  // -1: the run's keys count as absent
 };
 
-// A page's value scale as (log2, reciprocal); exact for powers of two.  Scales are positive; zero
-// and subnormal ones count as 2^-64, which leaves the keys in the denominator and adds nothing.
-__device__ __forceinline__ void value_scale(float s, float* add, float* inv) {
-  s = s != s ? s : fminf(fmaxf(s, 0x1p-64f), 0x1p120f);
-  const int bits = __float_as_int(s);
-  const float mant = __int_as_float((bits & 0x7fffff) | 0x3f800000);
-  *add = static_cast<float>((bits >> 23) - 127) + log2f(mant);
-  *inv = 1.0f / s;
-}
-
 // Copies 16 keys of a page and head to shared memory, 128- or 64-byte swizzled (a row's 16-byte piece
 // p lies at p ^ (row & 7), or p ^ ((row >> 1) & 3) for rows of 64 bytes).
 __device__ __forceinline__ void load_page(uint32_t dst, const void* map, int pos, int slot, int head,
@@ -334,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
     auto write_table = [&](int i) {
       RunScale sc;
       sc.mul = sk;
-      value_scale(sv, &sc.add, &sc.inv);
+      value_scale(c, sv, &sc.add, &sc.inv);
       sc.page = page;
       table[i & 63] = sc;
       __syncwarp();

@@ -381,14 +381,6 @@ __device__ __forceinline__ void store_wide(uint32_t lo, uint32_t hi, uint4 v) {
   sts128(hi, make_uint4(c.x, c.y, d.x, d.y));
 }
 
-__device__ __forceinline__ void value_scale(float s, float* add, float* inv) {
-  s = s != s ? s : fminf(fmaxf(s, 0x1p-64f), 0x1p120f);
-  const int bits = __float_as_int(s);
-  const float mant = __int_as_float((bits & 0x7fffff) | 0x3f800000);
-  *add = static_cast<float>((bits >> 23) - 127) + log2f(mant);
-  *inv = 1.0f / s;
-}
-
 // True in one lane of the (converged) warp, always the same.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -890,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
             const int slot = key_at(i) & ((1 << c.page_shift) - 1);
             sc.page = next_page;
             sc.mul = sk;
-            value_scale(sv, &sc.add, &sc.inv);
+            value_scale(c, sv, &sc.add, &sc.inv);
             sc.k_at = next_page * c.ks[0] + head * c.ks[1] + slot * c.ks[2];
             sc.v_at = next_page * c.vs[0] + head * c.vs[1] + slot * c.vs[2];
             next_page = page_at(i + 4);

@@ -64,7 +64,7 @@ enum StatusBits : unsigned int {
   kStSFree = 1u << 8,    // MMA warp waiting for the softmax warps to read S (lookahead kernel)
   kStPFree = 1u << 9,    // softmax warps waiting for a PV to release P (lookahead kernel)
   kStBounds = 1u << 10,  // FA_DEBUG_CHECKS builds: an index or address check failed
-  kStCacheIndex = 1u << 11,  // paged cache: a page, length, offset or position out of range
+  kStCacheIndex = 1u << 11,  // paged cache: a page, length, offset, position or value scale out of range
 };
 
 }  // namespace fa_sm100

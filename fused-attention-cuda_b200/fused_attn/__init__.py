@@ -163,7 +163,11 @@ def cache_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor
     for each sequence is a decoding step, a whole prompt or a chunk of one a prefill step; a batch
     may mix them.  Returns ``o`` [T, H, D], or ``(o, lse)`` with lse float32 [T, H]; a query
     without a key gets o = 0 and lse = +inf, rows behind the last sequence are zero.  As
-    [T, H, 1, D] and [T, H, 1], (o, lse) is a partial for ``combine``."""
+    [T, H, 1, D] and [T, H, 1], (o, lse) is a partial for ``combine``.
+
+    ``k_scale`` is positive and finite; ``v_scale`` lies in [2^-64, 2^120], which ``cache_append`` keeps
+    to, and within 2^96 from page to page of a sequence.  A value scale outside counts as the nearest
+    end and is reported by ``last_device_error`` as (1, bits)."""
     _require_ext()
     o, lse = torch.ops.fused_attn.cache_attention(q, k_cache, v_cache, k_scale, v_scale,
                                                   block_table, seq_lens, cu_seqlens,

@@ -120,8 +120,10 @@ size_t fa_noalloc_scratch_bytes(void);
  * Keys and values live in num_pages pages of page_size tokens (16, 32, 64 or 128) each, for every
  * kv head D e4m3 values a token; k_scale / v_scale [num_pages, Hkv] (fp32, contiguous) hold one
  * scale for each page and kv head, value = e4m3 * scale.  fa_cache_append writes powers of two in
- * [2^-64, 2^120]; fa_cache_attention takes any positive finite scale.  k_strides / v_strides are
- * the byte strides of (page, kv head, token), positive multiples of 16; d is contiguous.
+ * [2^-64, 2^120].  fa_cache_attention takes any positive finite k_scale, and any v_scale in that
+ * range; the value scales of one sequence and kv head lie within 2^96 of each other.  A value scale
+ * outside of [2^-64, 2^120] counts as the nearest end and is reported like a bad page.   k_strides /
+ * v_strides are the byte strides of (page, kv head, token), positive multiples of 16; d is contiguous.
  *
  * block_table [n_seqs, max_pages] (rows table_stride apart) lists each sequence's pages in order,
  * seq_lens [n_seqs] the keys that each holds, those of the current call included.  The current
@@ -185,7 +187,9 @@ int fa_cache_append(int dtype, const fa_cache_t* cache, const fa_append_t* p, in
  * (token, head)) over the cache; o [T, H, D] (contiguous, q's type) and lse [T, H] (fp32, natural
  * log) are written.  causal: a query sees the keys up to its own position; else all of its
  * sequence's.  A query without a key gets o = 0, lse = +inf; a key or value that is NaN reaches the
- * queries that see it and no others.  `workspace` (16-byte aligned) holds
+ * queries that see it and no others.  The weights that multiply the values are held in fp16, scaled so that
+ * the largest weight times value scale of a query is about 1: a key whose page has a value scale 2^-20 of
+ * the largest one counts with 4 bits in o, and below 2^-25 not at all (lse has all of them).  `workspace` (16-byte aligned) holds
  * fa_cache_attention_workspace_bytes(cache, H, T) bytes, belongs to this call until it has run, and
  * needs no initial value. */
 size_t fa_cache_attention_workspace_bytes(const fa_cache_t* cache, int H, int T);

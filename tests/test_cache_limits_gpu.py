@@ -66,3 +66,42 @@ def test_a_length_above_the_tables_room_with_many_rows():
     o, lse = attend_into_nan(s)
     assert fused_attn.last_device_error() == BAD_INDEX
     check_attention(s, o=o, lse=lse)
+
+
+@pytest.mark.parametrize("new", [1, 40], ids=["token", "rows"])
+@pytest.mark.parametrize("low,high", [(-64, -64), (120, 120), (-64, 32), (24, 120)])
+def test_value_scales_at_the_ends_of_their_range(low, high, new):
+    """2^-64 and 2^120, alone and in one sequence with scales 2^96 away.
+
+    The room grows with the scales' exponents: a score in units of log2 holds the exponent e, so it and the logarithm
+    of the sum are rounded to half a step below 2^7, 2^-18 each, and P with them: 2^-17 of what P's own rounding to
+    fp16, 2^-11, is in the oracle's room.  (The spread of 2^96 leaves 2^30 of the exponent's range for the scores.)"""
+    s = Setup([200, 90], [new, new], seed=63)
+    for at in range(s.P):
+        s.v_scale[at] = 2.0 ** (high if at % 2 else low)
+    o, lse = s.attend()
+    want = ref.attention(s.pages(), s.q, s.table.tolist(), s.lens, s.cu)
+    half = torch.finfo(s.dtype).eps / 2
+    room = want.o_room * (1 + 2.0**-6) * (1 + half) + want.o.abs() * half
+    assert bool(((o.cpu().double() - want.o).abs() <= room).all())
+    assert bool(((lse.cpu().double() - want.lse).abs() <= want.lse_room + 2.0**-17).all())
+    assert fused_attn.last_device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("new", [1, 40], ids=["token", "rows"])
+@pytest.mark.parametrize("scale,end", [(1e-20, 2.0**-64), (0.0, 2.0**-64), (-1.0, 2.0**-64), (2.0**-140, 2.0**-64),
+                                       (2.0**121, 2.0**120), (math.inf, 2.0**120)])
+def test_value_scales_outside_their_range_are_reported(scale, end, new):
+    """They count as the nearest end, and the status says so."""
+    s = Setup([70, 90], [new, new], seed=64)
+    s.v_scale[s.table[0, 1].item()] = end
+    want = s.attend()
+    assert fused_attn.last_device_error() == (0, 0)
+    s.v_scale[s.table[0, 1].item()] = scale
+    got = s.attend()
+    assert fused_attn.last_device_error() == BAD_INDEX
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    s.v_scale[s.table[0, 1].item()] = end
+    s.v_scale[[p for p in range(s.P) if p not in s.table.flatten().tolist()]] = scale  # a page that nobody has
+    s.attend()
+    assert fused_attn.last_device_error() == (0, 0)
