@@ -105,6 +105,8 @@ __device__ __forceinline__ int page_of(const CacheView& c, int s, int i) {
 // A page's value scale as (log2, reciprocal); exact for powers of two.  P / scale is summed, P at most
 // 2^8 and its exponent's range 2^-126, so the scales need a range of their own for the denominator to
 // hold: what lies outside of it (zero and what is negative, too) is reported and counts as its nearest end.
+// A scale that is NaN makes the scores of the rows that see its page NaN, by way of `add`; `inv` also meets
+// the zero weights of rows that do not, so it stays finite.
 constexpr float kMinValueScale = 0x1p-64f, kMaxValueScale = 0x1p120f;  // what cache_append writes
 __device__ __forceinline__ void value_scale(const CacheView& c, float s, float* add, float* inv) {
   const float in = fminf(fmaxf(s, kMinValueScale), kMaxValueScale);
@@ -112,7 +114,7 @@ __device__ __forceinline__ void value_scale(const CacheView& c, float s, float* 
   const int bits = __float_as_int(in);
   const float mant = __int_as_float((bits & 0x7fffff) | 0x3f800000);
   *add = s != s ? s : static_cast<float>((bits >> 23) - 127) + log2f(mant);
-  *inv = s != s ? s : 1.0f / in;
+  *inv = s != s ? 1.f : 1.0f / in;
 }
 
 // A key that some rows of a tile see and others do not has weight 0 in the latter, but 0 times NaN is

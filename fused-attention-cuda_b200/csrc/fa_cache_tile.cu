@@ -51,6 +51,7 @@ constexpr int kGroups = kKeys / 16;
 constexpr int kTables = 8;   // scale tables in flight: more than the tiles between load and softmax
 constexpr int kPairBarrier = 1;  // named barrier of the two softmax groups
 constexpr float kLazy = 8.0f;
+constexpr float kSmallest = 1.1754944e-38f;  // a factor that -inf times is -inf
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -381,6 +382,13 @@ __device__ __forceinline__ void store_wide(uint32_t lo, uint32_t hi, uint4 v) {
   sts128(hi, make_uint4(c.x, c.y, d.x, d.y));
 }
 
+// The larger one, NaN where one is NaN.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // True in one lane of the (converged) warp, always the same.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -556,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
 #pragma unroll
           for (int x = 0; x < kGroups / 2; ++x) {
             const float4 sc = *reinterpret_cast<const float4*>(&table[x]);
-            mul[x] = fmaxf(sc.x * row_mul, 1.1754944e-38f);
+            mul[x] = fmax_nan(sc.x * row_mul, kSmallest);
             add[x] = sc.y;
             inv[x] = sc.z;
           }
@@ -574,6 +582,10 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
 #pragma unroll
           for (int x = 0; x < kGroups / 2; ++x) {
             const int lx = table[x].page < 0 ? 0 : lim;
+            if (16 * x >= lx) {  // the page's scales are not this row's, and may be NaN
+              mul[x] = kSmallest;
+              add[x] = 0.f;
+            }
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               if (16 * x + j >= lx) u[16 * x + j] = 0xff800000u;  // -inf

@@ -122,8 +122,9 @@ size_t fa_noalloc_scratch_bytes(void);
  * scale for each page and kv head, value = e4m3 * scale.  fa_cache_append writes powers of two in
  * [2^-64, 2^120].  fa_cache_attention takes any positive finite k_scale, and any v_scale in that
  * range; the value scales of one sequence and kv head lie within 2^96 of each other.  A value scale
- * outside of [2^-64, 2^120] counts as the nearest end and is reported like a bad page.   k_strides /
- * v_strides are the byte strides of (page, kv head, token), positive multiples of 16; d is contiguous.
+ * outside of [2^-64, 2^120] counts as the nearest end and is reported like a bad page.  A scale that is NaN
+ * makes o and lse of the queries that see a key of its page NaN, and of no others.  k_strides / v_strides
+ * are the byte strides of (page, kv head, token), positive multiples of 16; d is contiguous.
  *
  * block_table [n_seqs, max_pages] (rows table_stride apart) lists each sequence's pages in order,
  * seq_lens [n_seqs] the keys that each holds, those of the current call included.  The current

@@ -105,3 +105,26 @@ def test_value_scales_outside_their_range_are_reported(scale, end, new):
     s.v_scale[[p for p in range(s.P) if p not in s.table.flatten().tolist()]] = scale  # a page that nobody has
     s.attend()
     assert fused_attn.last_device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("lens,new,page,at", [([50, 40], [1, 1], 16, 1), ([50, 40], [20, 3], 16, 2),
+                                              ([50, 40], [8, 3], 16, 3), ([100, 90], [60, 40], 16, 5),
+                                              ([100, 90], [60, 40], 16, 6), ([700, 64], [300, 40], 128, 4)], ids=str)
+def test_a_scale_that_is_nan_reaches_the_rows_that_see_its_page(lens, new, page, at, which, D):
+    s = Setup(lens, new, page=page, D=D, seed=65)
+    want = ref.attention(s.pages(), s.q, s.table.tolist(), s.lens, s.cu)
+    (s.k_scale if which == "k" else s.v_scale)[s.table[0, at].item(), 1] = math.nan
+    o, lse = s.attend()
+    sees = torch.zeros(sum(new), s.H, dtype=torch.bool)
+    for i in range(new[0]):
+        sees[i, s.H // 2:] = lens[0] - new[0] + i >= at * page
+    o, lse = o.cpu().double(), lse.cpu().double()
+    assert torch.equal(torch.isnan(lse), sees)
+    assert torch.equal(torch.isnan(o), sees[..., None].expand_as(o))
+    half = torch.finfo(s.dtype).eps / 2
+    room = want.o_room * (1 + half) + want.o.abs() * half
+    assert bool(((lse - want.lse).abs() <= want.lse_room)[~sees].all())
+    assert bool(((o - want.o).abs() <= room)[~sees].all())
+    assert fused_attn.last_device_error() == (0, 0)
