@@ -318,7 +318,8 @@ __device__ __forceinline__ void fill_page(const AppendArgs& p, const Grid& g, in
     s = find_item_seq(c, item, lane);
     first = item_base(c, s);
   }
-  const SeqInfo q = seq_info(c, s);
+  // Of a length past the table's room the tokens that have a page are stored where they belong.
+  const SeqInfo q = seq_info<true>(c, s);
   int begin = q.len - q.n;  // position of the first new token
   int t0 = q.t0;
   if (begin < 0) {  // tokens in front of the cache are not stored
@@ -561,7 +562,7 @@ __device__ __forceinline__ void rotate_q(const AppendArgs& p, const Grid& g, lon
   }
   if (t >= c.T) return;
   if (t < live && s < c.n_seqs) {
-    const SeqInfo q = seq_info(c, s);
+    const SeqInfo q = seq_info<true>(c, s);
     pos = t >= q.t0 && t < q.t0 + q.n ? q.len - q.n + t - q.t0 : -1;
     if (pos < 0 || pos >= p.table_rows) {
       report_cache_index(c);

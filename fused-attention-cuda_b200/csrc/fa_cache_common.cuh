@@ -14,7 +14,7 @@ namespace fa_sm100 {
 struct SeqInfo {
   int t0;    // first packed row
   int n;     // new tokens
-  int len;   // keys held, this call's included
+  int len;   // keys held, this call's included; no more than the table has room for, or as it was given
 };
 
 __device__ __forceinline__ void report_cache_index(const CacheView& c) {
@@ -26,6 +26,9 @@ __device__ __forceinline__ bool offsets_ok(const CacheView& c, int s, int t0, in
   return t0 >= 0 && end >= t0 && end <= c.T && (s > 0 || t0 == 0);
 }
 
+// What a length above the table's room means: the room (KEEP_LONG false), or that the sequence's last tokens
+// have no page, which is for the caller to see.
+template <bool KEEP_LONG = false>
 __device__ __forceinline__ SeqInfo seq_info(const CacheView& c, int s) {
   SeqInfo q;
   int len = c.seq_lens[s];
@@ -46,7 +49,7 @@ __device__ __forceinline__ SeqInfo seq_info(const CacheView& c, int s) {
   const long long room = static_cast<long long>(c.max_pages) << c.page_shift;
   if (len < 0 || len > room) {
     report_cache_index(c);
-    len = len < 0 ? 0 : static_cast<int>(room);
+    len = len < 0 ? 0 : KEEP_LONG ? len : static_cast<int>(room);
   }
   q.len = len;
   return q;

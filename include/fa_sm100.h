@@ -131,7 +131,9 @@ size_t fa_noalloc_scratch_bytes(void);
  * call's T packed tokens are split by cu_seqlens [n_seqs + 1] (NULL: T / n_seqs each) and are the
  * last ones of their sequences: new token i of n sits at position len - n + i.  These arrays live
  * in device memory and are checked there: a page, length, offset or position out of range is
- * skipped and reported by fa_last_device_error (cudaErrorInvalidValue), never followed.  Entries
+ * skipped and reported by fa_last_device_error (cudaErrorInvalidValue), never followed.  Of a length
+ * above max_pages * page_size fa_cache_append skips the tokens that have no place in the table, and
+ * fa_cache_attention sees the keys that the table has room for; a length below 0 counts as 0.  Entries
  * of block_table behind a sequence's last page are not read.  cu_seqlens begins with 0.  Rows of the
  * packed tensors that belong to no sequence -- behind cu_seqlens[n_seqs], or of a sequence whose
  * offsets are out of order -- store nothing, and outputs get zeros there. */

@@ -128,3 +128,18 @@ def test_a_scale_that_is_nan_reaches_the_rows_that_see_its_page(lens, new, page,
     assert bool(((lse - want.lse).abs() <= want.lse_room)[~sees].all())
     assert bool(((o - want.o).abs() <= room)[~sees].all())
     assert fused_attn.last_device_error() == (0, 0)
+
+
+@pytest.mark.parametrize("n", [1, 3, 40], ids=["token", "draft", "rows"])
+@pytest.mark.parametrize("over", [1, 2, 25, 10**6])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("rot", [None, 128], ids=["plain", "turned"])
+def test_tokens_past_the_table_are_not_stored(n, over, page, rot):
+    """A sequence that outgrows its table: the tokens that fit are stored, no row that was there changes, and the
+    status says so."""
+    s = Setup([128, 70], [n, 3], page=page, seed=66, rot=rot)
+    s.lens[0] += over
+    s.lens_d[0] += over
+    if rot and over < 100:  # angles for all of the positions
+        s.cos, s.sin = (torch.cat([t, t.flip(0)[:over]]) for t in (s.cos, s.sin))
+    check_append(s, errors=BAD_INDEX)
