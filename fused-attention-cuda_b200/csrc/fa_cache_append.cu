@@ -254,14 +254,15 @@ __device__ __forceinline__ void widen(const Raw& r, float (&x)[8], float (&y)[8]
   }
 }
 
-// The sequence of packed row t (t below live_rows): the last s with cu_seqlens[s] <= t.  Each round
-// the warp probes 32 places of the range that is left.
+// The sequence of packed row t, if it is one's: the last s with cu_seqlens[s] <= t.  Each round the warp
+// probes 32 places of the range that is left.  Compared without signs, so that a negative offset is not
+// below: an offset out of range then costs the sequences that it bounds and, among up to 32, no other.
 __device__ __forceinline__ int find_seq(const int* starts, int n, int t, int lane) {
   int lo = 0;
   while (n > 1) {
     const int step = (n + 31) / 32;
     const int at = lane * step;
-    const bool below = at < n && starts[lo + at] <= t;
+    const bool below = at < n && static_cast<unsigned>(starts[lo + at]) <= static_cast<unsigned>(t);
     const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
     lo += last * step;
     n = min(step, n - last * step);
@@ -275,13 +276,14 @@ __device__ __forceinline__ int item_base(const CacheView& c, int s) {
   return (c.cu_seqlens[s] >> c.page_shift) + 2 * s;
 }
 
-// The sequence of page item i: the last s with item_base(s) <= i.
+// The sequence of page item i: the last s with item_base(s) <= i, of those that begin in the batch (find_seq).
 __device__ __forceinline__ int find_item_seq(const CacheView& c, int i, int lane) {
   int lo = 0, n = c.n_seqs;
   while (n > 1) {
     const int step = (n + 31) / 32;
     const int at = lane * step;
-    const bool below = at < n && item_base(c, lo + at) <= i;
+    const bool below = at < n && static_cast<unsigned>(c.cu_seqlens[lo + at]) <= static_cast<unsigned>(c.T) &&
+                       item_base(c, lo + at) <= i;
     const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
     lo += last * step;
     n = min(step, n - last * step);
@@ -549,24 +551,29 @@ __device__ __forceinline__ void rotate_q(const AppendArgs& p, const Grid& g, lon
   for (int i = 0; i < kAhead; ++i) {
     if (h0 + i < h1) ring[i] = load_unit<T>(src + (h0 + i) * p.sq[1], u);
   }
-  const int live = live_rows(c);
   int pos = -1;
   // The lanes of a warp hold up to 32 / kLanes rows: find the first one's sequence, then step on.
   const int t_first = __shfl_sync(0xffffffffu, t, 0);
   int s = 0;
   if (c.cu_seqlens == nullptr) {
     s = t / max(1, c.T / c.n_seqs);
-  } else if (t_first < live) {
+  } else if (t_first < c.T) {
     s = find_seq(c.cu_seqlens, c.n_seqs, t_first, lane);
-    while (t < live && s + 1 < c.n_seqs && c.cu_seqlens[s + 1] <= t) ++s;
+    for (int next = s + 1; next < c.n_seqs; ++next) {
+      const int start = c.cu_seqlens[next];
+      if (start > t && start <= c.T) break;
+      if (start >= 0 && start <= t) s = next;
+    }
   }
   if (t >= c.T) return;
-  if (t < live && s < c.n_seqs) {
+  if (s < c.n_seqs) {
     const SeqInfo q = seq_info<true>(c, s);
-    pos = t >= q.t0 && t < q.t0 + q.n ? q.len - q.n + t - q.t0 : -1;
-    if (pos < 0 || pos >= p.table_rows) {
-      report_cache_index(c);
-      pos = -1;
+    if (t >= q.t0 && t < q.t0 + q.n) {  // else a row of no sequence
+      pos = q.len - q.n + t - q.t0;
+      if (pos < 0 || pos >= p.table_rows) {
+        report_cache_index(c);
+        pos = -1;
+      }
     }
   }
   Angles an;
@@ -608,6 +615,11 @@ __device__ __forceinline__ void fill_block(const AppendArgs& p, const Grid& g, i
   fill_page<T, D, ITEM_WARPS, ROTATES>(p, g, active ? static_cast<int>(item) : 0,
                                        static_cast<int>(id - item * jobs), active,
                                        threadIdx.x % (32 * ITEM_WARPS), red + sub * ITEM_WARPS);
+  if (block == 0 && p.c.cu_seqlens != nullptr) {  // offsets that are out of order may hide each other from the items
+    for (int s = threadIdx.x; s < p.c.n_seqs; s += kThreads) {
+      if (!offsets_ok(p.c, s, p.c.cu_seqlens[s], p.c.cu_seqlens[s + 1])) report_cache_index(p.c);
+    }
+  }
 }
 template <typename T, int D>
 __device__ __forceinline__ void rotate_block(const AppendArgs& p, const Grid& g, int block) {

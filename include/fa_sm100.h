@@ -136,7 +136,10 @@ size_t fa_noalloc_scratch_bytes(void);
  * fa_cache_attention sees the keys that the table has room for; a length below 0 counts as 0.  Entries
  * of block_table behind a sequence's last page are not read.  cu_seqlens begins with 0.  Rows of the
  * packed tensors that belong to no sequence -- behind cu_seqlens[n_seqs], or of a sequence whose
- * offsets are out of order -- store nothing, and outputs get zeros there. */
+ * offsets are out of order -- store nothing, and outputs get zeros there.  An offset outside of [0, T] costs
+ * the two sequences that it bounds.  Where offsets descend inside of the batch, or one is bad among more than
+ * 32 sequences, fa_cache_append may leave out rows of others too, and a row that two sequences claim gets
+ * the result of either. */
 typedef struct fa_cache {
   void* k;
   void* v;

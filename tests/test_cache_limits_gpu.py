@@ -143,3 +143,50 @@ def test_tokens_past_the_table_are_not_stored(n, over, page, rot):
     if rot and over < 100:  # angles for all of the positions
         s.cos, s.sin = (torch.cat([t, t.flip(0)[:over]]) for t in (s.cos, s.sin))
     check_append(s, errors=BAD_INDEX)
+
+
+@pytest.mark.parametrize("S,at,value", [(4, 4, 2), (4, 4, 0), (4, 4, -1), (4, 4, 10**6), (4, 3, -1), (4, 3, 10**6),
+                                        (4, 2, -5), (30, 17, -1), (30, 17, 10**6), (45, 45, 3), (45, 45, -1)])
+def test_an_offset_out_of_range_costs_its_sequences_only(S, at, value):
+    """The two sequences that an offset bounds store nothing and get zeros; the others are served."""
+    new = [2 + i % 4 for i in range(S)]
+    lens = [20 + 7 * i % 50 for i in range(S)]
+    s, good = (Setup(lens, new, rot=128, seed=67) for _ in range(2))
+    want = s.pages()
+    s.cu_d[at] = value
+    q = s.append()
+    o, lse = s.attend(q=q)
+    torch.cuda.synchronize()
+    assert fused_attn.last_device_error() == BAD_INDEX
+    for i in range(S):
+        rows = slice(good.cu[i], good.cu[i + 1])
+        if i in (at - 1, at):
+            for x in (q, o, lse):
+                assert not bool(x[rows].any())
+            continue
+        q_want = ref.append(want, s.k[rows], s.v[rows], [s.table[i].tolist()], [lens[i]], [0, new[i]], q=s.q[rows],
+                            cos=s.cos, sin=s.sin)
+        assert torch.equal(q[rows].cpu(), narrow(q_want, s.dtype))
+    same_pages(s.pages(), want)
+    q_good = good.append()
+    o_good, lse_good = good.attend(q=q_good)
+    for i in range(S):
+        rows = slice(good.cu[i], good.cu[i + 1])
+        if i not in (at - 1, at):
+            assert bool(((lse[rows] - lse_good[rows]).abs() <= 1e-4).all())
+
+
+@pytest.mark.parametrize("bounds", [[0, 50, 20, 60], [0, 100, 60, 20, 100], [0, 0, 90, 89, 100], [0, 30, 30, 0, 100]])
+def test_offsets_that_descend_are_reported_by_append(bounds):
+    """Every one in the batch, but some sequences end before they begin; pages of nobody stay as they are."""
+    n = len(bounds) - 1
+    s = Setup([120] * n, [25] * n, rot=128, seed=73, spare=5)
+    assert s.q.shape[0] <= 100
+    s.cu_d.copy_(torch.tensor(bounds).clamp(max=s.q.shape[0]))
+    spare = torch.ones(s.P, dtype=torch.bool)
+    spare[s.table.flatten().long()] = False
+    before = s.k_cache.view(torch.uint8)[spare.cuda()].clone()
+    s.append()
+    torch.cuda.synchronize()
+    assert fused_attn.last_device_error() == BAD_INDEX
+    assert torch.equal(s.k_cache.view(torch.uint8)[spare.cuda()], before)
