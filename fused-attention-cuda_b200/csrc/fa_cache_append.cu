@@ -65,6 +65,12 @@ __device__ __forceinline__ float to_odd(float h, float lo, float plain) {
   return lo != 0.f && (bits & 1) == 0 ? __int_as_float(bits + toward) : h;
 }
 
+// a b rounded to odd.
+__device__ __forceinline__ float times_odd(float a, float b) {
+  const float p = a * b;
+  return to_odd(p, fmaf(a, b, -p), p);
+}
+
 __device__ __forceinline__ float finite_or_nan(float x) {
   return fabsf(x) < INFINITY ? x : __int_as_float(0x7fffffff);
 }
@@ -103,6 +109,7 @@ __device__ __forceinline__ uint2 to_e4m3x8(const float (&y)[8], float mul) {
   return r;
 }
 
+// `mul` has 24 bits where the scale was no power of two, and then a float does not hold its products.
 __device__ __forceinline__ uint32_t rescale_e4m3x4(uint32_t u, float mul) {
   uint32_t r = 0;
 #pragma unroll
@@ -110,7 +117,7 @@ __device__ __forceinline__ uint32_t rescale_e4m3x4(uint32_t u, float mul) {
     const __half2_raw raw =
         __nv_cvt_fp8x2_to_halfraw2(static_cast<unsigned short>(u >> (16 * i)), __NV_E4M3);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw));
-    r |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(f.x * mul, f.y * mul),
+    r |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(times_odd(f.x, mul), times_odd(f.y, mul)),
                                                         __NV_SATFINITE, __NV_E4M3))
          << (16 * i);
   }

@@ -190,3 +190,19 @@ def test_offsets_that_descend_are_reported_by_append(bounds):
     torch.cuda.synchronize()
     assert fused_attn.last_device_error() == BAD_INDEX
     assert torch.equal(s.k_cache.view(torch.uint8)[spare.cuda()], before)
+
+
+@pytest.mark.parametrize("scale", [17 / 18, 19 / 18, 17 / 22, 21 / 26, 0.7312847, 3.1415927, 1e-3])
+@pytest.mark.parametrize("side", [-1, 0, 1])
+def test_earlier_rows_under_a_scale_that_is_no_power_of_two_are_rounded_once(scale, side):
+    """The scale next to a ratio that takes e4m3 values to the middle of two others, from below and above: the exact
+    product of a value and such a ratio does not fit 24 bits, and its rounding to them would be a tie."""
+    near = torch.tensor([scale], dtype=torch.float32)
+    near = (near.view(torch.int32) + side).view(torch.float32).item()
+    s = Setup([15], [1], seed=68, page=16)
+    s.k_scale.fill_(near)
+    s.v_scale.fill_(near * 2.0**30)
+    for c in (s.k_cache, s.v_cache):
+        every = torch.arange(s.P * 2 * 16 * 128, device="cuda").to(torch.uint8).view(s.P, 2, 16, 128)
+        c.view(torch.uint8).copy_(every)
+    check_append(s)
