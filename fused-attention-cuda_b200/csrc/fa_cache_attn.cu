@@ -852,9 +852,15 @@ size_t workspace_d(int eights, int sms) {
 
 }  // namespace
 
+// A workspace for T rows of a batch serves every smaller T: the kernels of fewer rows have more CTAs on a
+// multiprocessor, and with D = 64 that of 9 to 16 rows needs more than that of 17 to 24.
 size_t cache_attention_workspace(int H, int Hkv, int D, int T, int n_seqs, int sms) {
   const int eights = row_eights(H, Hkv, T, n_seqs);
-  return D == 64 ? workspace_d<64>(eights, sms) : workspace_d<128>(eights, sms);
+  size_t most = eights == 0 ? cache_tile_workspace(D, sms) : 0;
+  for (int e = 1; e <= (eights == 0 ? 4 : eights); ++e) {
+    most = std::max(most, D == 64 ? workspace_d<64>(e, sms) : workspace_d<128>(e, sms));
+  }
+  return most;
 }
 
 cudaError_t launch_cache_attention(const CacheAttnArgs& a, cudaStream_t stream) {

@@ -197,7 +197,7 @@ int fa_cache_append(int dtype, const fa_cache_t* cache, const fa_append_t* p, in
  * the largest weight times value scale of a query is about 1: a key whose page has a value scale 2^-20 of
  * the largest one counts with 4 bits in o, and below 2^-25 not at all (lse has all of them).  `workspace` (16-byte aligned) holds
  * fa_cache_attention_workspace_bytes(cache, H, T) bytes, belongs to this call until it has run, and
- * needs no initial value. */
+ * needs no initial value.  With the same n_seqs, one for T serves every smaller T. */
 size_t fa_cache_attention_workspace_bytes(const fa_cache_t* cache, int H, int T);
 int fa_cache_attention(int dtype, const fa_cache_t* cache, const void* q,
                        const long long* q_strides, void* o, float* lse, void* workspace, int T,
