@@ -871,12 +871,15 @@ __global__ void __launch_bounds__(kThreads, 1) fa_cache_tile_kernel(
       unsigned n = 0;  // tiles
       bool ok = true;
       do {
-        const int keys_end = min(part.t.q.len, (part.tile0 + part.n_tiles) * kKeys);
+        const unsigned keys_end = min(part.t.q.len, (part.tile0 + part.n_tiles) * kKeys);
         const int head = part.p.head;
-        auto key_at = [&](int i) { return (part.tile0 + i + (lane >> 3)) * kKeys + 16 * x; };
+        // Unsigned: up to seven tiles ahead of a key that may be next to 2^31.
+        auto key_at = [&](int i) {
+          return static_cast<unsigned>(part.tile0 + i + (lane >> 3)) * kKeys + 16 * x;
+        };
         auto page_at = [&](int i) {
-          const int key = key_at(i);
-          return key < keys_end ? page_of(c, part.p.s, key >> c.page_shift) : -1;
+          const unsigned key = key_at(i);
+          return key < keys_end ? page_of(c, part.p.s, static_cast<int>(key >> c.page_shift)) : -1;
         };
         float sk = 0.f, sv = 1.f;
         auto read_scales = [&](int page) {

@@ -206,3 +206,22 @@ def test_earlier_rows_under_a_scale_that_is_no_power_of_two_are_rounded_once(sca
         every = torch.arange(s.P * 2 * 16 * 128, device="cuda").to(torch.uint8).view(s.P, 2, 16, 128)
         c.view(torch.uint8).copy_(every)
     check_append(s)
+
+
+@pytest.mark.parametrize("new", [1, 70], ids=["token", "rows"])
+def test_lengths_next_to_two_to_the_31(new):
+    """One page under every entry of the longest table: no index wraps or is reported."""
+    D, page = 64, 128
+    entries = (2**31 - 1 - 128) // page
+    g = torch.Generator(device="cuda").manual_seed(69)
+    k, v = (torch.randn(2, 1, page, D, generator=g, device="cuda").to(E4M3) for _ in range(2))
+    scales = [torch.ones(2, 1, device="cuda") for _ in range(2)]
+    table = torch.ones(1, entries, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([entries * page], dtype=torch.int32, device="cuda")
+    q = torch.randn(new, 1, D, generator=g, device="cuda").half()
+    o, lse = fused_attn.cache_attention(q, k, v, *scales, table, lens, is_causal=False, return_lse=True)
+    assert fused_attn.last_device_error() == (0, 0)
+    _, one_lse = fused_attn.cache_attention(q, k, v, *scales, table[:, :1], lens.clamp(max=page), is_causal=False,
+                                              return_lse=True)
+    # A CTA's thread adds up to 2^31 / 128 / 148 / 2 tiles with 8 sums each in 32 bits, half a step each: 2^18.8 2^-24.
+    assert bool(((lse - one_lse - math.log(entries)).abs() <= 2.0**-5).all()) and bool(torch.isfinite(o).all())
