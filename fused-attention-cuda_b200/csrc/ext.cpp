@@ -395,6 +395,8 @@ at::Tensor cache_append_cuda(const std::optional<at::Tensor>& q, const at::Tenso
   const fa_cache_t c = make_cache(k_cache, v_cache, k_scale, v_scale, block_table, seq_lens,
                                   cu_seqlens, T);
   const at::Device dev = k_cache.device();
+  TORCH_CHECK(c.k != c.v && c.k_scale != c.v_scale,
+              "fused_attn: k_cache and v_cache, k_scale and v_scale must be different tensors");
   fa_append_t p = {};
   check_rows(k, "k", dev, c.D, p.k_strides);
   check_rows(v, "v", dev, c.D, p.v_strides);

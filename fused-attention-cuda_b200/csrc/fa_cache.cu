@@ -186,6 +186,9 @@ extern "C" int fa_cache_append(int dtype, const fa_cache_t* c, const fa_append_t
       return fail(fn, "q and q_out must be 16-byte aligned, H > 0, strides multiples of 16 bytes");
   }
   if (const cudaError_t e = check_device()) return e;
+  if (c->k == c->v || c->k_scale == c->v_scale)
+    return fail(fn, "keys and values need pages and scales of their own");
+  if (p->q != nullptr && p->q == p->q_out) return fail(fn, "q_out must not overlap q");
   if (T == 0) return cudaSuccess;
   cudaError_t e = cudaSuccess;
   unsigned* status = status_word(&e);
@@ -234,6 +237,7 @@ extern "C" int fa_cache_attention(int dtype, const fa_cache_t* c, const void* q,
     return fail(fn, "q strides must be positive multiples of 16 bytes");
   if (const cudaError_t e = check_device()) return e;
   if (T == 0) return cudaSuccess;
+  if (o == q) return fail(fn, "o must not overlap q");
   if (workspace == nullptr || !aligned(workspace, 16))
     return fail(fn, "workspace must be non-null and 16-byte aligned");
   cudaError_t e = cudaSuccess;

@@ -185,13 +185,14 @@ typedef struct fa_append {
  * the new step; rows behind the last token stay as they are.  Stored values are the rotated ones
  * rounded once, to nearest even; values that are not finite are stored as NaN.  A call must not
  * append to one page twice, by two sequences or two entries of the table: what that page then holds
- * is undefined.  q_out must not overlap q. */
+ * is undefined.  Keys and values need pages and scales of their own, and q_out must not overlap q; what
+ * begins at the same address is refused. */
 int fa_cache_append(int dtype, const fa_cache_t* cache, const fa_append_t* p, int T,
                     cudaStream_t stream);
 
 /* Attention of T new query rows q [T, H, D] (fp16 or bf16, H % Hkv == 0, element strides of
  * (token, head)) over the cache; o [T, H, D] (contiguous, q's type) and lse [T, H] (fp32, natural
- * log) are written.  causal: a query sees the keys up to its own position; else all of its
+ * log) are written; o must not overlap q.  causal: a query sees the keys up to its own position; else all of its
  * sequence's.  A query without a key gets o = 0, lse = +inf; a key or value that is NaN reaches the
  * queries that see it and no others.  The weights that multiply the values are held in fp16, scaled so that
  * the largest weight times value scale of a query is about 1: a key whose page has a value scale 2^-20 of

@@ -28,19 +28,23 @@ def _available():
     yield
 
 
-def attend_into_nan(s: Setup, causal=True):
-    """The C entry point on outputs and a workspace that hold NaN: what is not written shows."""
+def c_cache(s: Setup) -> abi.FaCache:
     P, Hkv, page, D = s.k_cache.shape
     strides = [tuple(c.stride(i) for i in range(3)) for c in (s.k_cache, s.v_cache)]
-    c = abi.FaCache(s.k_cache.data_ptr(), s.v_cache.data_ptr(), s.k_scale.data_ptr(), s.v_scale.data_ptr(), P, page,
-                    Hkv, D, *strides, s.table_d.data_ptr(), s.table_d.stride(0), s.table_d.shape[1],
-                    s.lens_d.data_ptr(), s.cu_d.data_ptr(), len(s.lens))
+    return abi.FaCache(s.k_cache.data_ptr(), s.v_cache.data_ptr(), s.k_scale.data_ptr(), s.v_scale.data_ptr(), P,
+                       page, Hkv, D, *strides, s.table_d.data_ptr(), s.table_d.stride(0), s.table_d.shape[1],
+                       s.lens_d.data_ptr(), s.cu_d.data_ptr(), len(s.lens))
+
+
+def attend_into_nan(s: Setup, causal=True):
+    """The C entry point on outputs and a workspace that hold NaN: what is not written shows."""
+    c = c_cache(s)
     T = s.q.shape[0]
-    o = torch.full((T, s.H, D), math.nan, dtype=s.dtype, device="cuda")
+    o = torch.full((T, s.H, s.D), math.nan, dtype=s.dtype, device="cuda")
     lse = torch.full((T, s.H), math.nan, device="cuda")
     ws = torch.full((abi.cache_attention_workspace_bytes(c, s.H, T),), 0xFF, dtype=torch.uint8, device="cuda")
     err = abi.cache_attention(abi.dtype_code(s.dtype), c, s.q.data_ptr(), (s.q.stride(0), s.q.stride(1)), o.data_ptr(),
-                              lse.data_ptr(), ws.data_ptr(), T, s.H, 1 / math.sqrt(D), causal,
+                              lse.data_ptr(), ws.data_ptr(), T, s.H, 1 / math.sqrt(s.D), causal,
                               torch.cuda.current_stream().cuda_stream)
     assert err == 0
     torch.cuda.synchronize()
@@ -225,3 +229,29 @@ def test_lengths_next_to_two_to_the_31(new):
                                               return_lse=True)
     # A CTA's thread adds up to 2^31 / 128 / 148 / 2 tiles with 8 sums each in 32 bits, half a step each: 2^18.8 2^-24.
     assert bool(((lse - one_lse - math.log(entries)).abs() <= 2.0**-5).all()) and bool(torch.isfinite(o).all())
+
+
+def test_outputs_and_pages_that_are_their_inputs_are_refused():
+    """Blocks of one call would read what others write: one pool for keys and values, one tensor for q and o."""
+    s = Setup([20, 33], [4, 3], rot=128, seed=74)
+    kept = s.pages()
+    with pytest.raises(RuntimeError, match="different tensors"):
+        fused_attn.cache_append(s.k, s.v, s.k_cache, s.k_cache, s.k_scale, s.v_scale, s.table_d, s.lens_d, s.cu_d)
+    with pytest.raises(RuntimeError, match="different tensors"):
+        fused_attn.cache_append(s.k, s.v, s.k_cache, s.v_cache, s.k_scale, s.k_scale, s.table_d, s.lens_d, s.cu_d)
+    c = c_cache(s)
+    p = abi.FaAppend(s.k.data_ptr(), s.v.data_ptr(), (2 * 128, 128), (2 * 128, 128), s.q.data_ptr(), s.q.data_ptr(),
+                     (4 * 128, 128), 4, s.cos.data_ptr(), s.sin.data_ptr(), s.cos.shape[0], 128, 0)
+    T, code = s.q.shape[0], abi.dtype_code(s.dtype)
+    assert abi.cache_append(code, c, p, T) == abi.CUDA_ERROR_INVALID_VALUE
+    c.v = c.k
+    p.q_out = torch.empty_like(s.q).data_ptr()
+    assert abi.cache_append(code, c, p, T) == abi.CUDA_ERROR_INVALID_VALUE
+    ws = torch.empty(abi.cache_attention_workspace_bytes(c, 4, T), dtype=torch.uint8, device="cuda")
+    lse = torch.empty(T, 4, device="cuda")
+    assert abi.cache_attention(code, c, s.q.data_ptr(), (4 * 128, 128), s.q.data_ptr(), lse.data_ptr(),
+                               ws.data_ptr(), T, 4, 0.1, True) == abi.CUDA_ERROR_INVALID_VALUE
+    same_pages(s.pages(), kept)
+    # read only, one pool may hold both
+    s.v_cache, s.v_scale = s.k_cache, s.k_scale
+    check_attention(s)
