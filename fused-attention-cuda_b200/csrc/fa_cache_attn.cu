@@ -163,12 +163,13 @@ struct Finder {
 };
 
 // Bounded wait for a phase of this warp's copies; false when the time limit ran out (reported).
-__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, const CacheAttnArgs& a) {
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, const CacheView& c,
+                                          unsigned long long timeout_ns) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > a.timeout_ns) {
-      atomicOr(a.c.status, kStKFull);
+    if (globaltimer_ns() - t0 > timeout_ns) {
+      atomicOr(c.status, kStKFull);
       return false;
     }
   }
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
     uint32_t nans = 0;  // V's NaN that were taken out (nan_columns)
     for (int i = 0; i < n_runs; ++i) {
       const int stage = taken % L::kStages;
-      if (alive) alive = wait_copy(bars + 8 * stage, (taken / L::kStages) & 1, a);
+      if (alive) alive = wait_copy(bars + 8 * stage, (taken / L::kStages) & 1, c, a.timeout_ns);
       alive = __all_sync(0xffffffffu, alive);
       if (!alive) break;
       ++taken;
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, NT>::kPerSm)) fa_cache_de
     }
     // Copies in flight when a wait ran out still write to this block's memory.
     while (taken != sent) {
-      wait_copy(bars + 8 * (taken % L::kStages), (taken / L::kStages) & 1, a);
+      wait_copy(bars + 8 * (taken % L::kStages), (taken / L::kStages) & 1, c, max(a.timeout_ns, kMinDrainNs));
       ++taken;
     }
 

@@ -334,7 +334,7 @@ __device__ __forceinline__ void wait_out(uint32_t bar, uint32_t parity, const Wa
   if (mbar_try_wait(bar, parity)) return;
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer_ns() - t0 > w.timeout_ns) {
+    if (globaltimer_ns() - t0 > max(w.timeout_ns, kMinDrainNs)) {
       atomicOr(w.status, kStDrain);
       return;
     }

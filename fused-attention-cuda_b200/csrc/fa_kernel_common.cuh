@@ -165,9 +165,10 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, cons
 }
 
 // Exit-path wait for this CTA's own in-flight work (copies / MMAs); ignores the abort flag but is
-// still bounded.
+// still bounded, by kMinDrainNs at least: a short limit is for the other waits.
 __device__ __forceinline__ void wait_drain(uint32_t bar, uint32_t parity,
                                            unsigned long long timeout_ns) {
+  timeout_ns = timeout_ns < kMinDrainNs ? kMinDrainNs : timeout_ns;
   if (mbar_try_wait(bar, parity)) return;
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity)) {

@@ -51,6 +51,10 @@ cudaError_t read_and_clear_status(unsigned int* bits);
 // Time limit of each device-side wait (fa_set_wait_timeout_ns).
 unsigned long long wait_timeout_ns();
 
+// The least time that a block waits on its way out for its own copies and products in flight, which take
+// microseconds: it must not leave its shared and tensor memory to others before they have ended.
+constexpr unsigned long long kMinDrainNs = 1000000000ull;
+
 // Device-side status bits (which wait ran out).
 enum StatusBits : unsigned int {
   kStQFull = 1u << 0,    // MMA warp waiting for the Q tile

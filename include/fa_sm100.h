@@ -236,7 +236,8 @@ size_t fa_dtype_size(int dtype);
 int fa_last_device_error(unsigned int* detail);
 
 /* No counterpart in the reference: the time limit of each device-side wait, in nanoseconds
- * (default 2e9).  Used by the failure-detection tests to make an injected stall end quickly. */
+ * (default 2e9).  Used by the failure-detection tests to make an injected stall end quickly.  A
+ * block that gives up waits a second at least for its own copies and products in flight. */
 void fa_set_wait_timeout_ns(unsigned long long ns);
 
 /* No counterpart in the reference: test-only fault injection on the host side of the launch.

@@ -255,3 +255,25 @@ def test_outputs_and_pages_that_are_their_inputs_are_refused():
     # read only, one pool may hold both
     s.v_cache, s.v_scale = s.k_cache, s.k_scale
     check_attention(s)
+
+
+@pytest.mark.parametrize("new", [1, 40], ids=["token", "rows"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_wait_that_runs_out_ends_the_call_with_a_status(D, new):
+    """A limit of a nanosecond: the first wait that is not over at once runs out, with copies and products on their way.
+    The kernels end by themselves, the host reads a timeout (or, where no wait was that long, has the result), and the
+    next call is right."""
+    s = Setup([3000, 500], [new, new], D=D, page=64, seed=75)
+    s.attend()
+    assert fused_attn.last_device_error() == (0, 0)
+    fused_attn.set_wait_timeout_ns(1)
+    try:
+        o, lse = s.attend()
+        err, bits = fused_attn.last_device_error()
+    finally:
+        fused_attn.set_wait_timeout_ns(2_000_000_000)
+    assert err in (0, 702) and (bits != 0) == (err != 0)
+    assert not bits & (1 << 7 | 1 << 11)  # neither a drain that gave up nor a bad index
+    if err == 0:
+        check_attention(s, o=o, lse=lse)
+    check_attention(s)
