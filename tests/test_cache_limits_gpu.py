@@ -277,3 +277,61 @@ def test_a_wait_that_runs_out_ends_the_call_with_a_status(D, new):
     if err == 0:
         check_attention(s, o=o, lse=lse)
     check_attention(s)
+
+
+@pytest.mark.parametrize("chunk", [200, 500])
+def test_single_tokens_and_a_chunk_in_one_call(chunk):
+    """A server's step: the batch's mean decides which kernel serves it, on both sides of the choice."""
+    new = [1] * 40 + [chunk] + [1] * 23
+    lens = [17 * i % 300 + 1 for i in range(64)]
+    lens[40] = chunk + 333
+    s = Setup(lens, new, H=4, Hkv=1, D=64, page=32, rot=64, seed=70)
+    s.q = s.append()
+    check_attention(s)
+
+
+def test_a_step_under_torch_compile():
+    """The ops' schemas and fakes carry a compiled step: pages and scales are changed in place."""
+    s = Setup([90, 260], [3, 5], rot=128, seed=71, page=32)
+
+    def step(q, k, v, k_cache, v_cache, k_scale, v_scale, table, lens, cu, cos, sin):
+        q = fused_attn.cache_append(k, v, k_cache, v_cache, k_scale, v_scale, table, lens, cu, q=q, cos=cos, sin=sin)
+        return q, *fused_attn.cache_attention(q, k_cache, v_cache, k_scale, v_scale, table, lens, cu, return_lse=True)
+
+    want = s.pages()
+    q_want = ref.append(want, s.k, s.v, s.table.tolist(), s.lens, s.cu, q=s.q, cos=s.cos, sin=s.sin)
+    q, o, lse = torch.compile(step, backend="aot_eager", fullgraph=True)(
+        s.q, s.k, s.v, s.k_cache, s.v_cache, s.k_scale, s.v_scale, s.table_d, s.lens_d, s.cu_d, s.cos, s.sin)
+    same_pages(s.pages(), want)
+    assert torch.equal(q.cpu(), narrow(q_want, s.dtype))
+    s.q = q
+    check_attention(s, o=o, lse=lse)
+
+
+FIRST_CALL = """
+import sys
+import torch
+sys.path[:0] = [{tests!r}, {root!r}, {package!r}]
+import fused_attn
+from test_cache_gpu import Setup, check_attention
+for new, page in ((1, 32), (70, 32)):
+    s = Setup([90, 260], [new, new], rot=128, seed=72, page=page)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        q = s.append()
+        o, lse = s.attend(q=q)
+    g.replay()
+    torch.cuda.synchronize()
+    s.q = q
+    check_attention(s, o=o, lse=lse)
+    del g
+print("captured")
+"""
+
+
+def test_the_first_call_of_a_process_can_be_captured():
+    tests = Path(__file__).resolve().parent
+    code = FIRST_CALL.format(tests=str(tests), root=str(tests.parent),
+                             package=str(tests.parent / "fused-attention-cuda_b200"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
