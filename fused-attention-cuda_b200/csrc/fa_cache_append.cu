@@ -17,8 +17,8 @@
 // one of some 2^12 for bf16, 2^9 for fp16, 2^18 for e4m3) the sum is done over as an unevaluated
 // sum of two floats, both products exactly (their errors by fma), the sum's error by the two-sum of
 // Knuth, rounded to odd in 32 bits (the last bit set where it is inexact), so that the rounding that
-// follows is that of the exact value.  A page's scale is settled likewise, by bounds on its largest
-// magnitude.  13613 tokens of 32 + 8 + 8 heads of 128, where the memory needs 47 us: 64-bit arithmetic
+// follows is that of the exact value.  (Products below 2^-102, whose own error leaves a float's range, aside.)
+// A page's scale is settled likewise, by bounds on its largest magnitude.  13613 tokens of 32 + 8 + 8 heads of 128, where the memory needs 47 us: 64-bit arithmetic
 // 129 us (conversions, 16 a cycle), every sum as two floats or these bounds 105 to 113 us (q alone 54, k
 // and v 59, of which the rotation 36: instructions bound it, not the memory).
 #include <algorithm>

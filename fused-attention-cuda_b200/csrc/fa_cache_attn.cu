@@ -26,11 +26,12 @@
 // leave fp32 partials, which a second kernel, launched while the first runs, merges.
 //
 // What bounds it: 64 sequences of 97 to 8191 keys of 8 heads of 128, one token of 32 heads each, 554 MB,
-// take 113 us (84 at the measured copy rate), one of 131071 keys 63 us (41): about 6.5 TB/s and some
-// 15 us that do not depend on the length (the table's and the first page's latency, the merge).  5 tokens
-// of 32 heads, 20 rows, take 71 us for 153 MB: the products' instructions and the softmax of 24 rows.
-// 777 keys take 12.6 us, two kernels of some 7 us that are chains of latencies.  One sequence's tables
-// were looked up by each run before (142 us for the first of these), rows as M (171 us).
+// take 111 us (84 at the measured copy rate), one of 131071 keys, 269 MB, 63 us (41): 5.9 TB/s between the
+// two and some 18 us that do not depend on the length (the table's and the first page's latency, the merge);
+// the kernel alone reads 5.2 to 5.4 TB/s.  5 tokens of 32 heads, 20 rows, take 71 us for 153 MB: the
+// products' instructions and the softmax of 24 rows.  777 keys take 12.6 us, two kernels of some 7 us that
+// are chains of latencies.  One sequence's tables were looked up by each run before (142 us for the first of
+// these), rows as M (171 us).
 #include <algorithm>
 #include <cmath>
 
@@ -818,7 +819,8 @@ cudaError_t launch_t(const CacheAttnArgs& a, cudaStream_t stream) {
 // Query rows of a tile in eights, by a sequence's mean; 0: the kernel on tcgen05 (fa_cache_tile.cu).
 // 32 sequences of 500 to 4003 keys, rows: this kernel / the other, us.  32 + 8 heads of 128: 16: 58 / 107,
 // 32: 93 / 110, 36: 157 / 112, 64: 172 / 113; 16 + 4 heads of 64: 32: 37 / 52, 36: 52 / 52, 64: 55 / 53,
-// 128: 99 / 58.
+// 128: 99 / 58.  Those batches are even.  For a skewed one the mean is a poor rule: 63 single tokens over
+// 500 to 4003 keys and a chunk of 200 (500) over 4000 take 179 (273) us in one call, 137 (151) in two.
 int row_eights(int H, int Hkv, int T, int n_seqs) {
   const long long rows = static_cast<long long>(T) * (H / Hkv);
   return rows > 32ll * n_seqs ? 0 : static_cast<int>(std::max(1ll, (rows + 8ll * n_seqs - 1) / (8ll * n_seqs)));

@@ -25,15 +25,21 @@
 // P_g (fp16) overwrites the first 32 of its own, O_g takes D.  While a group exponentiates one half
 // the products of the other are under way.
 //
-// What bounds it: 2048 new tokens of 32 heads over 16384 keys of 8 heads of 128 take 650 us, 790 TFLOP/s,
+// What bounds it: 2048 new tokens of 32 heads over 16384 keys of 8 heads of 128 take 644 us, 800 TFLOP/s,
 // about 4700 cycles for 256 rows by 128 keys where the products alone need 2048.  A group's softmax of
 // 64 keys takes 2250 cycles (maximum 500, exponentials 1000, the rest loads, stores and hand-offs), and
 // the products, S reading both operands from shared memory and sharing it with the conversion's stores,
-// 3400 of the 4700.  Measured and not kept: one S of 128 columns (a group waits for its products, 5900
-// cycles), four softmax groups with a row's maximum handed from half to half (650 us), a quarter of the
-// exponentials as polynomials on the FMA pipes (638 us), products issued by one lane of a diverged warp
-// (738 us: operands have to move to uniform registers one by one).  Taking V's NaN out of the tiles on the
-// diagonal is 10 of the 650.
+// 3400 of the 4700.  8 sequences of 1 to 801 new tokens over 300 to 6001 keys of 4 heads take 157 us, where a
+// change of tile, 24000 cycles from product to product instead of 4700, weighs most: a CTA has 26 units of 2.1
+// tiles on average and of 7 at most, and units alone are dealt evenly.
+//
+// Measured and not kept: four softmax groups with a row's maximum handed from half to half (650 us), a
+// quarter of the exponentials as polynomials on the FMA pipes (638 us), products issued by one lane of a
+// diverged warp (738 us: operands have to move to uniform registers one by one).  One S of 128 columns, one
+// warp for all products and one group of warps that converts K and V by way of e4m3 tiles in shared memory took
+// 611 us for the first of these calls on the GPU of the 644, and 184 for the second where this takes 156; with S
+// in halves and conversion through registers, 614 and 165.  Of the 33 us, 10 go into taking V's NaN out of
+// the tiles on the diagonal.
 #include <algorithm>
 #include <cmath>
 

@@ -144,8 +144,10 @@ def cache_append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale
     Scales are powers of two, the least that hold a page's largest magnitude (448 * scale).  A page
     that held earlier tokens keeps them: its scale only grows, and where it does they are rounded
     to the new step.  Values that are not finite are stored as NaN.  A call must not append to
-    one page twice (two sequences, or two entries of the table).  Pages, lengths, offsets and positions live on the device and are
-    checked there: what is out of range is skipped and reported by ``last_device_error`` as (1, bits).
+    one page twice (two sequences, or two entries of the table), and keys and values need tensors
+    of their own.  Pages, lengths, offsets and positions live on the device and are checked there:
+    what is out of range, a token past the table's room among it, is skipped and reported by
+    ``last_device_error`` as (1, bits).
     """
     _require_ext()
     out = torch.ops.fused_attn.cache_append(q, k, v, k_cache, v_cache, k_scale, v_scale,
@@ -167,7 +169,9 @@ def cache_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor
 
     ``k_scale`` is positive and finite; ``v_scale`` lies in [2^-64, 2^120], which ``cache_append`` keeps
     to, and within 2^96 from page to page of a sequence.  A value scale outside counts as the nearest
-    end and is reported by ``last_device_error`` as (1, bits)."""
+    end and is reported by ``last_device_error`` as (1, bits); a scale that is NaN makes o and lse of the
+    queries that see its page NaN.  Weights are fp16, relative to a query's largest weight times value
+    scale: next to it a page with 2^-20 of its scale counts with 4 bits in o, below 2^-25 not at all."""
     _require_ext()
     o, lse = torch.ops.fused_attn.cache_attention(q, k_cache, v_cache, k_scale, v_scale,
                                                   block_table, seq_lens, cu_seqlens,
@@ -205,7 +209,9 @@ def set_debug_overrides(block_m: int = 0, block_n: int = 0) -> None:
 
 def last_device_error() -> tuple[int, int]:
     """(cudaError_t, cause bits) of the kernel's bounded waits since the previous call;
-    synchronises the current device.  cudaErrorLaunchTimeout (702) means a wait ran out."""
+    synchronises the current device.  cudaErrorLaunchTimeout (702) means a wait ran out;
+    cudaErrorInvalidValue (1) with bit 11 that ``cache_append`` or ``cache_attention`` met a page,
+    length, offset, position or value scale out of range."""
     _require_ext()
     return abi.last_device_error()
 

@@ -121,7 +121,8 @@ size_t fa_noalloc_scratch_bytes(void);
  * kv head D e4m3 values a token; k_scale / v_scale [num_pages, Hkv] (fp32, contiguous) hold one
  * scale for each page and kv head, value = e4m3 * scale.  fa_cache_append writes powers of two in
  * [2^-64, 2^120].  fa_cache_attention takes any positive finite k_scale, and any v_scale in that
- * range; the value scales of one sequence and kv head lie within 2^96 of each other.  A value scale
+ * range; the value scales of one sequence and kv head lie within 2^96 of each other, else weights may be
+ * missing from the denominator (a page of zeros has 2^-64: values beside it stay below 2^40).  A value scale
  * outside of [2^-64, 2^120] counts as the nearest end and is reported like a bad page.  A scale that is NaN
  * makes o and lse of the queries that see a key of its page NaN, and of no others.  k_strides / v_strides
  * are the byte strides of (page, kv head, token), positive multiples of 16; d is contiguous.
@@ -230,8 +231,9 @@ size_t fa_dtype_size(int dtype);
  * status word, the kernel drains its own copies, frees its tensor memory and exits normally.
  * This call synchronises the current device, returns cudaErrorLaunchTimeout (702) if any
  * launch since the previous call timed out (cudaErrorAssert (710) instead when a build made
- * with -DFA_DEBUG_CHECKS found an index out of range; else the device's sticky error, or
- * cudaSuccess),
+ * with -DFA_DEBUG_CHECKS found an index out of range; cudaErrorInvalidValue (1), with bit 11 in
+ * *detail, when nothing worse happened and fa_cache_append or fa_cache_attention met a page, length,
+ * offset, position or value scale out of range; else the device's sticky error, or cudaSuccess),
  * stores the cause bits in *detail when detail != NULL, and clears the status word. */
 int fa_last_device_error(unsigned int* detail);
 
