@@ -335,3 +335,48 @@ def test_the_first_call_of_a_process_can_be_captured():
                              package=str(tests.parent / "fused-attention-cuda_b200"))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("new", [1, 5, 40], ids=["token", "draft", "rows"])
+def test_a_query_that_is_not_finite_stays_in_its_row(new, dtype):
+    s = Setup([300, 77], [new, new], D=64, page=32, seed=76, dtype=dtype)
+    want = ref.attention(s.pages(), s.q, s.table.tolist(), s.lens, s.cu)
+    s.q[0, 1, 7] = math.nan
+    s.q[new, 0, 3] = math.inf
+    o, lse = s.attend()
+    hit = torch.zeros(2 * new, s.H, dtype=torch.bool)
+    hit[0, 1] = hit[new, 0] = True
+    o, lse = o.cpu().double(), lse.cpu().double()
+    assert bool(torch.isnan(o[hit]).all()) and bool(torch.isnan(lse[hit]).all())
+    half = torch.finfo(dtype).eps / 2
+    room = want.o_room * (1 + half) + want.o.abs() * half + 1e-7
+    assert bool(((lse - want.lse).abs() <= want.lse_room)[~hit].all())
+    assert bool(((o - want.o).abs() <= room)[~hit].all())
+
+
+def test_calls_at_once_on_three_streams():
+    """Both attention kernels, appends and the forward side by side: the bits of the calls made alone."""
+    batches = [Setup([2000, 900], [300, 170], H=8, Hkv=2, page=64, rot=128, seed=77),
+               Setup([1500, 40, 333], [1, 1, 1], H=8, Hkv=2, page=16, rot=128, seed=78),
+               Setup([600] * 6, [600] * 6, H=4, Hkv=2, D=64, page=32, rot=64, seed=79, dtype=torch.float16)]
+    x = torch.randn(2, 4, 512, 128, device="cuda").half()
+    alone = []
+    for s in batches:
+        q = s.append()
+        alone.append((q, *s.attend(q=q), fused_attn.forward(x, x, x)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    got = [[] for _ in batches]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(8):
+        for s, st, out in zip(batches, streams, got):
+            with torch.cuda.stream(st):
+                q = s.append()
+                out.append((q, *s.attend(q=q), fused_attn.forward(x, x, x)))
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, got):
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert fused_attn.last_device_error() == (0, 0)
