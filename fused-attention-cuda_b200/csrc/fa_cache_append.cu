@@ -576,7 +576,7 @@ __device__ __forceinline__ void rotate_q(const AppendArgs& p, const Grid& g, lon
   if (s < c.n_seqs) {
     const SeqInfo q = seq_info<true>(c, s);
     if (t >= q.t0 && t < q.t0 + q.n) {  // else a row of no sequence
-      pos = q.len - q.n + t - q.t0;
+      pos = q.len - q.n + (t - q.t0);  // below len, which may be any int
       if (pos < 0 || pos >= p.table_rows) {
         report_cache_index(c);
         pos = -1;

@@ -149,6 +149,17 @@ def test_tokens_past_the_table_are_not_stored(n, over, page, rot):
     check_append(s, errors=BAD_INDEX)
 
 
+@pytest.mark.parametrize("n", [1, 40], ids=["token", "rows"])
+def test_the_largest_length_that_an_int_holds(n):
+    """Its tokens have neither a page nor angles; the other sequence is stored."""
+    s = Setup([70, 128], [30, n], page=32, seed=80, rot=128)
+    s.lens[1] = 2**31 - 1
+    s.lens_d[1] = 2**31 - 1
+    check_append(s, errors=BAD_INDEX)
+    _, lse = s.attend()
+    assert fused_attn.last_device_error() == BAD_INDEX and bool(torch.isfinite(lse).all())
+
+
 @pytest.mark.parametrize("S,at,value", [(4, 4, 2), (4, 4, 0), (4, 4, -1), (4, 4, 10**6), (4, 3, -1), (4, 3, 10**6),
                                         (4, 2, -5), (30, 17, -1), (30, 17, 10**6), (45, 45, 3), (45, 45, -1)])
 def test_an_offset_out_of_range_costs_its_sequences_only(S, at, value):
